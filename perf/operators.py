@@ -190,7 +190,7 @@ def _plain_widen(four, c):
 
 def _plain_weights(w, fmt):
     """Values of the weights: blocks run along the input channels of one tap; f4 has one scale per filter."""
-    return _plain_widen(_plain_narrow(w, fmt, w.abs().amax((1, 2, 3)) / (6.0 * 448.0) if fmt == "f4" else 1.0), w.shape[1])
+    return _plain_widen(_plain_narrow(w, fmt, w.abs().amax((1, 2, 3)) / w.new_tensor(6.0 * 448.0) if fmt == "f4" else 1.0), w.shape[1])
 
 
 def _plain_act(v, act):
@@ -423,7 +423,7 @@ def exact(case, seed):
     x = s["x"]
     if case["kind"] in ("narrow", "widen"):
         return _exact_narrow(x, fmt, s["x_scale"])
-    weights = lambda w: _exact_narrow(w, fmt, (w.abs().amax((1, 2, 3)) / (6.0 * 448.0)) if fmt == "f4" else 1.0)  # noqa: E731
+    weights = lambda w: _exact_narrow(w, fmt, (w.double().abs().amax((1, 2, 3)) / (6.0 * 448.0)).float() if fmt == "f4" else 1.0)  # noqa: E731
     x = _exact_narrow(x, fmt, s["x_scale"])
     if case["kind"] == "product":
         return _exact_conv(x, weights(s["w"]), s["b"], case["k"], case["stride"], case["act"])
