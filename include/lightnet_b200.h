@@ -49,14 +49,15 @@ enum ln_status {
 /* F32ActivationKind (lightnet-cuda/src/lib.rs:23-55), hot-path subset. */
 enum ln_activation { LN_ACT_LINEAR = 0, LN_ACT_LOGISTIC = 1, LN_ACT_LEAKY = 2, LN_ACT_MISH = 3, LN_ACT_SWISH = 4, LN_ACT_RELU = 5 };
 
-enum ln_dtype { LN_F32 = 0, LN_Q8 = 1, LN_I32 = 2, LN_F8 = 3, LN_F16 = 4 };
+enum ln_dtype { LN_F32 = 0, LN_Q8 = 1, LN_I32 = 2, LN_F8 = 3, LN_F16 = 4, LN_F4 = 5, LN_MX4 = 6 /* the two 4-bit types, see below */ };
 
 /* What a reduced-precision convolution writes. */
 enum ln_conv_out {
     LN_OUT_Q = 0,   /* same 8-bit storage type as the input, requantised with y_scale */
     LN_OUT_F32 = 1, /* f32 NCHW: the convolution feeding a detection head (ConvPrecision::NoLowPrecision policy,
                        lightnet-cuda/src/lib.rs:161, runtime/types.rs:146-170) */
-    LN_OUT_ACC = 2  /* raw int32 accumulators, NCHW (parity checks only; int8 inputs only) */
+    LN_OUT_ACC = 2, /* raw int32 accumulators, NCHW (parity checks only; int8 inputs only) */
+    LN_OUT_F16 = 3  /* binary16 NHWC (4-bit convolutions only) */
 };
 
 /* ---- context ------------------------------------------------------------------- */
@@ -88,6 +89,10 @@ int32_t ln_tensor_zeros_f32(ln_ctx* ctx, const int64_t shape[4], ln_tensor** out
 int32_t ln_tensor_download_f32(ln_ctx* ctx, const ln_tensor* t, float* host, int64_t count);
 int32_t ln_tensor_shape(const ln_tensor* t, int64_t shape[4]);
 int32_t ln_tensor_dtype(const ln_tensor* t);
+/* Device address of an f32 or binary16 tensor's first value, and the distance in values between neighbours along each axis, for a
+   program that hands the tensor to another library on the same GPU.  The handle keeps the memory; work on another stream has to be
+   ordered behind the ctx stream (ln_ctx_stream) by the caller, and in front of it again before the handle is released. */
+int32_t ln_tensor_device_data(const ln_tensor* t, void** data, int64_t strides[4]);
 int32_t ln_tensor_retain(ln_tensor* t);
 int32_t ln_tensor_release(ln_tensor* t);
 
@@ -213,6 +218,38 @@ int32_t ln_shortcut_fit_f16(ln_ctx* ctx, const ln_tensor* x, int64_t batch, cons
 int32_t ln_shortcut_add_act_f16(ln_ctx* ctx, const ln_tensor* a, const ln_tensor* b, int32_t activation, ln_tensor** out);
 int32_t ln_channel_affine_act_f16(ln_ctx* ctx, const ln_tensor* x, const ln_tensor* scale, const ln_tensor* bias, int64_t channels,
                                   int64_t channel_stride, int32_t activation, ln_tensor** out);
+
+/* ---- microscaled 4-bit tensors -------------------------------------------------------------- */
+/* (The reference emulates such a product on its CUDA cores, lightnet-cuda-oxide/src/kernels/gemm_fp4.rs:1-12, for its own matrix layers;
+   here it is the third storage type of the convolutions, with the set of operators that the 8-bit types have.)
+   Elements are E2M1: 0, 0.5, 1, 1.5, 2, 3, 4, 6 and a sign.  A block is consecutive channels of one pixel (of one tap of one filter
+   for weights) that share a scale:
+     LN_F4   16 channels, block scale s in E4M3, and one f32 scale g per tensor (ln_tensor_scale; per filter for weights):
+             s = e4m3(amax / (6 g)), d = s * g, code = e2m1(x / d), value = code * d.  s = 0 gives codes 0.
+             g = amax / (6 * 448) of a calibration run uses the whole range of s.
+     LN_MX4  32 channels, block scale d = 2^e, e = max(floor(log2(amax)) - 2, -127), code = e2m1(x / d), value = code * d (the
+             ranges of the OCP microscaling format).  There is no other scale: `scale` arguments have to be 1.
+   Divisions and products are binary32 operations; e4m3 and e2m1 round to nearest even and saturate (an infinite value becomes the
+   largest of its block, which is infinite again for LN_MX4).  A NaN makes its whole block NaN.  f32 and binary16 NHWC tensors
+   narrow to the same codes.  Storage is NHWC, two codes per byte, channels padded to 64, block scales behind the codes. */
+int32_t ln_tensor_narrow_f4(ln_ctx* ctx, const ln_tensor* t, float scale, int32_t dtype, ln_tensor** out);
+/* The values, as f32 (dtype LN_F32) or rounded once to binary16 (LN_F16). */
+int32_t ln_tensor_widen_f4(ln_ctx* ctx, const ln_tensor* t, int32_t dtype, ln_tensor** out);
+/* Codes in NCHW order, one per byte (bit 3 = sign), and block scales [batch, ceil(channels / block), height, width] as they are
+   stored (E4M3, or e + 127 with 255 = NaN).  Counts are checked against the tensor's. */
+int32_t ln_tensor_download_f4(ln_ctx* ctx, const ln_tensor* t, uint8_t* host_codes, int64_t code_count, uint8_t* host_scales, int64_t scale_count);
+/* f32 [filters, channels * k * k] weights -> 4 bits; LN_F4: g = max|w| / (6 * 448) per filter.  Released with ln_conv_weights_release. */
+int32_t ln_conv_weights_f4(ln_ctx* ctx, const ln_tensor* weights_f32, int64_t filters, int64_t channels, int64_t kernel_size,
+                           int32_t dtype, ln_conv_weights** out);
+/* acc = sum of the products of codes and block scales (binary32 sums), v = fma(acc, x.scale * w.scale[f], bias[f]), a = act(v).
+   LN_OUT_F32 stores a in NCHW, LN_OUT_F16 in binary16 NHWC, LN_OUT_Q narrows a to the input's 4-bit type again with y_scale.
+   A 1x1 convolution of [tokens, channels, 1, 1] is the matrix product of tokens and weights.  groups and dilation must be 1.
+   The call does not wait for the GPU: should the kernel give up a wait, ln_sync, a download or the next 4-bit call returns LN_ERR_TIMEOUT. */
+int32_t ln_conv2d_bias_act_f4(ln_ctx* ctx, const ln_tensor* x, const ln_conv_weights* weights, const ln_tensor* bias,
+                              const int64_t output_shape[4], int64_t channels, int64_t input_height, int64_t input_width,
+                              int64_t filters, int64_t kernel_size, int64_t stride_x, int64_t stride_y, int64_t dilation,
+                              int64_t padding, int64_t groups, int32_t activation, float y_scale, int32_t out_kind,
+                              ln_tensor** out);
 
 /* ---- [yolo] decode + NMS on the device ---------------------------------------------- */
 /* Optional device path for decode_network_detections (lightnet-train/src/detect.rs:113-244): the Rust shim

@@ -18,8 +18,8 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 # the in-tree library; LIGHTNET_B200_LIB names another build of it (e.g. one compiled with extra -D switches for an A/B run)
 LIB_PATH = os.environ.get("LIGHTNET_B200_LIB") or os.path.join(_HERE, "liblightnet_b200.so")
 
-LN_F32, LN_Q8, LN_I32, LN_F8, LN_F16 = 0, 1, 2, 3, 4
-LN_OUT_Q, LN_OUT_F32, LN_OUT_ACC = 0, 1, 2
+LN_F32, LN_Q8, LN_I32, LN_F8, LN_F16, LN_F4, LN_MX4 = 0, 1, 2, 3, 4, 5, 6
+LN_OUT_Q, LN_OUT_F32, LN_OUT_ACC, LN_OUT_F16 = 0, 1, 2, 3
 ACTIVATIONS = {"linear": 0, "logistic": 1, "leaky": 2, "mish": 3, "swish": 4, "relu": 5}
 STATUS = {0: "ok", 1: "shape", 2: "cuda", 3: "timeout", 4: "unsupported", 5: "argument", 6: "parse"}
 
@@ -85,6 +85,7 @@ SYMBOLS = {
     "ln_tensor_download_f32": (C.c_int32, [_VP, _VP, _VP, C.c_int64]),
     "ln_tensor_shape": (C.c_int32, [_VP, _I64P]),
     "ln_tensor_dtype": (C.c_int32, [_VP]),
+    "ln_tensor_device_data": (C.c_int32, [_VP, _PP, _I64P]),
     "ln_tensor_retain": (C.c_int32, [_VP]),
     "ln_tensor_release": (C.c_int32, [_VP]),
     "ln_conv2d_f32": (C.c_int32, [_VP, _VP, _VP, _I64P] + [C.c_int64] * 10 + [_PP]),
@@ -158,6 +159,11 @@ SYMBOLS = {
     "ln_shortcut_fit_f16": (C.c_int32, [_VP, _VP, C.c_int64, _I64P, _PP]),
     "ln_shortcut_add_act_f16": (C.c_int32, [_VP, _VP, _VP, C.c_int32, _PP]),
     "ln_channel_affine_act_f16": (C.c_int32, [_VP, _VP, _VP, _VP, C.c_int64, C.c_int64, C.c_int32, _PP]),
+    "ln_tensor_narrow_f4": (C.c_int32, [_VP, _VP, C.c_float, C.c_int32, _PP]),
+    "ln_tensor_widen_f4": (C.c_int32, [_VP, _VP, C.c_int32, _PP]),
+    "ln_tensor_download_f4": (C.c_int32, [_VP, _VP, _VP, C.c_int64, _VP, C.c_int64]),
+    "ln_conv_weights_f4": (C.c_int32, [_VP, _VP, C.c_int64, C.c_int64, C.c_int64, C.c_int32, _PP]),
+    "ln_conv2d_bias_act_f4": (C.c_int32, [_VP, _VP, _VP, _VP, _I64P] + [C.c_int64] * 10 + [C.c_int32, C.c_float, C.c_int32, _PP]),
     "ln_debug_score_key_error": (C.c_int32, [_VP, C.c_float, C.c_float, C.c_float, C.c_float, C.c_int32, C.c_int32, C.POINTER(C.c_uint32)]),
     "ln_ctx_debug_cycles": (C.c_int32, [_VP, _I64P]),
     "ln_debug_net_replays": (C.c_int64, [_VP]),
@@ -226,6 +232,18 @@ class Tensor:
     @property
     def scale(self):
         return float(_lib.ln_tensor_scale(self.h))
+
+    @property
+    def __cuda_array_interface__(self):
+        """f32 and binary16 tensors for other libraries on the same GPU (`torch.as_tensor(t, device="cuda")` shares the memory and keeps
+        the handle); order their work behind the backend's stream."""
+        dtype = self.dtype
+        if dtype not in (LN_F32, LN_F16):
+            raise AttributeError("only f32 and binary16 tensors have an array interface")
+        size, p, s = 4 if dtype == LN_F32 else 2, C.c_void_p(), (C.c_int64 * 4)()
+        self.backend._check(_lib.ln_tensor_device_data(self.h, C.byref(p), s))
+        return {"shape": self.shape, "typestr": "<f%d" % size, "data": (p.value, False), "strides": tuple(size * v for v in s), "version": 3,
+                "stream": int(self.backend.stream)}
 
 
 class ConvWeights:
@@ -502,6 +520,33 @@ class B200Backend:
 
     def shortcut_add_act_q(self, a, b, activation, y_scale):
         return self._out(self.lib.ln_shortcut_add_act_q, a.h, b.h, _act(activation), float(y_scale))
+
+    # ---- microscaled 4-bit tensors ----------------------------------------------------------------
+    def narrow_f4(self, t, scale=1.0, dtype=LN_F4):
+        """An f32 or binary16 tensor in 4 bits (LN_F4: blocks of 16 with the tensor scale `scale`; LN_MX4: blocks of 32, scale 1)."""
+        return self._out(self.lib.ln_tensor_narrow_f4, t.h, float(scale), dtype)
+
+    def widen_f4(self, t, dtype=LN_F32):
+        return self._out(self.lib.ln_tensor_widen_f4, t.h, dtype)
+
+    def download_f4(self, t):
+        """Codes [n, c, h, w], one per byte, and block scales [n, blocks, h, w] as they are stored."""
+        n, c, h, w = t.shape
+        codes = np.empty((n, c, h, w), np.uint8)
+        scales = np.empty((n, -(-c // (32 if t.dtype == LN_MX4 else 16)), h, w), np.uint8)
+        self._check(self.lib.ln_tensor_download_f4(self.ctx, t.h, _ptr(codes), codes.size, _ptr(scales), scales.size))
+        return codes, scales
+
+    def conv_weights_f4(self, weights, filters, channels, kernel_size, dtype=LN_F4):
+        h = C.c_void_p()
+        self._check(self.lib.ln_conv_weights_f4(self.ctx, weights.h, filters, channels, kernel_size, dtype, C.byref(h)))
+        return ConvWeights(self, h)
+
+    def conv2d_bias_act_f4(self, x, weights, bias, output_shape, channels, input_height, input_width, filters, kernel_size,
+                           stride_x, stride_y, dilation, padding, groups, activation, y_scale=1.0, out_kind=LN_OUT_Q):
+        return self._out(self.lib.ln_conv2d_bias_act_f4, x.h, weights.h, bias.h, _shape4(output_shape), channels, input_height,
+                         input_width, filters, kernel_size, stride_x, stride_y, dilation, padding, groups, _act(activation),
+                         float(y_scale), out_kind)
 
     # ---- [yolo] decode + NMS ---------------------------------------------------------------------
     @staticmethod

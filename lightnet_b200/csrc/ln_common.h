@@ -60,7 +60,9 @@ struct ln_tensor {
     size_t bytes = 0;
     ln_tensor* parent = nullptr;         // keeps the owner of a view alive
     int64_t cstride = 0;                 // 8-bit and binary16 NHWC tensors: bytes between consecutive pixels
-    float scale = 1.0f;                  // 8-bit tensors: value = code * scale
+    float scale = 1.0f;                  // 8-bit tensors: value = code * scale; LN_F4: value = code * block scale * scale
+    void* sf = nullptr;                  // 4-bit tensors: block scales, sf_stride bytes per pixel (behind the codes in the same block)
+    int64_t sf_stride = 0;
     int64_t count() const { return n * c * h * w; }
 };
 
@@ -72,6 +74,7 @@ struct ln_conv_weights {
     void* w = nullptr;              // [fpad][k][k][cpad] 8-bit codes
     float* wscale = nullptr;        // [fpad] per-filter scale (device)
     std::vector<float> h_wscale;    // host copy
+    void* sf = nullptr;             // 4-bit weights: block scales as the tensor cores read them (ln_f4.h)
     float max_l1 = 0.0f;            // max over filters of the sum of |code| (bounds the int8 accumulators)
     float max_scale = 0.0f;         // largest per-filter scale
     void* w_oihw = nullptr;         // [filters][channels][k][k] codes in the reference's weight order (SIMT path)

@@ -1,0 +1,124 @@
+// Storage of the microscaled 4-bit types, shared by their operators.
+//
+// A tensor is NHWC: per pixel two codes per byte (channel 2i in the low nibble), channels padded to 64, so that a pixel is a multiple
+// of the 32 bytes that one tensor-core instruction consumes; behind the codes of all pixels the block scales, sf_stride bytes per
+// pixel.  Codes and scales of the padding up to 64 channels are zero; scale bytes behind those are never read.
+#pragma once
+
+#include <cstdint>
+
+#include "ln_common.h"
+
+inline bool ln_is_f4(int dtype) { return dtype == LN_F4 || dtype == LN_MX4; }
+inline int ln_f4_block(int dtype) { return dtype == LN_MX4 ? 32 : 16; }
+inline int64_t ln_f4_cstride(int64_t c) { return ln_round_up(c, 64) / 2; }
+// The scales of up to 256 channels (the channels of one k-block of the product) are read with one access of 4, 8 or 16 bytes.
+inline int64_t ln_f4_sf_stride(int dtype, int64_t c) {
+    const int64_t need = ln_round_up(c, 64) / ln_f4_block(dtype);
+    if (dtype == LN_MX4) return c <= 128 ? 4 : ln_round_up(need, 8);
+    return c <= 64 ? 4 : (c <= 128 ? 8 : ln_round_up(need, 16));
+}
+
+// Weights: codes [filters][k * k][cstride]; block scales in the order in which the tensor cores take them.  The k range is cut into
+// k-blocks of `bk` bytes of one tap (the last one of a tap may be shorter); per 128 filters and k-block there are `words` groups of
+// 512 bytes: [32 filters][4 groups of 32 filters][4 scale bytes], so that filter f has the word ((f % 32) * 4 + f / 32 % 4).
+// LN_F4: a word holds the scales of 64 channels (one instruction); LN_MX4: of 128 (two).
+struct ln_f4_kblocks {
+    int bk, cblocks, words;
+};
+inline ln_f4_kblocks ln_f4_kblocks_of(int dtype, int64_t c) {
+    const int64_t cstride = ln_f4_cstride(c);
+    ln_f4_kblocks k;
+    k.bk = cstride <= 32 ? 32 : (cstride <= 64 ? 64 : 128);
+    k.cblocks = (int)((cstride + k.bk - 1) / k.bk);
+    k.words = dtype == LN_MX4 ? (k.bk + 63) / 64 : k.bk / 32;
+    return k;
+}
+constexpr int64_t kF4FilterPad = 256;  // filters that the scales of weights are padded to (zeros): the widest filter tile
+
+#ifdef __CUDACC__
+// ---- the number formats -----------------------------------------------------------------------------------------------------------
+
+// max that hands a NaN on
+__device__ __forceinline__ float ln_max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+// x >= 0 -> E4M3 (nearest even, saturating at 448; NaN is 0x7F) and back
+__device__ __forceinline__ uint32_t ln_e4m3_of(float x) {
+    uint16_t d;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(d) : "f"(0.0f), "f"(x));  // second source -> low byte
+    return d & 0xFFu;
+}
+__device__ __forceinline__ float ln_e4m3_value(uint32_t code) {
+    uint32_t h;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((uint16_t)code));
+    return __half2float(__ushort_as_half((unsigned short)(h & 0xFFFFu)));
+}
+// 2^(code - 127): 0 is 2^-127, 255 is NaN
+__device__ __forceinline__ float ln_e8m0_value(uint32_t code) {
+    return code == 255u ? __uint_as_float(0x7FC00000u) : (code ? __uint_as_float(code << 23) : __uint_as_float(0x00400000u));
+}
+// eight values -> eight E2M1 codes (nearest even, saturating at 6), the first in the lowest nibble
+__device__ __forceinline__ uint32_t ln_e2m1x8(float a, float b, float c, float d, float e, float f, float g, float h) {
+    uint32_t r;
+    asm("{\n\t.reg .b8 p, q, r, s;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 p, %2, %1;\n\t"  // first source -> high nibble
+        "cvt.rn.satfinite.e2m1x2.f32 q, %4, %3;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 r, %6, %5;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 s, %8, %7;\n\t"
+        "mov.b32 %0, {p, q, r, s};\n\t}"
+        : "=r"(r)
+        : "f"(a), "f"(b), "f"(c), "f"(d), "f"(e), "f"(f), "f"(g), "f"(h));
+    return r;
+}
+// eight codes -> four binary16 pairs, in order
+__device__ __forceinline__ void ln_e2m1x8_to_h2(uint32_t codes, uint32_t (&h)[4]) {
+    asm("{\n\t.reg .b8 p, q, r, s;\n\t"
+        "mov.b32 {p, q, r, s}, %4;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %0, p;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %1, q;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %2, r;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %3, s;\n\t}"
+        : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
+        : "r"(codes));
+}
+
+// Block scale: its stored byte and the binary32 factor d of the codes (g is not used for LN_MX4).
+template <int FMT>
+__device__ __forceinline__ uint32_t ln_f4_scale_of(float amax, float six_g) {
+    if (FMT == LN_F4) return ln_e4m3_of(__fdiv_rn(amax, six_g));
+    const uint32_t bits = __float_as_uint(amax), field = (bits >> 23) & 0xFFu;
+    if (bits > 0x7F800000u) return 255u;
+    return field > 2u ? field - 2u : 0u;  // e + 127 = (field - 127) - 2 + 127
+}
+template <int FMT>
+__device__ __forceinline__ float ln_f4_factor(uint32_t scale, float g) {
+    return FMT == LN_F4 ? __fmul_rn(ln_e4m3_value(scale), g) : ln_e8m0_value(scale);
+}
+
+// The codes of one block: B = 16 (LN_F4) or 32 (LN_MX4) values -> B / 8 words.  Returns the scale byte.
+template <int FMT>
+__device__ __forceinline__ uint32_t ln_f4_quantise(const float* x, float g, float six_g, uint32_t* codes) {
+    constexpr int B = FMT == LN_F4 ? 16 : 32;
+    float amax = 0.0f;
+#pragma unroll
+    for (int i = 0; i < B; ++i) amax = ln_max_nan(amax, fabsf(x[i]));
+    const uint32_t scale = ln_f4_scale_of<FMT>(amax, six_g);
+    float t[B];
+    if (FMT == LN_F4) {
+        const float d = ln_f4_factor<FMT>(scale, g);
+#pragma unroll
+        for (int i = 0; i < B; ++i) t[i] = scale ? __fdiv_rn(x[i], d) : 0.0f;
+    } else {
+        const float inv = __uint_as_float((254u - (scale > 253u ? 253u : scale)) << 23);  // 2^-e, exact
+#pragma unroll
+        for (int i = 0; i < B; ++i) t[i] = __fmul_rn(x[i], inv);
+    }
+#pragma unroll
+    for (int w = 0; w < B / 8; ++w)
+        codes[w] = ln_e2m1x8(t[8 * w], t[8 * w + 1], t[8 * w + 2], t[8 * w + 3], t[8 * w + 4], t[8 * w + 5], t[8 * w + 6], t[8 * w + 7]);
+    return scale;
+}
+#endif

@@ -1,0 +1,443 @@
+// Microscaled 4-bit tensors: narrow, widen, weights and the convolution (LN_F4, LN_MX4; formats and storage in ln_f4.h).
+//
+// What bounds them: narrow and widen move 4.5 (binary16) to 9 (f32) bytes for each byte of codes, so HBM; the product has its own notes.
+#include <exception>
+#include <new>
+
+#include "ln_conv_plan.h"
+#include "ln_f4.h"
+
+namespace {
+
+constexpr int kThreads = 256;
+
+int grid_for(ln_ctx* ctx, int64_t n) {
+    const int64_t b = (n + kThreads - 1) / kThreads, cap = (int64_t)ctx->sm_count * 16;
+    return (int)(b < 1 ? 1 : (b > cap ? cap : b));
+}
+int check_launch(ln_ctx* ctx, const char* what) {
+    ctx->launches++;
+    const cudaError_t e = cudaGetLastError();
+    return e == cudaSuccess ? LN_OK : ln_fail(ctx, LN_ERR_CUDA, "%s: kernel launch failed: %s", what, cudaGetErrorString(e));
+}
+// A new tensor, or the status of why there is none.
+int new_tensor(ln_ctx* ctx, int dtype, int64_t n, int64_t c, int64_t h, int64_t w, ln_tensor** out) {
+    *out = ln_tensor_new(ctx, dtype, n, c, h, w);
+    return *out ? LN_OK : (ctx->err.find("cudaMalloc") != std::string::npos ? LN_ERR_CUDA : LN_ERR_SHAPE);
+}
+// Nothing is thrown across the boundary: what the host code can throw is a failed allocation.
+template <typename F>
+int32_t guarded(ln_ctx* ctx, const char* who, F&& body) {
+    try {
+        return body();
+    } catch (const std::exception&) {
+        return ln_fail(ctx, LN_ERR_CUDA, "%s: host memory exhausted", who);
+    }
+}
+// Tensor scales that keep 6 g, every product of g with a block scale and its reciprocal normal numbers.
+bool usable_scale(int dtype, float s) { return dtype == LN_MX4 ? s == 1.0f : s >= 0x1p-100f && s <= 0x1p100f; }
+
+// ---- narrow ---------------------------------------------------------------------------------------------------------------------
+// One thread per block of 16 or 32 channels.
+
+template <int FMT>
+__device__ __forceinline__ void store_block(const float* x, float g, float six_g, uint8_t* codes, uint8_t* scale) {
+    constexpr int B = FMT == LN_F4 ? 16 : 32;
+    uint32_t w[B / 8];
+    *scale = (uint8_t)ln_f4_quantise<FMT>(x, g, six_g, w);
+    if (FMT == LN_F4) *reinterpret_cast<uint2*>(codes) = make_uint2(w[0], w[1]);
+    else *reinterpret_cast<uint4*>(codes) = make_uint4(w[0], w[1], w[B / 8 - 2], w[B / 8 - 1]);
+}
+
+// f32 NCHW: consecutive threads take consecutive pixels, so that the reads are contiguous.
+template <int FMT>
+__global__ void narrow_f32_kernel(const float* __restrict__ x, uint8_t* __restrict__ codes, uint8_t* __restrict__ sf, int64_t pixels, int64_t hw, int C, int blocks,
+                                  int64_t cstride, int64_t sf_stride, float g, float six_g) {
+    constexpr int B = FMT == LN_F4 ? 16 : 32;
+    for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < pixels * blocks; i += (int64_t)gridDim.x * blockDim.x) {
+        const int64_t pix = i % pixels;
+        const int b = (int)(i / pixels);
+        const float* src = x + (pix / hw * C + b * B) * hw + pix % hw;
+        float v[B];
+#pragma unroll
+        for (int j = 0; j < B; ++j) v[j] = b * B + j < C ? src[j * hw] : 0.0f;
+        store_block<FMT>(v, g, six_g, codes + pix * cstride + b * (B / 2), sf + pix * sf_stride + b);
+    }
+}
+// binary16 NHWC: consecutive threads take consecutive blocks of a pixel.
+template <int FMT>
+__global__ void narrow_f16_kernel(const __half* __restrict__ x, int64_t xs, uint8_t* __restrict__ codes, uint8_t* __restrict__ sf, int64_t pixels, int C, int blocks,
+                                  int64_t cstride, int64_t sf_stride, float g, float six_g) {
+    constexpr int B = FMT == LN_F4 ? 16 : 32;
+    for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < pixels * blocks; i += (int64_t)gridDim.x * blockDim.x) {
+        const int64_t pix = i / blocks;
+        const int b = (int)(i - pix * blocks);
+        float v[B];
+#pragma unroll
+        for (int j = 0; j < B; j += 8) {
+            uint4 q = make_uint4(0, 0, 0, 0);
+            if (b * B + j < C) q = *reinterpret_cast<const uint4*>(x + pix * xs + b * B + j);  // (a pixel's channels are padded to 32)
+            const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[k]));
+                v[j + 2 * k] = b * B + j + 2 * k < C ? f.x : 0.0f;
+                v[j + 2 * k + 1] = b * B + j + 2 * k + 1 < C ? f.y : 0.0f;
+            }
+        }
+        store_block<FMT>(v, g, six_g, codes + pix * cstride + b * (B / 2), sf + pix * sf_stride + b);
+    }
+}
+
+// ---- widen ----------------------------------------------------------------------------------------------------------------------
+// One thread per 16 channels of a pixel.
+
+template <int FMT>
+__device__ __forceinline__ void load_16(const uint8_t* codes, const uint8_t* sf, int b16, float g, float (&v)[16]) {
+    const float d = ln_f4_factor<FMT>(sf[FMT == LN_F4 ? b16 : b16 >> 1], g);
+    const uint2 w = *reinterpret_cast<const uint2*>(codes + b16 * 8);
+    uint32_t h[8];
+    ln_e2m1x8_to_h2(w.x, *reinterpret_cast<uint32_t(*)[4]>(h));
+    ln_e2m1x8_to_h2(w.y, *reinterpret_cast<uint32_t(*)[4]>(h + 4));
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[k]));
+        v[2 * k] = __fmul_rn(f.x, d);
+        v[2 * k + 1] = __fmul_rn(f.y, d);
+    }
+}
+template <int FMT>
+__global__ void widen_f32_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ sf, float* __restrict__ y, int64_t pixels, int64_t hw, int C, int blocks,
+                                 int64_t cstride, int64_t sf_stride, float g) {
+    for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < pixels * blocks; i += (int64_t)gridDim.x * blockDim.x) {
+        const int64_t pix = i % pixels;
+        const int b = (int)(i / pixels);
+        float v[16];
+        load_16<FMT>(codes + pix * cstride, sf + pix * sf_stride, b, g, v);
+        float* dst = y + (pix / hw * C + b * 16) * hw + pix % hw;
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+            if (b * 16 + j < C) dst[j * hw] = v[j];
+    }
+}
+template <int FMT>
+__global__ void widen_f16_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ sf, __half* __restrict__ y, int64_t ys, int64_t pixels, int C, int blocks,
+                                 int64_t cstride, int64_t sf_stride, float g) {
+    for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < pixels * blocks; i += (int64_t)gridDim.x * blockDim.x) {
+        const int64_t pix = i / blocks;
+        const int b = (int)(i - pix * blocks);
+        float v[16];
+        load_16<FMT>(codes + pix * cstride, sf + pix * sf_stride, b, g, v);
+        uint32_t h[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            // (a NaN block that ends inside the padding must not reach it)
+            const __half2 p = __floats2half2_rn(b * 16 + 2 * k < C ? v[2 * k] : 0.0f, b * 16 + 2 * k + 1 < C ? v[2 * k + 1] : 0.0f);
+            h[k] = *reinterpret_cast<const uint32_t*>(&p);
+        }
+        uint4* dst = reinterpret_cast<uint4*>(y + pix * ys + b * 16);
+        dst[0] = make_uint4(h[0], h[1], h[2], h[3]);
+        dst[1] = make_uint4(h[4], h[5], h[6], h[7]);
+    }
+}
+// codes (one per byte) and scales in NCHW order
+__global__ void unpack_f4_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ sf, uint8_t* __restrict__ out_codes, uint8_t* __restrict__ out_sf, int64_t n, int64_t hw,
+                                 int C, int sf_blocks, int64_t cstride, int64_t sf_stride) {
+    const int64_t first = n * C * hw, total = first + n * sf_blocks * hw;
+    for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
+        const int64_t k = i < first ? i : i - first;
+        const int per = i < first ? C : sf_blocks;
+        const int64_t p = k % hw, img = k / hw / per;
+        const int c = (int)(k / hw % per);
+        if (i < first) out_codes[k] = (codes[(img * hw + p) * cstride + c / 2] >> (4 * (c & 1))) & 15;
+        else out_sf[k] = sf[(img * hw + p) * sf_stride + c];
+    }
+}
+
+// ---- weights --------------------------------------------------------------------------------------------------------------------
+// One thread block per filter: its largest magnitude, then the blocks of each tap (a filter's scale 0 leaves zero codes).
+template <int FMT>
+__global__ void pack_weights_f4_kernel(const float* __restrict__ w, int C, int k2, int64_t cstride, uint8_t* __restrict__ codes, uint8_t* __restrict__ sf, float* __restrict__ wscale,
+                                       int bk, int cblocks, int words) {
+    constexpr int B = FMT == LN_F4 ? 16 : 32;
+    const int f = blockIdx.x;
+    const float* src = w + (int64_t)f * C * k2;
+    float amax = 0.0f;
+    for (int64_t i = threadIdx.x; i < (int64_t)C * k2; i += blockDim.x) amax = ln_max_nan(amax, fabsf(src[i]));
+    for (int o = 16; o; o >>= 1) amax = ln_max_nan(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, o));
+    __shared__ float part[32];
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = amax;
+    __syncthreads();
+    amax = 0.0f;
+    for (int i = 0; i < (int)(blockDim.x >> 5); ++i) amax = ln_max_nan(amax, part[i]);
+    // g stays in the range of tensor scales: 1 for a filter of zeros or with a NaN (whose block is NaN), the end of the range behind it
+    float g = 1.0f;
+    if (FMT == LN_F4 && amax > 0.0f) g = fminf(fmaxf(__fdiv_rn(amax, 6.0f * 448.0f), 0x1p-100f), 0x1p100f);
+    if (threadIdx.x == 0) wscale[f] = g;
+    const int blocks = (int)(cstride * 2 / B), per_kblock = 2 * bk / B;
+    for (int i = threadIdx.x; i < k2 * blocks; i += blockDim.x) {
+        const int tap = i / blocks, b = i - tap * blocks;
+        float v[B];
+#pragma unroll
+        for (int j = 0; j < B; ++j) v[j] = b * B + j < C ? src[(int64_t)(b * B + j) * k2 + tap] : 0.0f;
+        const int cb = b / per_kblock, in = b - cb * per_kblock;  // k-block of the tap, scale byte inside it
+        const int64_t at = ((((int64_t)(f / 128) * k2 + tap) * cblocks + cb) * words + in / 4) * 512 + (f % 32) * 16 + f / 32 % 4 * 4 + in % 4;
+        store_block<FMT>(v, g, 6.0f * g, codes + ((int64_t)f * k2 + tap) * cstride + b * (B / 2), sf + at);
+    }
+}
+
+// ---- the product on the CUDA cores ----------------------------------------------------------------------------------------------
+struct simt_params {
+    const uint8_t *x, *xsf, *w, *wsf;
+    const float *wscale, *bias;
+    void* y;
+    int64_t xs, xsf_stride, ys, total;
+    int C, H, W, F, k, sx, sy, pad, OH, OW, blocks, bk, cblocks, words, act, out_f16;
+    float xscale;
+};
+// One thread per output value, filters fastest.  Takes every geometry.
+template <int FMT, bool EXACT>
+__global__ void conv_f4_simt_kernel(const simt_params p) {
+    constexpr int B = FMT == LN_F4 ? 16 : 32;
+    for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < p.total; i += (int64_t)gridDim.x * blockDim.x) {
+        const int f = (int)(i % p.F);
+        const int64_t pix = i / p.F;
+        const int ox = (int)(pix % p.OW), oy = (int)(pix / p.OW % p.OH);
+        const int64_t n = pix / p.OW / p.OH;
+        float acc = 0.0f;
+        for (int r = 0; r < p.k; ++r) {
+            const int yy = oy * p.sy - p.pad + r;
+            if (yy < 0 || yy >= p.H) continue;
+            for (int s = 0; s < p.k; ++s) {
+                const int xx = ox * p.sx - p.pad + s;
+                if (xx < 0 || xx >= p.W) continue;
+                const int64_t q = (n * p.H + yy) * p.W + xx;
+                const int tap = r * p.k + s;
+                const uint8_t* xc = p.x + q * p.xs;
+                const uint8_t* wc = p.w + ((int64_t)f * p.k * p.k + tap) * p.xs;
+                for (int b = 0; b < p.blocks; ++b) {
+                    const int per_kblock = 2 * p.bk / B, cb = b / per_kblock, in = b - cb * per_kblock;
+                    const int64_t at = ((((int64_t)(f / 128) * p.k * p.k + tap) * p.cblocks + cb) * p.words + in / 4) * 512 + (f % 32) * 16 + f / 32 % 4 * 4 + in % 4;
+                    float sum = 0.0f;  // exact: multiples of 0.25 below 2^11
+#pragma unroll
+                    for (int j = 0; j < B / 8; ++j) {
+                        uint32_t a[4], c[4];
+                        ln_e2m1x8_to_h2(*reinterpret_cast<const uint32_t*>(xc + b * (B / 2) + 4 * j), a);
+                        ln_e2m1x8_to_h2(*reinterpret_cast<const uint32_t*>(wc + b * (B / 2) + 4 * j), c);
+#pragma unroll
+                        for (int t = 0; t < 4; ++t) {
+                            const float2 u = __half22float2(*reinterpret_cast<const __half2*>(&a[t])), v = __half22float2(*reinterpret_cast<const __half2*>(&c[t]));
+                            sum = __fmaf_rn(u.x, v.x, sum);
+                            sum = __fmaf_rn(u.y, v.y, sum);
+                        }
+                    }
+                    // (block scales first: their product is exact for LN_F4, and a sum of zero times it is never zero times infinity)
+                    if (FMT == LN_F4) acc = __fmaf_rn(sum, __fmul_rn(ln_e4m3_value(p.xsf[q * p.xsf_stride + b]), ln_e4m3_value(p.wsf[at])), acc);
+                    else acc = __fmaf_rn(__fmul_rn(sum, ln_e8m0_value(p.xsf[q * p.xsf_stride + b])), ln_e8m0_value(p.wsf[at]), acc);
+                }
+            }
+        }
+        const float v = ln_epilogue_act<EXACT>(p.act, __fmaf_rn(acc, __fmul_rn(p.xscale, p.wscale[f]), p.bias[f]));
+        if (p.out_f16) ((__half*)p.y)[pix * p.ys + f] = __float2half_rn(v);
+        else ((float*)p.y)[((n * p.F + f) * p.OH + oy) * p.OW + ox] = v;
+    }
+}
+
+int narrow_into(ln_ctx* ctx, const ln_tensor* t, ln_tensor* q) {
+    const int64_t pixels = t->n * t->h * t->w, hw = t->h * t->w;
+    const int blocks = (int)(q->cstride * 2 / ln_f4_block(q->dtype));
+    const int grid = grid_for(ctx, pixels * blocks);
+    uint8_t *codes = (uint8_t*)q->ptr, *sf = (uint8_t*)q->sf;
+    const float g = q->scale, six_g = 6.0f * g;
+    if (t->dtype == LN_F32) {
+        if (q->dtype == LN_F4) narrow_f32_kernel<LN_F4><<<grid, kThreads, 0, ctx->stream>>>((const float*)t->ptr, codes, sf, pixels, hw, (int)t->c, blocks, q->cstride, q->sf_stride, g, six_g);
+        else narrow_f32_kernel<LN_MX4><<<grid, kThreads, 0, ctx->stream>>>((const float*)t->ptr, codes, sf, pixels, hw, (int)t->c, blocks, q->cstride, q->sf_stride, g, six_g);
+    } else {
+        if (q->dtype == LN_F4) narrow_f16_kernel<LN_F4><<<grid, kThreads, 0, ctx->stream>>>((const __half*)t->ptr, t->cstride / 2, codes, sf, pixels, (int)t->c, blocks, q->cstride, q->sf_stride, g, six_g);
+        else narrow_f16_kernel<LN_MX4><<<grid, kThreads, 0, ctx->stream>>>((const __half*)t->ptr, t->cstride / 2, codes, sf, pixels, (int)t->c, blocks, q->cstride, q->sf_stride, g, six_g);
+    }
+    return check_launch(ctx, "ln_tensor_narrow_f4");
+}
+
+}  // namespace
+
+extern "C" {
+
+int32_t ln_tensor_narrow_f4(ln_ctx* ctx, const ln_tensor* t, float scale, int32_t dtype, ln_tensor** out) {
+    const char* who = "ln_tensor_narrow_f4";
+    if (!ctx || !t || !out) return ln_fail(ctx, LN_ERR_ARG, "%s: NULL argument", who);
+    if (t->dtype != LN_F32 && t->dtype != LN_F16) return ln_fail(ctx, LN_ERR_ARG, "%s: f32 or binary16 tensor required", who);
+    if (t->ctx != ctx) return ln_fail(ctx, LN_ERR_ARG, "%s: the tensor belongs to another context", who);
+    if (!ln_is_f4(dtype)) return ln_fail(ctx, LN_ERR_ARG, "%s: dtype must be LN_F4 or LN_MX4", who);
+    if (!usable_scale(dtype, scale)) return ln_fail(ctx, LN_ERR_ARG, "%s: scale %g is not %s", who, scale, dtype == LN_MX4 ? "1 (LN_MX4 has no tensor scale)" : "in [2^-100, 2^100]");
+    return guarded(ctx, who, [&]() -> int32_t {
+        cudaSetDevice(ctx->device);
+        ln_tensor* q = nullptr;
+        int rc = new_tensor(ctx, dtype, t->n, t->c, t->h, t->w, &q);
+        if (rc) return rc;
+        q->scale = scale;
+        rc = narrow_into(ctx, t, q);
+        if (rc) { ln_tensor_release(q); return rc; }
+        *out = q;
+        return LN_OK;
+    });
+}
+
+int32_t ln_tensor_widen_f4(ln_ctx* ctx, const ln_tensor* t, int32_t dtype, ln_tensor** out) {
+    const char* who = "ln_tensor_widen_f4";
+    if (!ctx || !t || !out) return ln_fail(ctx, LN_ERR_ARG, "%s: NULL argument", who);
+    if (!ln_is_f4(t->dtype)) return ln_fail(ctx, LN_ERR_ARG, "%s: 4-bit tensor required", who);
+    if (t->ctx != ctx) return ln_fail(ctx, LN_ERR_ARG, "%s: the tensor belongs to another context", who);
+    if (dtype != LN_F32 && dtype != LN_F16) return ln_fail(ctx, LN_ERR_ARG, "%s: dtype must be LN_F32 or LN_F16", who);
+    return guarded(ctx, who, [&]() -> int32_t {
+        cudaSetDevice(ctx->device);
+        ln_tensor* y = nullptr;
+        int rc = new_tensor(ctx, dtype, t->n, t->c, t->h, t->w, &y);
+        if (rc) return rc;
+        const int64_t pixels = t->n * t->h * t->w, hw = t->h * t->w;
+        const uint8_t *codes = (const uint8_t*)t->ptr, *sf = (const uint8_t*)t->sf;
+        if (dtype == LN_F32) {
+            const int blocks = (int)((t->c + 15) / 16), grid = grid_for(ctx, pixels * blocks);
+            if (t->dtype == LN_F4) widen_f32_kernel<LN_F4><<<grid, kThreads, 0, ctx->stream>>>(codes, sf, (float*)y->ptr, pixels, hw, (int)t->c, blocks, t->cstride, t->sf_stride, t->scale);
+            else widen_f32_kernel<LN_MX4><<<grid, kThreads, 0, ctx->stream>>>(codes, sf, (float*)y->ptr, pixels, hw, (int)t->c, blocks, t->cstride, t->sf_stride, 1.0f);
+        } else {
+            const int blocks = (int)(y->cstride / 32), grid = grid_for(ctx, pixels * blocks);
+            if (t->dtype == LN_F4) widen_f16_kernel<LN_F4><<<grid, kThreads, 0, ctx->stream>>>(codes, sf, (__half*)y->ptr, y->cstride / 2, pixels, (int)t->c, blocks, t->cstride, t->sf_stride, t->scale);
+            else widen_f16_kernel<LN_MX4><<<grid, kThreads, 0, ctx->stream>>>(codes, sf, (__half*)y->ptr, y->cstride / 2, pixels, (int)t->c, blocks, t->cstride, t->sf_stride, 1.0f);
+        }
+        rc = check_launch(ctx, who);
+        if (rc) { ln_tensor_release(y); return rc; }
+        *out = y;
+        return LN_OK;
+    });
+}
+
+int32_t ln_tensor_download_f4(ln_ctx* ctx, const ln_tensor* t, uint8_t* host_codes, int64_t code_count, uint8_t* host_scales, int64_t scale_count) {
+    const char* who = "ln_tensor_download_f4";
+    if (!ctx || !t || !host_codes || !host_scales) return ln_fail(ctx, LN_ERR_ARG, "%s: NULL argument", who);
+    if (!ln_is_f4(t->dtype)) return ln_fail(ctx, LN_ERR_ARG, "%s: 4-bit tensor required", who);
+    if (t->ctx != ctx) return ln_fail(ctx, LN_ERR_ARG, "%s: the tensor belongs to another context", who);
+    const int sf_blocks = (int)((t->c + ln_f4_block(t->dtype) - 1) / ln_f4_block(t->dtype));
+    const int64_t hw = t->h * t->w, scales = t->n * sf_blocks * hw;
+    if (code_count != t->count() || scale_count != scales)
+        return ln_fail(ctx, LN_ERR_SHAPE, "%s: the tensor has %lld codes and %lld scales", who, (long long)t->count(), (long long)scales);
+    return guarded(ctx, who, [&]() -> int32_t {
+        cudaSetDevice(ctx->device);
+        uint8_t* tmp = (uint8_t*)ln_pool_alloc(ctx, (size_t)(code_count + scales));
+        if (!tmp) return LN_ERR_CUDA;
+        unpack_f4_kernel<<<grid_for(ctx, code_count + scales), kThreads, 0, ctx->stream>>>((const uint8_t*)t->ptr, (const uint8_t*)t->sf, tmp, tmp + code_count, t->n, hw, (int)t->c, sf_blocks,
+                                                                                         t->cstride, t->sf_stride);
+        int rc = check_launch(ctx, who);
+        cudaError_t e = cudaSuccess;
+        if (rc == LN_OK) {
+            e = cudaMemcpyAsync(host_codes, tmp, (size_t)code_count, cudaMemcpyDeviceToHost, ctx->stream);
+            if (e == cudaSuccess) e = cudaMemcpyAsync(host_scales, tmp + code_count, (size_t)scales, cudaMemcpyDeviceToHost, ctx->stream);
+            const cudaError_t s = cudaStreamSynchronize(ctx->stream);
+            if (e == cudaSuccess) e = s;
+        }
+        ln_pool_free(ctx, tmp, 0);
+        if (e != cudaSuccess) return ln_fail(ctx, LN_ERR_CUDA, "%s: %s", who, cudaGetErrorString(e));
+        return rc ? rc : ln_status(ctx, who);
+    });
+}
+
+int32_t ln_conv_weights_f4(ln_ctx* ctx, const ln_tensor* weights_f32, int64_t filters, int64_t channels, int64_t kernel_size, int32_t dtype, ln_conv_weights** out) {
+    const char* who = "ln_conv_weights_f4";
+    if (!ctx || !weights_f32 || !out) return ln_fail(ctx, LN_ERR_ARG, "%s: NULL argument", who);
+    if (weights_f32->dtype != LN_F32) return ln_fail(ctx, LN_ERR_ARG, "%s: f32 weights required", who);
+    if (weights_f32->ctx != ctx) return ln_fail(ctx, LN_ERR_ARG, "%s: the tensor belongs to another context", who);
+    if (!ln_is_f4(dtype)) return ln_fail(ctx, LN_ERR_ARG, "%s: dtype must be LN_F4 or LN_MX4", who);
+    if (filters < 1 || channels < 1 || kernel_size < 1 || filters > (1 << 24) || channels > (1 << 24) || kernel_size > 64 || weights_f32->count() != filters * channels * kernel_size * kernel_size)
+        return ln_fail(ctx, LN_ERR_SHAPE, "%s: weight tensor has %lld elements, expected %lld x %lld x %lld x %lld", who, (long long)weights_f32->count(), (long long)filters, (long long)channels,
+                       (long long)kernel_size, (long long)kernel_size);
+    return guarded(ctx, who, [&]() -> int32_t {
+        cudaSetDevice(ctx->device);
+        const int64_t k2 = kernel_size * kernel_size;
+        const ln_f4_kblocks kb = ln_f4_kblocks_of(dtype, channels);
+        ln_conv_weights* w = new ln_conv_weights();
+        w->ctx = ctx; w->dtype = dtype;
+        w->filters = filters; w->channels = channels; w->k = kernel_size;
+        w->fpad = ln_round_up(filters, kF4FilterPad); w->cpad = ln_f4_cstride(channels);
+        const size_t sf_bytes = (size_t)(w->fpad / 128 * k2 * kb.cblocks * kb.words * 512);
+        w->w = ln_pool_alloc(ctx, (size_t)(filters * k2 * w->cpad));
+        w->sf = ln_pool_alloc(ctx, sf_bytes);
+        w->wscale = (float*)ln_pool_alloc(ctx, (size_t)filters * 4);
+        if (!w->w || !w->sf || !w->wscale) { ln_conv_weights_release(w); return LN_ERR_CUDA; }
+        int rc = LN_OK;
+        const cudaError_t e = cudaMemsetAsync(w->sf, 0, sf_bytes, ctx->stream);
+        if (e != cudaSuccess) rc = ln_fail(ctx, LN_ERR_CUDA, "%s: %s", who, cudaGetErrorString(e));
+        if (rc == LN_OK) {
+            if (dtype == LN_F4) pack_weights_f4_kernel<LN_F4><<<(int)filters, 256, 0, ctx->stream>>>((const float*)weights_f32->ptr, (int)channels, (int)k2, w->cpad, (uint8_t*)w->w, (uint8_t*)w->sf, w->wscale, kb.bk, kb.cblocks, kb.words);
+            else pack_weights_f4_kernel<LN_MX4><<<(int)filters, 256, 0, ctx->stream>>>((const float*)weights_f32->ptr, (int)channels, (int)k2, w->cpad, (uint8_t*)w->w, (uint8_t*)w->sf, w->wscale, kb.bk, kb.cblocks, kb.words);
+            rc = check_launch(ctx, who);
+        }
+        if (rc) { ln_conv_weights_release(w); return rc; }
+        *out = w;
+        return LN_OK;
+    });
+}
+
+int32_t ln_conv2d_bias_act_f4(ln_ctx* ctx, const ln_tensor* x, const ln_conv_weights* weights, const ln_tensor* bias, const int64_t output_shape[4], int64_t channels,
+                              int64_t input_height, int64_t input_width, int64_t filters, int64_t kernel_size, int64_t stride_x, int64_t stride_y, int64_t dilation,
+                              int64_t padding, int64_t groups, int32_t activation, float y_scale, int32_t out_kind, ln_tensor** out) {
+    const char* who = "ln_conv2d_bias_act_f4";
+    if (!ctx || !x || !weights || !bias || !output_shape || !out) return ln_fail(ctx, LN_ERR_ARG, "%s: NULL argument", who);
+    if (!ln_is_f4(x->dtype)) return ln_fail(ctx, LN_ERR_ARG, "%s: 4-bit input required", who);
+    if (weights->dtype != x->dtype) return ln_fail(ctx, LN_ERR_ARG, "%s: input and weights have different types", who);
+    if (x->ctx != ctx || weights->ctx != ctx || bias->ctx != ctx) return ln_fail(ctx, LN_ERR_ARG, "%s: an operand belongs to another context", who);
+    if (bias->dtype != LN_F32 || bias->count() != filters) return ln_fail(ctx, LN_ERR_SHAPE, "%s: bias must be f32 [filters]", who);
+    if (groups != 1 || dilation != 1) return ln_fail(ctx, LN_ERR_UNSUPPORTED, "%s: groups and dilation must be 1", who);
+    if (kernel_size < 1 || stride_x < 1 || stride_y < 1 || stride_x > 64 || stride_y > 64 || padding < 0 || padding > 64) return ln_fail(ctx, LN_ERR_SHAPE, "%s: invalid geometry", who);
+    if (x->c != channels || x->h != input_height || x->w != input_width || weights->filters != filters || weights->channels != channels || weights->k != kernel_size)
+        return ln_fail(ctx, LN_ERR_SHAPE, "%s: geometry does not match the tensors", who);
+    if (activation < LN_ACT_LINEAR || activation > LN_ACT_RELU) return ln_fail(ctx, LN_ERR_UNSUPPORTED, "%s: activation %d is not on the detector path", who, activation);
+    if (out_kind != LN_OUT_Q && out_kind != LN_OUT_F32 && out_kind != LN_OUT_F16) return ln_fail(ctx, LN_ERR_ARG, "%s: out_kind must be LN_OUT_Q, LN_OUT_F32 or LN_OUT_F16", who);
+    if (out_kind == LN_OUT_Q && !usable_scale(x->dtype, y_scale)) return ln_fail(ctx, LN_ERR_ARG, "%s: y_scale %g is not %s", who, y_scale, x->dtype == LN_MX4 ? "1 (LN_MX4 has no tensor scale)" : "in [2^-100, 2^100]");
+    const int64_t oh = (input_height + 2 * padding - kernel_size < 0 ? 0 : input_height + 2 * padding - kernel_size) / stride_y + 1;
+    const int64_t ow = (input_width + 2 * padding - kernel_size < 0 ? 0 : input_width + 2 * padding - kernel_size) / stride_x + 1;
+    if (output_shape[0] != x->n || output_shape[1] != filters || output_shape[2] != oh || output_shape[3] != ow)
+        return ln_fail(ctx, LN_ERR_SHAPE, "%s: output_shape does not match [%lld,%lld,%lld,%lld]", who, (long long)x->n, (long long)filters, (long long)oh, (long long)ow);
+    if (input_height > (1 << 24) || input_width > (1 << 24)) return ln_fail(ctx, LN_ERR_UNSUPPORTED, "%s: more than 2^24 rows or columns", who);
+    int rc = ln_status(ctx, who);  // of an earlier call
+    if (rc) return rc;
+    return guarded(ctx, who, [&]() -> int32_t {
+        cudaSetDevice(ctx->device);
+        ln_tensor *y = nullptr, *wide = nullptr;
+        int rc = new_tensor(ctx, out_kind == LN_OUT_Q ? x->dtype : (out_kind == LN_OUT_F16 ? LN_F16 : LN_F32), x->n, filters, oh, ow, &y);
+        if (rc == LN_OK && out_kind == LN_OUT_Q) {
+            y->scale = y_scale;
+            rc = new_tensor(ctx, LN_F32, x->n, filters, oh, ow, &wide);
+        }
+        if (rc == LN_OK && y->dtype == LN_F16 && y->cstride != 2 * filters) {
+            const cudaError_t e = cudaMemsetAsync(y->ptr, 0, y->bytes, ctx->stream);
+            if (e != cudaSuccess) rc = ln_fail(ctx, LN_ERR_CUDA, "%s: %s", who, cudaGetErrorString(e));
+        }
+        if (rc == LN_OK) {
+            const ln_f4_kblocks kb = ln_f4_kblocks_of(x->dtype, channels);
+            const ln_tensor* dst = wide ? wide : y;
+            simt_params p;
+            p.x = (const uint8_t*)x->ptr; p.xsf = (const uint8_t*)x->sf; p.w = (const uint8_t*)weights->w; p.wsf = (const uint8_t*)weights->sf;
+            p.wscale = weights->wscale; p.bias = (const float*)bias->ptr; p.y = dst->ptr;
+            p.xs = x->cstride; p.xsf_stride = x->sf_stride; p.ys = dst->cstride / 2; p.total = x->n * oh * ow * filters;
+            p.C = (int)channels; p.H = (int)input_height; p.W = (int)input_width; p.F = (int)filters; p.k = (int)kernel_size; p.sx = (int)stride_x; p.sy = (int)stride_y; p.pad = (int)padding;
+            p.OH = (int)oh; p.OW = (int)ow; p.blocks = (int)(x->cstride * 2 / ln_f4_block(x->dtype)); p.bk = kb.bk; p.cblocks = kb.cblocks; p.words = kb.words;
+            p.act = activation; p.out_f16 = dst->dtype == LN_F16; p.xscale = x->scale;
+            const int grid = grid_for(ctx, p.total);
+            if (x->dtype == LN_F4) {
+                if (ctx->exact_epilogue) conv_f4_simt_kernel<LN_F4, true><<<grid, kThreads, 0, ctx->stream>>>(p);
+                else conv_f4_simt_kernel<LN_F4, false><<<grid, kThreads, 0, ctx->stream>>>(p);
+            } else {
+                if (ctx->exact_epilogue) conv_f4_simt_kernel<LN_MX4, true><<<grid, kThreads, 0, ctx->stream>>>(p);
+                else conv_f4_simt_kernel<LN_MX4, false><<<grid, kThreads, 0, ctx->stream>>>(p);
+            }
+            rc = check_launch(ctx, who);
+            if (rc == LN_OK && wide) rc = narrow_into(ctx, wide, y);
+        }
+        if (wide) ln_tensor_release(wide);
+        if (rc) { if (y) ln_tensor_release(y); return rc; }
+        *out = y;
+        return LN_OK;
+    });
+}
+
+}  // extern "C"

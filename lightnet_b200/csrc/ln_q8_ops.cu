@@ -1285,6 +1285,7 @@ int32_t ln_conv_weights_release(ln_conv_weights* w) {
     if (w->w) ln_pool_free(ctx, w->w, (size_t)(w->fpad * w->k * w->k * w->cpad));
     if (w->w_oihw) ln_pool_free(ctx, w->w_oihw, (size_t)(w->filters * w->channels * w->k * w->k));
     if (w->wscale) ln_pool_free(ctx, w->wscale, (size_t)w->fpad * 8);
+    if (w->sf) ln_pool_free(ctx, w->sf, 0);
     ln_tensor_release(w->src_f32);
     delete w;
     return LN_OK;

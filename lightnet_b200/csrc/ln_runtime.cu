@@ -3,6 +3,7 @@
 #include <cstring>
 
 #include "ln_common.h"
+#include "ln_f4.h"
 
 static thread_local std::string g_create_error;
 
@@ -87,6 +88,10 @@ static size_t storage_bytes(int dtype, int64_t n, int64_t c, int64_t h, int64_t 
         *cstride = 2 * ln_round_up(c, 32);
         return (size_t)(n * h * w * *cstride);
     }
+    if (ln_is_f4(dtype)) {  // NHWC, two codes per byte, channels padded to 64; then the block scales of all pixels
+        *cstride = ln_f4_cstride(c);
+        return (size_t)(n * h * w * (*cstride + ln_f4_sf_stride(dtype, c)));
+    }
     *cstride = 0;
     return (size_t)(n * c * h * w) * 4;
 }
@@ -105,6 +110,10 @@ ln_tensor* ln_tensor_new(ln_ctx* ctx, int dtype, int64_t n, int64_t c, int64_t h
     t->base = ln_pool_alloc(ctx, t->bytes);
     if (!t->base) { delete t; return nullptr; }
     t->ptr = t->base;
+    if (ln_is_f4(dtype)) {
+        t->sf = (char*)t->ptr + n * h * w * t->cstride;
+        t->sf_stride = ln_f4_sf_stride(dtype, c);
+    }
     return t;
 }
 
@@ -198,7 +207,7 @@ const char* ln_last_error(ln_ctx* ctx) { return ctx ? ctx->err.c_str() : g_creat
 int32_t ln_sync(ln_ctx* ctx) {
     if (!ctx) return LN_ERR_ARG;
     LN_CUDA(ctx, cudaStreamSynchronize(ctx->stream));
-    return LN_OK;
+    return ln_status(ctx, "ln_sync");
 }
 
 void* ln_ctx_stream(ln_ctx* ctx) { return ctx ? (void*)ctx->stream : nullptr; }
@@ -276,7 +285,7 @@ int32_t ln_tensor_download_f32(ln_ctx* ctx, const ln_tensor* t, float* host, int
     if (count != t->count()) return ln_fail(ctx, LN_ERR_SHAPE, "download of %lld elements from a tensor of %lld", (long long)count, (long long)t->count());
     LN_CUDA(ctx, cudaMemcpyAsync(host, t->ptr, (size_t)count * 4, cudaMemcpyDeviceToHost, ctx->stream));
     LN_CUDA(ctx, cudaStreamSynchronize(ctx->stream));
-    return LN_OK;
+    return ln_status(ctx, "ln_tensor_download_f32");
 }
 
 int32_t ln_tensor_download_i32(ln_ctx* ctx, const ln_tensor* t, int32_t* host, int64_t count) {
@@ -295,6 +304,19 @@ int32_t ln_tensor_shape(const ln_tensor* t, int64_t shape[4]) {
 }
 
 int32_t ln_tensor_dtype(const ln_tensor* t) { return t ? t->dtype : -1; }
+
+int32_t ln_tensor_device_data(const ln_tensor* t, void** data, int64_t strides[4]) {
+    if (!t || !data || !strides) return LN_ERR_ARG;
+    if (t->dtype == LN_F32) {
+        strides[3] = 1; strides[2] = t->w; strides[1] = t->h * t->w; strides[0] = t->c * t->h * t->w;
+    } else if (t->dtype == LN_F16) {
+        strides[1] = 1; strides[3] = t->cstride / 2; strides[2] = t->w * strides[3]; strides[0] = t->h * strides[2];
+    } else
+        return ln_fail(t->ctx, LN_ERR_ARG, "ln_tensor_device_data: f32 or binary16 tensor required");
+    *data = t->ptr;
+    return LN_OK;
+}
+
 float ln_tensor_scale(const ln_tensor* t) { return t ? t->scale : 0.0f; }
 
 int32_t ln_tensor_retain(ln_tensor* t) {
