@@ -34,7 +34,8 @@ inline ln_f4_kblocks ln_f4_kblocks_of(int dtype, int64_t c) {
     k.words = dtype == LN_MX4 ? (k.bk + 63) / 64 : k.bk / 32;
     return k;
 }
-constexpr int64_t kF4FilterPad = 256;  // filters that the scales of weights are padded to (zeros): the widest filter tile
+// Scales are there for this many filters behind the last group of 128 (zeros): a tile of up to 256 filters may start at the last one.
+constexpr int64_t kF4FilterPad = 256;
 
 #ifdef __CUDACC__
 // ---- the number formats -----------------------------------------------------------------------------------------------------------
@@ -122,3 +123,15 @@ __device__ __forceinline__ uint32_t ln_f4_quantise(const float* x, float g, floa
     return scale;
 }
 #endif
+
+// ---- the product on the tensor cores (ln_f4_umma.cu) --------------------------------------------------------------------------------
+struct ln_f4_conv {  // one convolution: operands, geometry, output
+    int dtype = LN_F4;
+    const ln_tensor* x = nullptr;
+    const ln_conv_weights* w = nullptr;
+    const float* bias = nullptr;
+    ln_tensor* y = nullptr;
+    int k = 1, stride = 1, pad = 0, act = 0, out_kind = LN_OUT_F32;
+};
+bool ln_f4_umma_takes(const ln_f4_conv& c, int64_t stride_x, int64_t stride_y);
+int ln_f4_umma_launch(ln_ctx* ctx, const ln_f4_conv& c);

@@ -357,7 +357,7 @@ int32_t ln_conv_weights_f4(ln_ctx* ctx, const ln_tensor* weights_f32, int64_t fi
         ln_conv_weights* w = new ln_conv_weights();
         w->ctx = ctx; w->dtype = dtype;
         w->filters = filters; w->channels = channels; w->k = kernel_size;
-        w->fpad = ln_round_up(filters, kF4FilterPad); w->cpad = ln_f4_cstride(channels);
+        w->fpad = ln_round_up(filters, 128) + kF4FilterPad; w->cpad = ln_f4_cstride(channels);
         const size_t sf_bytes = (size_t)(w->fpad / 128 * k2 * kb.cblocks * kb.words * 512);
         w->w = ln_pool_alloc(ctx, (size_t)(filters * k2 * w->cpad));
         w->sf = ln_pool_alloc(ctx, sf_bytes);
@@ -404,10 +404,17 @@ int32_t ln_conv2d_bias_act_f4(ln_ctx* ctx, const ln_tensor* x, const ln_conv_wei
         cudaSetDevice(ctx->device);
         ln_tensor *y = nullptr, *wide = nullptr;
         int rc = new_tensor(ctx, out_kind == LN_OUT_Q ? x->dtype : (out_kind == LN_OUT_F16 ? LN_F16 : LN_F32), x->n, filters, oh, ow, &y);
-        if (rc == LN_OK && out_kind == LN_OUT_Q) {
-            y->scale = y_scale;
-            rc = new_tensor(ctx, LN_F32, x->n, filters, oh, ow, &wide);
+        ln_f4_conv c;
+        c.dtype = x->dtype; c.x = x; c.w = weights; c.bias = (const float*)bias->ptr; c.y = y;
+        c.k = (int)kernel_size; c.stride = (int)stride_x; c.pad = (int)padding; c.act = activation; c.out_kind = out_kind;
+        if (rc == LN_OK && out_kind == LN_OUT_Q) y->scale = y_scale;
+        if (rc == LN_OK && ln_f4_umma_takes(c, stride_x, stride_y)) {
+            rc = ln_f4_umma_launch(ctx, c);
+            if (rc) { ln_tensor_release(y); return rc; }
+            *out = y;
+            return LN_OK;
         }
+        if (rc == LN_OK && out_kind == LN_OUT_Q) rc = new_tensor(ctx, LN_F32, x->n, filters, oh, ow, &wide);
         if (rc == LN_OK && y->dtype == LN_F16 && y->cstride != 2 * filters) {
             const cudaError_t e = cudaMemsetAsync(y->ptr, 0, y->bytes, ctx->stream);
             if (e != cudaSuccess) rc = ln_fail(ctx, LN_ERR_CUDA, "%s: %s", who, cudaGetErrorString(e));

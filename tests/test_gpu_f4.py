@@ -30,7 +30,7 @@ def be():
 
 
 def f32(v):
-    with np.errstate(over="ignore"):
+    with np.errstate(over="ignore", invalid="ignore"):
         return np.asarray(v, np.float64).astype(np.float32).astype(np.float64)
 
 
