@@ -61,8 +61,8 @@ struct ln_tensor {
     ln_tensor* parent = nullptr;         // keeps the owner of a view alive
     int64_t cstride = 0;                 // 8-bit and binary16 NHWC tensors: bytes between consecutive pixels
     float scale = 1.0f;                  // 8-bit tensors: value = code * scale; LN_F4: value = code * block scale * scale
-    void* sf = nullptr;                  // 4-bit tensors: block scales, sf_stride bytes per pixel (behind the codes in the same block)
-    int64_t sf_stride = 0;
+    void* sf = nullptr;                  // 4-bit tensors: block scales (behind the codes in the same block, order in ln_f4.h)
+    int64_t sf_words = 0;                // and their 4-byte words per pixel
     int64_t count() const { return n * c * h * w; }
 };
 

@@ -1,8 +1,13 @@
 // Storage of the microscaled 4-bit types, shared by their operators.
 //
 // A tensor is NHWC: per pixel two codes per byte (channel 2i in the low nibble), channels padded to 64, so that a pixel is a multiple
-// of the 32 bytes that one tensor-core instruction consumes; behind the codes of all pixels the block scales, sf_stride bytes per
-// pixel.  Codes and scales of the padding up to 64 channels are zero; scale bytes behind those are never read.
+// of the 32 bytes that one tensor-core instruction consumes.  Weights are the same with a filter's taps in the place of a pixel.
+// The k range of a product is cut into k-blocks of `bk` bytes of one tap (the last one of a tap may be shorter), a k-block's scales into
+// `words` of 4 bytes: LN_F4 has one word for the 64 channels of an instruction, LN_MX4 one for the 128 of two.
+// Block scales lie behind the codes in the order in which the tensor cores take them: per 128 pixels (filters) and k-block `words`
+// groups of 512 bytes, [32 pixels][4 groups of 32 pixels][4 scale bytes], so that pixel q has its word at q % 32 * 16 + q / 32 % 4 * 4.
+// A product over pixels in their own order copies them as they are; one whose taps shift the pixels gathers words.
+// Codes and scales of the padding up to 64 channels are zero; the other scale bytes of a group are never used.
 #pragma once
 
 #include <cstdint>
@@ -12,17 +17,6 @@
 inline bool ln_is_f4(int dtype) { return dtype == LN_F4 || dtype == LN_MX4; }
 inline int ln_f4_block(int dtype) { return dtype == LN_MX4 ? 32 : 16; }
 inline int64_t ln_f4_cstride(int64_t c) { return ln_round_up(c, 64) / 2; }
-// The scales of up to 256 channels (the channels of one k-block of the product) are read with one access of 4, 8 or 16 bytes.
-inline int64_t ln_f4_sf_stride(int dtype, int64_t c) {
-    const int64_t need = ln_round_up(c, 64) / ln_f4_block(dtype);
-    if (dtype == LN_MX4) return c <= 128 ? 4 : ln_round_up(need, 8);
-    return c <= 64 ? 4 : (c <= 128 ? 8 : ln_round_up(need, 16));
-}
-
-// Weights: codes [filters][k * k][cstride]; block scales in the order in which the tensor cores take them.  The k range is cut into
-// k-blocks of `bk` bytes of one tap (the last one of a tap may be shorter); per 128 filters and k-block there are `words` groups of
-// 512 bytes: [32 filters][4 groups of 32 filters][4 scale bytes], so that filter f has the word ((f % 32) * 4 + f / 32 % 4).
-// LN_F4: a word holds the scales of 64 channels (one instruction); LN_MX4: of 128 (two).
 struct ln_f4_kblocks {
     int bk, cblocks, words;
 };
@@ -34,10 +28,20 @@ inline ln_f4_kblocks ln_f4_kblocks_of(int dtype, int64_t c) {
     k.words = dtype == LN_MX4 ? (k.bk + 63) / 64 : k.bk / 32;
     return k;
 }
+inline int64_t ln_f4_sf_words(int dtype, int64_t c) {  // of a pixel
+    const ln_f4_kblocks k = ln_f4_kblocks_of(dtype, c);
+    return (int64_t)k.cblocks * k.words;
+}
+inline int64_t ln_f4_sf_bytes(int dtype, int64_t pixels, int64_t c) { return (pixels + 127) / 128 * ln_f4_sf_words(dtype, c) * 512; }
 // Scales are there for this many filters behind the last group of 128 (zeros): a tile of up to 256 filters may start at the last one.
 constexpr int64_t kF4FilterPad = 256;
 
 #ifdef __CUDACC__
+// byte of the scales at which word w of pixel q starts
+__host__ __device__ __forceinline__ int64_t ln_f4_sf_at(int64_t q, int64_t w, int64_t words_per_pixel) {
+    return ((q >> 7) * words_per_pixel + w) * 512 + (q & 31) * 16 + (q >> 5 & 3) * 4;
+}
+
 // ---- the number formats -----------------------------------------------------------------------------------------------------------
 
 // max that hands a NaN on
@@ -110,8 +114,19 @@ __device__ __forceinline__ uint32_t ln_f4_quantise(const float* x, float g, floa
     float t[B];
     if (FMT == LN_F4) {
         const float d = ln_f4_factor<FMT>(scale, g);
+        if (scale == 126u) {  // the scale may have saturated: quotients of any size
 #pragma unroll
-        for (int i = 0; i < B; ++i) t[i] = scale ? __fdiv_rn(x[i], d) : 0.0f;
+            for (int i = 0; i < B; ++i) t[i] = __fdiv_rn(x[i], d);
+        } else {
+            // |x / d| < 8 here (or everything is NaN): x / d by one correction of x * (1 / d), three operations instead of a division.
+            // The result is the rounded quotient but where that is within 2^-22 steps of the middle of two numbers.
+            const float r = scale ? __frcp_rn(d) : 0.0f;
+#pragma unroll
+            for (int i = 0; i < B; ++i) {
+                const float q = __fmul_rn(x[i], r);
+                t[i] = __fmaf_rn(__fmaf_rn(-q, d, x[i]), r, q);
+            }
+        }
     } else {
         const float inv = __uint_as_float((254u - (scale > 253u ? 253u : scale)) << 23);  // 2^-e, exact
 #pragma unroll

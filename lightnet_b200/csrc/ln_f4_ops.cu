@@ -52,7 +52,7 @@ __device__ __forceinline__ void store_block(const float* x, float g, float six_g
 // f32 NCHW: consecutive threads take consecutive pixels, so that the reads are contiguous.
 template <int FMT>
 __global__ void narrow_f32_kernel(const float* __restrict__ x, uint8_t* __restrict__ codes, uint8_t* __restrict__ sf, int64_t pixels, int64_t hw, int C, int blocks,
-                                  int64_t cstride, int64_t sf_stride, float g, float six_g) {
+                                  int64_t cstride, int64_t sf_words, float g, float six_g) {
     constexpr int B = FMT == LN_F4 ? 16 : 32;
     for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < pixels * blocks; i += (int64_t)gridDim.x * blockDim.x) {
         const int64_t pix = i % pixels;
@@ -61,13 +61,13 @@ __global__ void narrow_f32_kernel(const float* __restrict__ x, uint8_t* __restri
         float v[B];
 #pragma unroll
         for (int j = 0; j < B; ++j) v[j] = b * B + j < C ? src[j * hw] : 0.0f;
-        store_block<FMT>(v, g, six_g, codes + pix * cstride + b * (B / 2), sf + pix * sf_stride + b);
+        store_block<FMT>(v, g, six_g, codes + pix * cstride + b * (B / 2), sf + ln_f4_sf_at(pix, b >> 2, sf_words) + (b & 3));
     }
 }
 // binary16 NHWC: consecutive threads take consecutive blocks of a pixel.
 template <int FMT>
 __global__ void narrow_f16_kernel(const __half* __restrict__ x, int64_t xs, uint8_t* __restrict__ codes, uint8_t* __restrict__ sf, int64_t pixels, int C, int blocks,
-                                  int64_t cstride, int64_t sf_stride, float g, float six_g) {
+                                  int64_t cstride, int64_t sf_words, float g, float six_g) {
     constexpr int B = FMT == LN_F4 ? 16 : 32;
     for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < pixels * blocks; i += (int64_t)gridDim.x * blockDim.x) {
         const int64_t pix = i / blocks;
@@ -85,7 +85,7 @@ __global__ void narrow_f16_kernel(const __half* __restrict__ x, int64_t xs, uint
                 v[j + 2 * k + 1] = b * B + j + 2 * k + 1 < C ? f.y : 0.0f;
             }
         }
-        store_block<FMT>(v, g, six_g, codes + pix * cstride + b * (B / 2), sf + pix * sf_stride + b);
+        store_block<FMT>(v, g, six_g, codes + pix * cstride + b * (B / 2), sf + ln_f4_sf_at(pix, b >> 2, sf_words) + (b & 3));
     }
 }
 
@@ -93,8 +93,9 @@ __global__ void narrow_f16_kernel(const __half* __restrict__ x, int64_t xs, uint
 // One thread per 16 channels of a pixel.
 
 template <int FMT>
-__device__ __forceinline__ void load_16(const uint8_t* codes, const uint8_t* sf, int b16, float g, float (&v)[16]) {
-    const float d = ln_f4_factor<FMT>(sf[FMT == LN_F4 ? b16 : b16 >> 1], g);
+__device__ __forceinline__ void load_16(const uint8_t* codes, const uint8_t* sf, int64_t pix, int64_t sf_words, int b16, float g, float (&v)[16]) {
+    const int b = FMT == LN_F4 ? b16 : b16 >> 1;
+    const float d = ln_f4_factor<FMT>(sf[ln_f4_sf_at(pix, b >> 2, sf_words) + (b & 3)], g);
     const uint2 w = *reinterpret_cast<const uint2*>(codes + b16 * 8);
     uint32_t h[8];
     ln_e2m1x8_to_h2(w.x, *reinterpret_cast<uint32_t(*)[4]>(h));
@@ -108,12 +109,12 @@ __device__ __forceinline__ void load_16(const uint8_t* codes, const uint8_t* sf,
 }
 template <int FMT>
 __global__ void widen_f32_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ sf, float* __restrict__ y, int64_t pixels, int64_t hw, int C, int blocks,
-                                 int64_t cstride, int64_t sf_stride, float g) {
+                                 int64_t cstride, int64_t sf_words, float g) {
     for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < pixels * blocks; i += (int64_t)gridDim.x * blockDim.x) {
         const int64_t pix = i % pixels;
         const int b = (int)(i / pixels);
         float v[16];
-        load_16<FMT>(codes + pix * cstride, sf + pix * sf_stride, b, g, v);
+        load_16<FMT>(codes + pix * cstride, sf, pix, sf_words, b, g, v);
         float* dst = y + (pix / hw * C + b * 16) * hw + pix % hw;
 #pragma unroll
         for (int j = 0; j < 16; ++j)
@@ -122,12 +123,12 @@ __global__ void widen_f32_kernel(const uint8_t* __restrict__ codes, const uint8_
 }
 template <int FMT>
 __global__ void widen_f16_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ sf, __half* __restrict__ y, int64_t ys, int64_t pixels, int C, int blocks,
-                                 int64_t cstride, int64_t sf_stride, float g) {
+                                 int64_t cstride, int64_t sf_words, float g) {
     for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < pixels * blocks; i += (int64_t)gridDim.x * blockDim.x) {
         const int64_t pix = i / blocks;
         const int b = (int)(i - pix * blocks);
         float v[16];
-        load_16<FMT>(codes + pix * cstride, sf + pix * sf_stride, b, g, v);
+        load_16<FMT>(codes + pix * cstride, sf, pix, sf_words, b, g, v);
         uint32_t h[8];
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
@@ -142,7 +143,7 @@ __global__ void widen_f16_kernel(const uint8_t* __restrict__ codes, const uint8_
 }
 // codes (one per byte) and scales in NCHW order
 __global__ void unpack_f4_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ sf, uint8_t* __restrict__ out_codes, uint8_t* __restrict__ out_sf, int64_t n, int64_t hw,
-                                 int C, int sf_blocks, int64_t cstride, int64_t sf_stride) {
+                                 int C, int sf_blocks, int64_t cstride, int64_t sf_words) {
     const int64_t first = n * C * hw, total = first + n * sf_blocks * hw;
     for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
         const int64_t k = i < first ? i : i - first;
@@ -150,7 +151,7 @@ __global__ void unpack_f4_kernel(const uint8_t* __restrict__ codes, const uint8_
         const int64_t p = k % hw, img = k / hw / per;
         const int c = (int)(k / hw % per);
         if (i < first) out_codes[k] = (codes[(img * hw + p) * cstride + c / 2] >> (4 * (c & 1))) & 15;
-        else out_sf[k] = sf[(img * hw + p) * sf_stride + c];
+        else out_sf[k] = sf[ln_f4_sf_at(img * hw + p, c >> 2, sf_words) + (c & 3)];
     }
 }
 
@@ -158,7 +159,7 @@ __global__ void unpack_f4_kernel(const uint8_t* __restrict__ codes, const uint8_
 // One thread block per filter: its largest magnitude, then the blocks of each tap (a filter's scale 0 leaves zero codes).
 template <int FMT>
 __global__ void pack_weights_f4_kernel(const float* __restrict__ w, int C, int k2, int64_t cstride, uint8_t* __restrict__ codes, uint8_t* __restrict__ sf, float* __restrict__ wscale,
-                                       int bk, int cblocks, int words) {
+                                       int64_t sf_words) {
     constexpr int B = FMT == LN_F4 ? 16 : 32;
     const int f = blockIdx.x;
     const float* src = w + (int64_t)f * C * k2;
@@ -174,14 +175,13 @@ __global__ void pack_weights_f4_kernel(const float* __restrict__ w, int C, int k
     float g = 1.0f;
     if (FMT == LN_F4 && amax > 0.0f) g = fminf(fmaxf(__fdiv_rn(amax, 6.0f * 448.0f), 0x1p-100f), 0x1p100f);
     if (threadIdx.x == 0) wscale[f] = g;
-    const int blocks = (int)(cstride * 2 / B), per_kblock = 2 * bk / B;
+    const int blocks = (int)(cstride * 2 / B);
     for (int i = threadIdx.x; i < k2 * blocks; i += blockDim.x) {
         const int tap = i / blocks, b = i - tap * blocks;
         float v[B];
 #pragma unroll
         for (int j = 0; j < B; ++j) v[j] = b * B + j < C ? src[(int64_t)(b * B + j) * k2 + tap] : 0.0f;
-        const int cb = b / per_kblock, in = b - cb * per_kblock;  // k-block of the tap, scale byte inside it
-        const int64_t at = ((((int64_t)(f / 128) * k2 + tap) * cblocks + cb) * words + in / 4) * 512 + (f % 32) * 16 + f / 32 % 4 * 4 + in % 4;
+        const int64_t at = ln_f4_sf_at(f, (int64_t)tap * sf_words + (b >> 2), k2 * sf_words) + (b & 3);
         store_block<FMT>(v, g, 6.0f * g, codes + ((int64_t)f * k2 + tap) * cstride + b * (B / 2), sf + at);
     }
 }
@@ -191,8 +191,8 @@ struct simt_params {
     const uint8_t *x, *xsf, *w, *wsf;
     const float *wscale, *bias;
     void* y;
-    int64_t xs, xsf_stride, ys, total;
-    int C, H, W, F, k, sx, sy, pad, OH, OW, blocks, bk, cblocks, words, act, out_f16;
+    int64_t xs, xsf_words, ys, total;
+    int C, H, W, F, k, sx, sy, pad, OH, OW, blocks, act, out_f16;
     float xscale;
 };
 // One thread per output value, filters fastest.  Takes every geometry.
@@ -216,8 +216,7 @@ __global__ void conv_f4_simt_kernel(const simt_params p) {
                 const uint8_t* xc = p.x + q * p.xs;
                 const uint8_t* wc = p.w + ((int64_t)f * p.k * p.k + tap) * p.xs;
                 for (int b = 0; b < p.blocks; ++b) {
-                    const int per_kblock = 2 * p.bk / B, cb = b / per_kblock, in = b - cb * per_kblock;
-                    const int64_t at = ((((int64_t)(f / 128) * p.k * p.k + tap) * p.cblocks + cb) * p.words + in / 4) * 512 + (f % 32) * 16 + f / 32 % 4 * 4 + in % 4;
+                    const int64_t at = ln_f4_sf_at(f, (int64_t)tap * p.xsf_words + (b >> 2), p.k * p.k * p.xsf_words) + (b & 3), xat = ln_f4_sf_at(q, b >> 2, p.xsf_words) + (b & 3);
                     float sum = 0.0f;  // exact: multiples of 0.25 below 2^11
 #pragma unroll
                     for (int j = 0; j < B / 8; ++j) {
@@ -232,8 +231,8 @@ __global__ void conv_f4_simt_kernel(const simt_params p) {
                         }
                     }
                     // (block scales first: their product is exact for LN_F4, and a sum of zero times it is never zero times infinity)
-                    if (FMT == LN_F4) acc = __fmaf_rn(sum, __fmul_rn(ln_e4m3_value(p.xsf[q * p.xsf_stride + b]), ln_e4m3_value(p.wsf[at])), acc);
-                    else acc = __fmaf_rn(__fmul_rn(sum, ln_e8m0_value(p.xsf[q * p.xsf_stride + b])), ln_e8m0_value(p.wsf[at]), acc);
+                    if (FMT == LN_F4) acc = __fmaf_rn(sum, __fmul_rn(ln_e4m3_value(p.xsf[xat]), ln_e4m3_value(p.wsf[at])), acc);
+                    else acc = __fmaf_rn(__fmul_rn(sum, ln_e8m0_value(p.xsf[xat])), ln_e8m0_value(p.wsf[at]), acc);
                 }
             }
         }
@@ -250,11 +249,11 @@ int narrow_into(ln_ctx* ctx, const ln_tensor* t, ln_tensor* q) {
     uint8_t *codes = (uint8_t*)q->ptr, *sf = (uint8_t*)q->sf;
     const float g = q->scale, six_g = 6.0f * g;
     if (t->dtype == LN_F32) {
-        if (q->dtype == LN_F4) narrow_f32_kernel<LN_F4><<<grid, kThreads, 0, ctx->stream>>>((const float*)t->ptr, codes, sf, pixels, hw, (int)t->c, blocks, q->cstride, q->sf_stride, g, six_g);
-        else narrow_f32_kernel<LN_MX4><<<grid, kThreads, 0, ctx->stream>>>((const float*)t->ptr, codes, sf, pixels, hw, (int)t->c, blocks, q->cstride, q->sf_stride, g, six_g);
+        if (q->dtype == LN_F4) narrow_f32_kernel<LN_F4><<<grid, kThreads, 0, ctx->stream>>>((const float*)t->ptr, codes, sf, pixels, hw, (int)t->c, blocks, q->cstride, q->sf_words, g, six_g);
+        else narrow_f32_kernel<LN_MX4><<<grid, kThreads, 0, ctx->stream>>>((const float*)t->ptr, codes, sf, pixels, hw, (int)t->c, blocks, q->cstride, q->sf_words, g, six_g);
     } else {
-        if (q->dtype == LN_F4) narrow_f16_kernel<LN_F4><<<grid, kThreads, 0, ctx->stream>>>((const __half*)t->ptr, t->cstride / 2, codes, sf, pixels, (int)t->c, blocks, q->cstride, q->sf_stride, g, six_g);
-        else narrow_f16_kernel<LN_MX4><<<grid, kThreads, 0, ctx->stream>>>((const __half*)t->ptr, t->cstride / 2, codes, sf, pixels, (int)t->c, blocks, q->cstride, q->sf_stride, g, six_g);
+        if (q->dtype == LN_F4) narrow_f16_kernel<LN_F4><<<grid, kThreads, 0, ctx->stream>>>((const __half*)t->ptr, t->cstride / 2, codes, sf, pixels, (int)t->c, blocks, q->cstride, q->sf_words, g, six_g);
+        else narrow_f16_kernel<LN_MX4><<<grid, kThreads, 0, ctx->stream>>>((const __half*)t->ptr, t->cstride / 2, codes, sf, pixels, (int)t->c, blocks, q->cstride, q->sf_words, g, six_g);
     }
     return check_launch(ctx, "ln_tensor_narrow_f4");
 }
@@ -298,12 +297,12 @@ int32_t ln_tensor_widen_f4(ln_ctx* ctx, const ln_tensor* t, int32_t dtype, ln_te
         const uint8_t *codes = (const uint8_t*)t->ptr, *sf = (const uint8_t*)t->sf;
         if (dtype == LN_F32) {
             const int blocks = (int)((t->c + 15) / 16), grid = grid_for(ctx, pixels * blocks);
-            if (t->dtype == LN_F4) widen_f32_kernel<LN_F4><<<grid, kThreads, 0, ctx->stream>>>(codes, sf, (float*)y->ptr, pixels, hw, (int)t->c, blocks, t->cstride, t->sf_stride, t->scale);
-            else widen_f32_kernel<LN_MX4><<<grid, kThreads, 0, ctx->stream>>>(codes, sf, (float*)y->ptr, pixels, hw, (int)t->c, blocks, t->cstride, t->sf_stride, 1.0f);
+            if (t->dtype == LN_F4) widen_f32_kernel<LN_F4><<<grid, kThreads, 0, ctx->stream>>>(codes, sf, (float*)y->ptr, pixels, hw, (int)t->c, blocks, t->cstride, t->sf_words, t->scale);
+            else widen_f32_kernel<LN_MX4><<<grid, kThreads, 0, ctx->stream>>>(codes, sf, (float*)y->ptr, pixels, hw, (int)t->c, blocks, t->cstride, t->sf_words, 1.0f);
         } else {
             const int blocks = (int)(y->cstride / 32), grid = grid_for(ctx, pixels * blocks);
-            if (t->dtype == LN_F4) widen_f16_kernel<LN_F4><<<grid, kThreads, 0, ctx->stream>>>(codes, sf, (__half*)y->ptr, y->cstride / 2, pixels, (int)t->c, blocks, t->cstride, t->sf_stride, t->scale);
-            else widen_f16_kernel<LN_MX4><<<grid, kThreads, 0, ctx->stream>>>(codes, sf, (__half*)y->ptr, y->cstride / 2, pixels, (int)t->c, blocks, t->cstride, t->sf_stride, 1.0f);
+            if (t->dtype == LN_F4) widen_f16_kernel<LN_F4><<<grid, kThreads, 0, ctx->stream>>>(codes, sf, (__half*)y->ptr, y->cstride / 2, pixels, (int)t->c, blocks, t->cstride, t->sf_words, t->scale);
+            else widen_f16_kernel<LN_MX4><<<grid, kThreads, 0, ctx->stream>>>(codes, sf, (__half*)y->ptr, y->cstride / 2, pixels, (int)t->c, blocks, t->cstride, t->sf_words, 1.0f);
         }
         rc = check_launch(ctx, who);
         if (rc) { ln_tensor_release(y); return rc; }
@@ -326,7 +325,7 @@ int32_t ln_tensor_download_f4(ln_ctx* ctx, const ln_tensor* t, uint8_t* host_cod
         uint8_t* tmp = (uint8_t*)ln_pool_alloc(ctx, (size_t)(code_count + scales));
         if (!tmp) return LN_ERR_CUDA;
         unpack_f4_kernel<<<grid_for(ctx, code_count + scales), kThreads, 0, ctx->stream>>>((const uint8_t*)t->ptr, (const uint8_t*)t->sf, tmp, tmp + code_count, t->n, hw, (int)t->c, sf_blocks,
-                                                                                         t->cstride, t->sf_stride);
+                                                                                         t->cstride, t->sf_words);
         int rc = check_launch(ctx, who);
         cudaError_t e = cudaSuccess;
         if (rc == LN_OK) {
@@ -353,12 +352,12 @@ int32_t ln_conv_weights_f4(ln_ctx* ctx, const ln_tensor* weights_f32, int64_t fi
     return guarded(ctx, who, [&]() -> int32_t {
         cudaSetDevice(ctx->device);
         const int64_t k2 = kernel_size * kernel_size;
-        const ln_f4_kblocks kb = ln_f4_kblocks_of(dtype, channels);
+        const int64_t sf_words = ln_f4_sf_words(dtype, channels);
         ln_conv_weights* w = new ln_conv_weights();
         w->ctx = ctx; w->dtype = dtype;
         w->filters = filters; w->channels = channels; w->k = kernel_size;
         w->fpad = ln_round_up(filters, 128) + kF4FilterPad; w->cpad = ln_f4_cstride(channels);
-        const size_t sf_bytes = (size_t)(w->fpad / 128 * k2 * kb.cblocks * kb.words * 512);
+        const size_t sf_bytes = (size_t)(w->fpad / 128 * k2 * sf_words * 512);
         w->w = ln_pool_alloc(ctx, (size_t)(filters * k2 * w->cpad));
         w->sf = ln_pool_alloc(ctx, sf_bytes);
         w->wscale = (float*)ln_pool_alloc(ctx, (size_t)filters * 4);
@@ -367,8 +366,8 @@ int32_t ln_conv_weights_f4(ln_ctx* ctx, const ln_tensor* weights_f32, int64_t fi
         const cudaError_t e = cudaMemsetAsync(w->sf, 0, sf_bytes, ctx->stream);
         if (e != cudaSuccess) rc = ln_fail(ctx, LN_ERR_CUDA, "%s: %s", who, cudaGetErrorString(e));
         if (rc == LN_OK) {
-            if (dtype == LN_F4) pack_weights_f4_kernel<LN_F4><<<(int)filters, 256, 0, ctx->stream>>>((const float*)weights_f32->ptr, (int)channels, (int)k2, w->cpad, (uint8_t*)w->w, (uint8_t*)w->sf, w->wscale, kb.bk, kb.cblocks, kb.words);
-            else pack_weights_f4_kernel<LN_MX4><<<(int)filters, 256, 0, ctx->stream>>>((const float*)weights_f32->ptr, (int)channels, (int)k2, w->cpad, (uint8_t*)w->w, (uint8_t*)w->sf, w->wscale, kb.bk, kb.cblocks, kb.words);
+            if (dtype == LN_F4) pack_weights_f4_kernel<LN_F4><<<(int)filters, 256, 0, ctx->stream>>>((const float*)weights_f32->ptr, (int)channels, (int)k2, w->cpad, (uint8_t*)w->w, (uint8_t*)w->sf, w->wscale, sf_words);
+            else pack_weights_f4_kernel<LN_MX4><<<(int)filters, 256, 0, ctx->stream>>>((const float*)weights_f32->ptr, (int)channels, (int)k2, w->cpad, (uint8_t*)w->w, (uint8_t*)w->sf, w->wscale, sf_words);
             rc = check_launch(ctx, who);
         }
         if (rc) { ln_conv_weights_release(w); return rc; }
@@ -420,14 +419,13 @@ int32_t ln_conv2d_bias_act_f4(ln_ctx* ctx, const ln_tensor* x, const ln_conv_wei
             if (e != cudaSuccess) rc = ln_fail(ctx, LN_ERR_CUDA, "%s: %s", who, cudaGetErrorString(e));
         }
         if (rc == LN_OK) {
-            const ln_f4_kblocks kb = ln_f4_kblocks_of(x->dtype, channels);
             const ln_tensor* dst = wide ? wide : y;
             simt_params p;
             p.x = (const uint8_t*)x->ptr; p.xsf = (const uint8_t*)x->sf; p.w = (const uint8_t*)weights->w; p.wsf = (const uint8_t*)weights->sf;
             p.wscale = weights->wscale; p.bias = (const float*)bias->ptr; p.y = dst->ptr;
-            p.xs = x->cstride; p.xsf_stride = x->sf_stride; p.ys = dst->cstride / 2; p.total = x->n * oh * ow * filters;
+            p.xs = x->cstride; p.xsf_words = x->sf_words; p.ys = dst->cstride / 2; p.total = x->n * oh * ow * filters;
             p.C = (int)channels; p.H = (int)input_height; p.W = (int)input_width; p.F = (int)filters; p.k = (int)kernel_size; p.sx = (int)stride_x; p.sy = (int)stride_y; p.pad = (int)padding;
-            p.OH = (int)oh; p.OW = (int)ow; p.blocks = (int)(x->cstride * 2 / ln_f4_block(x->dtype)); p.bk = kb.bk; p.cblocks = kb.cblocks; p.words = kb.words;
+            p.OH = (int)oh; p.OW = (int)ow; p.blocks = (int)(x->cstride * 2 / ln_f4_block(x->dtype));
             p.act = activation; p.out_f16 = dst->dtype == LN_F16; p.xscale = x->scale;
             const int grid = grid_for(ctx, p.total);
             if (x->dtype == LN_F4) {

@@ -4,15 +4,17 @@
 // GEMM view as for the 8-bit types: D[pixel, filter] = sum over (tap, channel block) of X[pixel shifted by the tap, c] * W[filter, tap, c];
 // a tile is 128 output pixels (a TW x TH x TN box; a 1x1 stride-1 convolution is flattened to one row of pixels) by bn filters, a
 // k-block 128 bytes = 256 channels of one tap (fewer where the tensor has fewer): four instructions of 64 channels.
-// Codes come by TMA (taps outside the image are zero filled; stride 2 has one tensor map per parity class of the input).  The scales
-// of the weights lie in memory as the tensor core takes them and come by bulk copies.  Those of the pixels cannot: every tap needs the
-// scales of other pixels in the rows of the tile, so two warps gather them, one lane for the rows l, l + 32, l + 64, l + 96, whose four
-// words it stores transposed as one 16-byte piece per instruction.  The issuing thread copies both from shared memory to TMEM
-// (tcgen05.cp, executed in order with the instructions that read them) right before the k-block that they belong to.
+// Codes come by TMA (taps outside the image are zero filled; stride 2 has one tensor map per parity class of the input).  Block scales
+// lie in memory as the tensor core takes them: those of the weights, and of pixels in their own order, come by bulk copies.  Taps shift
+// the pixels, so there four warps gather words, a lane for the rows l, l + 32, l + 64, l + 96, one 16-byte piece per instruction.  The
+// issuing thread copies both from shared memory to TMEM (tcgen05.cp, executed in order with the instructions that read them) right
+// before the k-block that they belong to.
 //
-// Roles: warp 0 loads, warp 1 issues, warps 2 and 3 gather scales (every second k-block each), 16 epilogue warps.  An accumulator tile is
-// handed out as `subs` units of CH columns; a unit is read into registers whole and its part of TMEM handed back before any arithmetic.
-// TMEM: 416 columns of accumulators (one tile of 256 filters, two of 192, three of 128, six of 64), 2 x 48 of scales.
+// Roles: warp 0 loads, warp 1 issues, warps 2 to 5 gather scales (every fourth k-block each; the ring has at least four stages, so none
+// comes back to a stage whose use before is still to be filled), warps 8 to 15 are the epilogue: two groups of four that take the units
+// of 64 columns of the tiles in turn.  TMEM: 416 columns of accumulators, 2 x 48 of scales.  Two tiles of 192 filters, three of 128 or
+// six of 64 fit; two of 256 overlap by 96 columns (0..255 and 160..415), so their epilogue reads the two units that overlap first and
+// the next tile starts as soon as those are in registers.
 // Every wait is bounded (see ln_umma.h).
 #include <cstdlib>
 
@@ -21,11 +23,13 @@
 
 namespace {
 
-constexpr int kThreadsF4 = 32 * 20;
+constexpr int kThreadsF4 = 32 * 16, kFirstEpilogueWarp = 8, kGatherWarps = 4;
 constexpr int kMaxStagesF4 = 8, kMaxBufsF4 = 6;
+constexpr int CH = 64;  // columns of an epilogue unit
+constexpr int kOverlapBase = 160;  // first column of the second accumulator of 256
 constexpr uint32_t kScaleCols = 416, kScaleSet = 48, kScaleB = 16;  // TMEM columns: two sets of [16 pixels' | 32 filters'] scale words
 constexpr uint32_t kBarBytesF4 = 512;
-constexpr uint32_t kTabBytesF4 = 16 * 512;  // {multiplier, bias} of the columns that a warp is at
+constexpr uint32_t kTabBytesF4 = 8 * 512;  // {multiplier, bias} of the columns that a warp is at
 constexpr int kMaxSmemF4 = 227 * 1024;
 
 struct f4_params {
@@ -35,14 +39,14 @@ struct f4_params {
     void* y;
     uint8_t* ysf;
     int* status;
-    long long ys, ysf_stride;  // bytes per pixel of an NHWC output, of its scales
+    long long ys, ysf_words;  // bytes per pixel of an NHWC output, words of scales
     float xscale, g, six_g;    // tensor scale of the input; of a 4-bit output
-    int sf_stride, cstride;
-    int bk, bn, cblocks, words, wblocks;  // wblocks: groups of 128 filters a tile's scales are in
+    int sf_words, cstride;
+    int bk, bn, cblocks, words;
     int R, S, stride, pad, H, W, N, OH, OW, F, hw;
     int TW, TH, TN, log_tw, log_th, tiles_f, tiles_w, tiles_h, num_tiles;
     unsigned long long magic_f, magic_w, magic_h;
-    int stages, nbuf, subs, act, exact;
+    int stages, nbuf, acc_step, subs, act, exact, flat;
     uint32_t off_b, off_sfa, off_sfb, stage_bytes;
 };
 
@@ -80,10 +84,9 @@ __device__ __forceinline__ void tc_mma_scaled(uint32_t d, uint64_t a, uint64_t b
 // descriptor of 32 rows of 16 bytes (no swizzle, groups of 8 rows 128 bytes apart)
 __device__ __forceinline__ uint64_t scale_desc(uint32_t addr) { return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)(128u >> 4) << 32) | (1ull << 46); }
 
-template <int CH>
-__device__ __forceinline__ void act_all(int act, bool exact, float (&v)[CH]) {
+__device__ __forceinline__ void act_all(int act, bool exact, float (&v)[32]) {
 #define LN_ALL(E, A)                                                       \
-    _Pragma("unroll") for (int i = 0; i < CH; ++i) v[i] = ln_epilogue_act<E>(A, v[i]); \
+    _Pragma("unroll") for (int i = 0; i < 32; ++i) v[i] = ln_epilogue_act<E>(A, v[i]); \
     break;
     switch (act) {
         case LN_ACT_LEAKY: LN_ALL(true, LN_ACT_LEAKY)
@@ -102,6 +105,9 @@ __device__ __forceinline__ void act_all(int act, bool exact, float (&v)[CH]) {
 #undef LN_ALL
 }
 
+__device__ __forceinline__ void store_32(uint8_t* dst, const uint32_t (&v)[8]) {  // a whole sector
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
+}
 // the tile's place: output box origin and first filter
 struct f4_tile {
     int ow0, oh0, n0, f0;
@@ -113,7 +119,7 @@ __device__ __forceinline__ f4_tile tile_at(const f4_params& p, int unit) {
     return {tw * p.TW, th * p.TH, tn * p.TN, tf * p.bn};
 }
 
-template <int FMT, int OUT, int CH>
+template <int FMT, int OUT, int WBLOCKS>
 __global__ void __launch_bounds__(kThreadsF4, 1) f4_umma_kernel(const __grid_constant__ f4_params p) {
     extern __shared__ uint8_t smem_raw[];
     const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -122,20 +128,23 @@ __global__ void __launch_bounds__(kThreadsF4, 1) f4_umma_kernel(const __grid_con
     auto empty_bar = [&](int s) { return bar_base + 8u * (kMaxStagesF4 + s); };
     auto tfull_bar = [&](int b) { return bar_base + 8u * (2 * kMaxStagesF4 + b); };
     auto tempty_bar = [&](int b) { return bar_base + 8u * (2 * kMaxStagesF4 + kMaxBufsF4 + b); };
-    volatile uint32_t* tmem_slot = (volatile uint32_t*)(smem_raw + (bar_base - smem_u32(smem_raw)) + 8u * (2 * kMaxStagesF4 + 2 * kMaxBufsF4));
+    auto early_bar = [&](int b) { return bar_base + 8u * (2 * kMaxStagesF4 + 2 * kMaxBufsF4 + b); };  // (overlapping accumulators)
+    volatile uint32_t* tmem_slot = (volatile uint32_t*)(smem_raw + (bar_base - smem_u32(smem_raw)) + 8u * (2 * kMaxStagesF4 + 2 * kMaxBufsF4 + 2));
     volatile int* abort_flag = (volatile int*)(tmem_slot + 2);
     const uint32_t tab_base = bar_base + kBarBytesF4;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < p.stages; ++s) {
-            mbar_init(full_bar(s), 2);  // the loader (with the copies' bytes) and the warp that gathers scales
+            mbar_init(full_bar(s), p.flat ? 1 : 2);  // the loader (with the copies' bytes) and a warp that gathers scales
             mbar_init(empty_bar(s), 1);
         }
         for (int b = 0; b < p.nbuf; ++b) {
             mbar_init(tfull_bar(b), 1);
             mbar_init(tempty_bar(b), 4 * p.subs);
         }
+        mbar_init(early_bar(0), 8);
+        mbar_init(early_bar(1), 8);
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -148,17 +157,19 @@ __global__ void __launch_bounds__(kThreadsF4, 1) f4_umma_kernel(const __grid_con
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
     const int kblocks = p.R * p.S * p.cblocks, step = (int)gridDim.x;
+    const bool overlap = p.bn == 256;
 
     if (warp == 0) {
         // ------------------------------------------------------------------ loads
         if (lane == 0) {
-            const uint32_t bytes = (uint32_t)(128 + p.bn) * p.bk + (uint32_t)p.wblocks * p.words * 512u;
+            const uint32_t sf_bytes = (uint32_t)p.words * 512u, bytes = (uint32_t)(128 + p.bn) * p.bk + (WBLOCKS + (p.flat ? 1u : 0u)) * sf_bytes;
             int stage = 0;
             uint32_t phase = 0;
             bool ok = true;
             for (int unit = (int)blockIdx.x; ok && unit < p.num_tiles; unit += step) {
                 const f4_tile t = tile_at(p, unit);
-                const uint8_t* wsf = p.wsf + (size_t)(t.f0 >> 7) * kblocks * p.words * 512u;
+                const uint8_t* wsf = p.wsf + (size_t)(t.f0 >> 7) * kblocks * sf_bytes;
+                const uint8_t* xsf = p.xsf + (size_t)(t.ow0 >> 7) * kblocks * sf_bytes;  // (flat)
                 int wcol = 0, kb = 0;
                 for (int r = 0; ok && r < p.R; ++r)
                     for (int s = 0; ok && s < p.S; ++s, wcol += p.cstride) {
@@ -175,8 +186,9 @@ __global__ void __launch_bounds__(kThreadsF4, 1) f4_umma_kernel(const __grid_con
                             mbar_arrive_expect_tx(bar, bytes);
                             tma_load_4d(at, &p.tmA[map], c0, t.ow0 + tx, t.oh0 + ty, t.n0, bar);
                             tma_load_2d(at + p.off_b, &p.tmB, wcol + c0, t.f0, bar);
-                            for (int b = 0; b < p.wblocks; ++b)
-                                bulk_load(at + p.off_sfb + (uint32_t)(b * p.words) * 512u, wsf + ((size_t)b * kblocks + kb) * p.words * 512u, (uint32_t)p.words * 512u, bar);
+#pragma unroll
+                            for (int b = 0; b < WBLOCKS; ++b) bulk_load(at + p.off_sfb + b * sf_bytes, wsf + ((size_t)b * kblocks + kb) * sf_bytes, sf_bytes, bar);
+                            if (p.flat) bulk_load(at + p.off_sfa, xsf + (size_t)kb * sf_bytes, sf_bytes, bar);
                             if (++stage == p.stages) { stage = 0; phase ^= 1u; }
                         }
                     }
@@ -189,14 +201,17 @@ __global__ void __launch_bounds__(kThreadsF4, 1) f4_umma_kernel(const __grid_con
         // E2M1 operands (bits 7, 10: type 1), N / 8, scale type (bit 23: 1 = E8M0), M / 128, K-major; the scale ids go to bits 4 and 29
         const uint32_t idesc = (1u << 7) | (1u << 10) | ((uint32_t)(p.bn >> 3) << 17) | ((FMT == LN_MX4 ? 1u : 0u) << 23) | (1u << 27);
         const uint64_t desc_base = make_smem_desc(0u, p.bk);
+        constexpr int kWords = FMT == LN_MX4 ? 2 : 4, kBlocks = WBLOCKS;  // of a whole k-block
+        const uint64_t sfa_desc = scale_desc(p.off_sfa), sfb_desc = scale_desc(p.off_sfb);
         int stage = 0, t = 0;
         uint32_t phase = 0, set = 0;
         bool ok = true;
         for (int unit = (int)blockIdx.x; ok && unit < p.num_tiles; unit += step, ++t) {
             const int buf = t % p.nbuf;
             if (!(ok = warp_wait(tempty_bar(buf), (uint32_t)((t / p.nbuf) & 1) ^ 1u, abort_flag, p.status, LN_STATUS_MMA_TIMEOUT))) break;
+            if (overlap && t > 0 && !(ok = warp_wait(early_bar(buf ^ 1), (uint32_t)(((t - 1) >> 1) & 1), abort_flag, p.status, LN_STATUS_MMA_TIMEOUT))) break;
             tc_fence_after();
-            const uint32_t d = tmem_base + (uint32_t)(buf * p.bn);
+            const uint32_t d = tmem_base + (uint32_t)(buf * p.acc_step);
             const int tf = unit - fast_div(unit, p.magic_f) * p.tiles_f;
             const uint32_t shift = (uint32_t)((tf * p.bn & 127) >> 5);  // first column of the tile's filters inside their group of 128
             int c0 = 0;
@@ -206,17 +221,34 @@ __global__ void __launch_bounds__(kThreadsF4, 1) f4_umma_kernel(const __grid_con
                 const uint32_t at = smem_base + (uint32_t)stage * p.stage_bytes;
                 const uint32_t sfa = tmem_base + kScaleCols + set * kScaleSet, sfb = sfa + kScaleB;
                 const int left = p.cstride - c0, n = (left < p.bk ? left : p.bk) >> 5;  // instructions of this k-block
-                if (leader) {
+                const uint64_t a_desc = desc_base + (at >> 4), b_desc = desc_base + ((at + p.off_b) >> 4);
+                if (n == 4) {
+                    // a whole k-block of 128 bytes, unrolled with constant offsets: as loops with run-time bounds the copies and
+                    // instructions of a k-block took their thread 1100 cycles, this way 420, less than the 530 that they run for
+                    if (leader) {
+#pragma unroll
+                        for (int j = 0; j < kWords; ++j) {
+                            tc_copy_scales(sfa + 4u * j, sfa_desc + ((at + 512u * j) >> 4));
+#pragma unroll
+                            for (int b = 0; b < kBlocks; ++b) tc_copy_scales(sfb + 4u * (j * kBlocks + b), sfb_desc + ((at + 512u * (b * kWords + j)) >> 4));
+                        }
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const uint32_t word = FMT == LN_MX4 ? i >> 1 : i, id = FMT == LN_MX4 ? (uint32_t)(i & 1) * 2u : 0u;
+                            tc_mma_scaled<FMT>(d, a_desc + 2u * i, b_desc + 2u * i, idesc | (id << 4) | (id << 29), sfa + 4u * word, sfb + 4u * word * kBlocks + shift, i ? 1u : (uint32_t)(kb != 0));
+                        }
+                        tc_commit(empty_bar(stage));
+                    }
+                } else if (leader) {
                     for (int j = 0; j < p.words; ++j) {
                         tc_copy_scales(sfa + 4u * j, scale_desc(at + p.off_sfa + 512u * j));
-                        for (int b = 0; b < p.wblocks; ++b) tc_copy_scales(sfb + 4u * (j * p.wblocks + b), scale_desc(at + p.off_sfb + 512u * (b * p.words + j)));
+                        for (int b = 0; b < WBLOCKS; ++b) tc_copy_scales(sfb + 4u * (j * WBLOCKS + b), scale_desc(at + p.off_sfb + 512u * (b * p.words + j)));
                     }
-                    const uint64_t a_desc = desc_base + (at >> 4), b_desc = desc_base + ((at + p.off_b) >> 4);
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
                         if (i < n) {
                             const uint32_t word = FMT == LN_MX4 ? i >> 1 : i, id = FMT == LN_MX4 ? (uint32_t)(i & 1) * 2u : 0u;
-                            tc_mma_scaled<FMT>(d, a_desc + 2u * i, b_desc + 2u * i, idesc | (id << 4) | (id << 29), sfa + 4u * word, sfb + 4u * word * p.wblocks + shift, (uint32_t)((kb | i) != 0));
+                            tc_mma_scaled<FMT>(d, a_desc + 2u * i, b_desc + 2u * i, idesc | (id << 4) | (id << 29), sfa + 4u * word, sfb + 4u * word * WBLOCKS + shift, (uint32_t)((kb | i) != 0));
                         }
                     tc_commit(empty_bar(stage));
                 }
@@ -230,9 +262,8 @@ __global__ void __launch_bounds__(kThreadsF4, 1) f4_umma_kernel(const __grid_con
             if (leader) tc_commit(tfull_bar(buf));
             __syncwarp();
         }
-    } else if (warp < 4) {
-        // ------------------------------------------------------------------ scales of the pixels
-        const int which = warp - 2;
+    } else if (warp < 2 + kGatherWarps) {
+        // ------------------------------------------------------------------ scales of the pixels under shifted taps
         int unit = (int)blockIdx.x, r = 0, s = 0, cb = 0;
         int iy0[4], ix0[4], img[4];
         auto enter_tile = [&]() {
@@ -260,62 +291,58 @@ __global__ void __launch_bounds__(kThreadsF4, 1) f4_umma_kernel(const __grid_con
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
                 const int y = iy0[g] + r, x = ix0[g] + s;
-                uint4 q = make_uint4(0u, 0u, 0u, 0u);
-                if (y >= 0 && y < p.H && x >= 0 && x < p.W && img[g] < p.N) {
-                    const uint8_t* src = p.xsf + (((long long)img[g] * p.H + y) * p.W + x) * p.sf_stride + (long long)cb * p.words * 4;
-                    if (p.words == 4) q = __ldg((const uint4*)src);
-                    else if (p.words == 2) { const uint2 h = __ldg((const uint2*)src); q.x = h.x; q.y = h.y; }
-                    else q.x = __ldg((const uint32_t*)src);
-                }
-                v[g][0] = q.x; v[g][1] = q.y; v[g][2] = q.z; v[g][3] = q.w;
+                const bool inside = y >= 0 && y < p.H && x >= 0 && x < p.W && img[g] < p.N;
+                const uint8_t* src = p.xsf + (inside ? ln_f4_sf_at((img[g] * p.H + y) * p.W + x, cb * p.words, p.sf_words) : 0);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[g][j] = inside && j < p.words ? __ldg((const uint32_t*)(src + 512 * j)) : 0u;
             }
         };
-        enter_tile();
-        if (which == 1) advance();
-        int stage = which == 1 ? 1 % p.stages : 0;
-        uint32_t phase = which == 1 && p.stages == 1 ? 1u : 0u;
-        uint32_t now[4][4], next[4][4];
-        bool more = unit < p.num_tiles, ok = true;
-        if (more) fetch(now);
-        while (more && ok) {
-            advance();
-            advance();
-            more = unit < p.num_tiles;
-            if (more) fetch(next);
-            if (!(ok = warp_wait(empty_bar(stage), phase ^ 1u, abort_flag, p.status, LN_STATUS_PRODUCER_TIMEOUT))) break;
-            const uint32_t dst = smem_base + (uint32_t)stage * p.stage_bytes + p.off_sfa + 16u * lane;
+        if (!p.flat) {
+            enter_tile();
+            for (int i = 2; i < warp; ++i) advance();
+            int stage = warp - 2;  // (fewer than stages)
+            uint32_t phase = 0;
+            uint32_t now[4][4], next[4][4];
+            bool more = unit < p.num_tiles, ok = true;
+            if (more) fetch(now);
+            while (more && ok) {
+                for (int i = 0; i < kGatherWarps; ++i) advance();
+                more = unit < p.num_tiles;
+                if (more) fetch(next);
+                if (!(ok = warp_wait(empty_bar(stage), phase ^ 1u, abort_flag, p.status, LN_STATUS_PRODUCER_TIMEOUT))) break;
+                const uint32_t dst = smem_base + (uint32_t)stage * p.stage_bytes + p.off_sfa + 16u * lane;
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (j < p.words)
-                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + 512u * j), "r"(now[0][j]), "r"(now[1][j]), "r"(now[2][j]), "r"(now[3][j]) : "memory");
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) mbar_arrive(full_bar(stage));
-            stage += 2;
-            if (stage >= p.stages) { stage -= p.stages; phase ^= 1u; }
+                for (int j = 0; j < 4; ++j)
+                    if (j < p.words)
+                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + 512u * j), "r"(now[0][j]), "r"(now[1][j]), "r"(now[2][j]), "r"(now[3][j]) : "memory");
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(full_bar(stage));
+                stage += kGatherWarps;
+                if (stage >= p.stages) { stage -= p.stages; phase ^= 1u; }
 #pragma unroll
-            for (int g = 0; g < 4; ++g)
+                for (int g = 0; g < 4; ++g)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) now[g][j] = next[g][j];
+                    for (int j = 0; j < 4; ++j) now[g][j] = next[g][j];
+            }
         }
-    } else {
+    } else if (warp >= kFirstEpilogueWarp) {
         // ------------------------------------------------------------------ epilogue
-        // Units (tile, sub) in order; group g takes those with number % groups == g.  Never more groups than nbuf * subs: a group that
-        // waits for a tile's accumulator has finished a unit of the tile nbuf before it or a later one, so the parity is unambiguous.
-        const int quad = warp & 3, group = (warp - 4) >> 2;
-        const int groups = p.nbuf * p.subs < 4 ? p.nbuf * p.subs : 4;
+        // Group g takes the units with number % 2 == g.  (nbuf * subs >= 2: a group that waits for a tile's accumulator has finished a unit
+        // of the tile nbuf before it or a later one, so the parity is unambiguous.)
+        const int quad = warp & 3, group = (warp - kFirstEpilogueWarp) >> 2;
         const int row = quad * 32 + lane, pw = row & (p.TW - 1), ph = (row >> p.log_tw) & (p.TH - 1), pn = row >> (p.log_tw + p.log_th);
-        const uint32_t tab = tab_base + (uint32_t)(warp - 4) * 512u;
+        const uint32_t tab = tab_base + (uint32_t)(warp - kFirstEpilogueWarp) * 512u;
         int t = 0, turn = 0;
         bool ok = true;
-        for (int unit = (int)blockIdx.x; ok && group < groups && unit < p.num_tiles; unit += step, ++t)
-            for (int sub = 0; ok && sub < p.subs; ++sub, turn = turn + 1 == groups ? 0 : turn + 1) {
+        for (int unit = (int)blockIdx.x; ok && unit < p.num_tiles; unit += step, ++t)
+            for (int order = 0; ok && order < p.subs; ++order, turn ^= 1) {
                 if (turn != group) continue;
                 const f4_tile at = tile_at(p, unit);
+                const int buf = t % p.nbuf, sub = overlap && buf == 0 ? order ^ 2 : order;  // (what overlaps the other accumulator first)
                 const int ow = at.ow0 + pw, oh = at.oh0 + ph, n = at.n0 + pn, f0 = at.f0 + sub * CH;
                 const bool valid = ow < p.OW && oh < p.OH && n < p.N;
                 const long long pix = ((long long)n * p.OH + oh) * p.OW + ow;
-                const int buf = t % p.nbuf;
                 __syncwarp();  // (the table of the unit before has been read)
 #pragma unroll
                 for (int i = lane; i < CH; i += 32) {
@@ -326,59 +353,69 @@ __global__ void __launch_bounds__(kThreadsF4, 1) f4_umma_kernel(const __grid_con
                 __syncwarp();
                 if (!(ok = warp_wait(tfull_bar(buf), (uint32_t)((t / p.nbuf) & 1), abort_flag, p.status, LN_STATUS_EPILOGUE_TIMEOUT))) break;
                 tc_fence_after();
-                const uint32_t taddr = tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(buf * p.bn + sub * CH);
+                const uint32_t taddr = tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(buf * p.acc_step + sub * CH);
                 uint32_t acc[CH / 32][32];
 #pragma unroll
                 for (int c = 0; c < CH / 32; ++c) tmem_ld_32x32(taddr + 32u * c, acc[c]);
                 tmem_ld_wait();
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(tempty_bar(buf));
-                if (f0 >= p.F && !(OUT == LN_OUT_Q && f0 < ((p.F + 63) & ~63))) continue;  // nothing but padding (the columns of a tile that no filter has)
-                float v[CH];
-#pragma unroll
-                for (int i = 0; i < CH; i += 2) {
-                    float4 e;  // (volatile: the table is another one for every unit)
-                    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(e.x), "=f"(e.y), "=f"(e.z), "=f"(e.w) : "r"(tab + 8u * i) : "memory");
-                    v[i] = __fmaf_rn(__uint_as_float(acc[i >> 5][i & 31]), e.x, e.y);
-                    v[i + 1] = __fmaf_rn(__uint_as_float(acc[i >> 5][(i & 31) + 1]), e.z, e.w);
+                if (lane == 0) {
+                    mbar_arrive(tempty_bar(buf));
+                    if (overlap && order < 2) mbar_arrive(early_bar(buf));
                 }
-                act_all<CH>(p.act, p.exact != 0, v);
-                if (f0 + CH > p.F) {
+                if (f0 >= p.F) continue;  // nothing but padding
+                uint32_t sf = 0;
 #pragma unroll
-                    for (int i = 0; i < CH; ++i)
-                        if (f0 + i >= p.F) v[i] = 0.0f;
-                }
-                if (!valid) continue;
-                if (OUT == LN_OUT_F32) {
-                    const long long img = pix / p.hw;
-                    float* dst = (float*)p.y + (img * p.F + f0) * p.hw + (pix - img * p.hw);
+                for (int c0 = 0; c0 < CH; c0 += 32) {
+                    if (f0 + c0 >= p.F && OUT != LN_OUT_Q) break;  // (binary16 channels are padded to 32, 4-bit ones to 64)
+                    float v[32];
 #pragma unroll
-                    for (int i = 0; i < CH; ++i)
-                        if (f0 + i < p.F) dst[(long long)i * p.hw] = v[i];
-                } else if (OUT == LN_OUT_F16) {
-                    uint4* dst = (uint4*)((uint8_t*)p.y + pix * p.ys + 2 * f0);
-#pragma unroll
-                    for (int c = 0; c < CH; c += 8) {
-                        if ((c & 31) == 0 && f0 + c >= p.F) break;  // (channels are padded to 32)
-                        uint32_t h[4];
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const __half2 q = __floats2half2_rn(v[c + 2 * i], v[c + 2 * i + 1]);
-                            h[i] = *reinterpret_cast<const uint32_t*>(&q);
-                        }
-                        dst[c >> 3] = make_uint4(h[0], h[1], h[2], h[3]);
+                    for (int i = 0; i < 32; i += 2) {
+                        float4 e;  // (volatile: the table is another one for every unit)
+                        asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(e.x), "=f"(e.y), "=f"(e.z), "=f"(e.w) : "r"(tab + 8u * (c0 + i)) : "memory");
+                        v[i] = __fmaf_rn(__uint_as_float(acc[c0 / 32][i]), e.x, e.y);
+                        v[i + 1] = __fmaf_rn(__uint_as_float(acc[c0 / 32][i + 1]), e.z, e.w);
                     }
-                } else {
-                    constexpr int B = FMT == LN_F4 ? 16 : 32;
-                    uint8_t* dst = (uint8_t*)p.y + pix * p.ys + f0 / 2;
-                    uint8_t* sf = p.ysf + pix * p.ysf_stride + f0 / B;
+                    act_all(p.act, p.exact != 0, v);
+                    if (f0 + c0 + 32 > p.F) {
 #pragma unroll
-                    for (int c = 0; c < CH; c += 32) {
+                        for (int i = 0; i < 32; ++i)
+                            if (f0 + c0 + i >= p.F) v[i] = 0.0f;
+                    }
+                    if (OUT == LN_OUT_F32) {
+                        if (valid) {
+                            const long long img = pix / p.hw;
+                            float* dst = (float*)p.y + (img * p.F + f0 + c0) * p.hw + (pix - img * p.hw);
+#pragma unroll
+                            for (int i = 0; i < 32; ++i)
+                                if (f0 + c0 + i < p.F) dst[(long long)i * p.hw] = v[i];
+                        }
+                    } else if (OUT == LN_OUT_F16) {
+                        uint32_t h[2][8];
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            const __half2 q = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+                            h[i >> 3][i & 7] = *reinterpret_cast<const uint32_t*>(&q);
+                        }
+                        if (valid) {
+                            uint8_t* dst = (uint8_t*)p.y + pix * p.ys + 2 * (f0 + c0);
+                            store_32(dst, h[0]);
+                            store_32(dst + 32, h[1]);
+                        }
+                    } else {
+                        constexpr int B = FMT == LN_F4 ? 16 : 32;
                         uint32_t q[4];
 #pragma unroll
-                        for (int b = 0; b < 32 / B; ++b) sf[c / B + b] = (uint8_t)ln_f4_quantise<FMT>(v + c + b * B, p.g, p.six_g, q + b * B / 8);
-                        *(uint4*)(dst + c / 2) = make_uint4(q[0], q[1], q[2], q[3]);
+                        for (int b = 0; b < 32 / B; ++b) sf |= ln_f4_quantise<FMT>(v + b * B, p.g, p.six_g, q + b * B / 8) << (8 * (c0 / B + b));
+                        if (valid) {
+                            *(uint4*)((uint8_t*)p.y + pix * p.ys + (f0 + c0) / 2) = make_uint4(q[0], q[1], q[2], q[3]);
+                            uint8_t* at_sf = p.ysf + ln_f4_sf_at(pix, f0 / (4 * B), p.ysf_words);
+                            if (c0 + 32 == CH) {
+                                if (FMT == LN_F4) *(uint32_t*)at_sf = sf;
+                                else *(uint16_t*)(at_sf + f0 / B % 4) = (uint16_t)sf;
+                            }
+                        }
                     }
                 }
             }
@@ -414,7 +451,7 @@ cudaError_t launch(ln_ctx* ctx, const f4_params& p, int grid, size_t smem) {
         k<<<grid, kThreadsF4, smem, ctx->stream>>>(p);
         return cudaGetLastError();
     };
-    return p.bn >= 192 ? go(f4_umma_kernel<FMT, OUT, 64>) : go(f4_umma_kernel<FMT, OUT, 32>);
+    return p.bn > 128 ? go(f4_umma_kernel<FMT, OUT, 2>) : go(f4_umma_kernel<FMT, OUT, 1>);
 }
 
 }  // namespace
@@ -441,7 +478,7 @@ int ln_f4_umma_launch(ln_ctx* ctx, const ln_f4_conv& c) {
     p.F = (int)y.c; p.hw = (int)(y.h * y.w);
     p.R = p.S = c.k; p.stride = c.stride; p.pad = c.pad;
     p.bk = kb.bk; p.cblocks = kb.cblocks; p.words = kb.words;
-    p.cstride = (int)x.cstride; p.sf_stride = (int)x.sf_stride;
+    p.cstride = (int)x.cstride; p.sf_words = (int)x.sf_words;
     // box of 128 output pixels: the fewest tiles, ties to the widest
     int64_t best = -1;
     for (int lw = 0; lw <= 7; ++lw)
@@ -465,9 +502,11 @@ int ln_f4_umma_launch(ln_ctx* ctx, const ln_f4_conv& c) {
         for (int bn : cand)
             if (atoi(e) == bn) p.bn = bn;
     }
-    p.wblocks = p.bn > 128 ? 2 : 1;
-    p.nbuf = (int)kScaleCols / p.bn;
-    p.subs = p.bn >= 192 ? p.bn / 64 : p.bn / 32;
+    const int wblocks = p.bn > 128 ? 2 : 1;
+    p.nbuf = p.bn == 256 ? 2 : (int)kScaleCols / p.bn;
+    p.acc_step = p.bn == 256 ? kOverlapBase : p.bn;
+    p.subs = p.bn / CH;
+    p.flat = flat ? 1 : 0;
     p.tiles_f = (p.F + p.bn - 1) / p.bn; p.tiles_w = (p.OW + p.TW - 1) / p.TW; p.tiles_h = (p.OH + p.TH - 1) / p.TH;
     const int64_t num_tiles = best * p.tiles_f;
     if (num_tiles >= (1 << 20)) return ln_fail(ctx, LN_ERR_UNSUPPORTED, "%s: %lld tiles", who, (long long)num_tiles);
@@ -477,12 +516,12 @@ int ln_f4_umma_launch(ln_ctx* ctx, const ln_f4_conv& c) {
     p.off_b = 128u * p.bk;
     p.off_sfa = p.off_b + (uint32_t)p.bn * p.bk;
     p.off_sfb = p.off_sfa + (uint32_t)p.words * 512u;
-    p.stage_bytes = (uint32_t)ln_round_up(p.off_sfb + (uint32_t)(p.words * p.wblocks) * 512u, 1024);
+    p.stage_bytes = (uint32_t)ln_round_up(p.off_sfb + (uint32_t)(p.words * wblocks) * 512u, 1024);
     p.stages = (int)((kMaxSmemF4 - 1024 - kBarBytesF4 - kTabBytesF4) / p.stage_bytes);
     if (p.stages > kMaxStagesF4) p.stages = kMaxStagesF4;
     const size_t smem = 1024 + (size_t)p.stages * p.stage_bytes + kBarBytesF4 + kTabBytesF4;
     p.xsf = (const uint8_t*)x.sf; p.wsf = (const uint8_t*)c.w->sf; p.wscale = c.w->wscale; p.bias = c.bias;
-    p.y = y.ptr; p.ys = y.cstride; p.ysf = (uint8_t*)y.sf; p.ysf_stride = y.sf_stride;
+    p.y = y.ptr; p.ys = y.cstride; p.ysf = (uint8_t*)y.sf; p.ysf_words = y.sf_words;
     p.xscale = x.scale; p.g = y.scale; p.six_g = 6.0f * y.scale;
     p.act = c.act; p.exact = ctx->exact_epilogue ? 1 : 0;
     p.status = ctx->h_status;

@@ -90,7 +90,7 @@ static size_t storage_bytes(int dtype, int64_t n, int64_t c, int64_t h, int64_t 
     }
     if (ln_is_f4(dtype)) {  // NHWC, two codes per byte, channels padded to 64; then the block scales of all pixels
         *cstride = ln_f4_cstride(c);
-        return (size_t)(n * h * w * (*cstride + ln_f4_sf_stride(dtype, c)));
+        return (size_t)(ln_round_up(n * h * w * *cstride, 128) + ln_f4_sf_bytes(dtype, n * h * w, c));
     }
     *cstride = 0;
     return (size_t)(n * c * h * w) * 4;
@@ -111,8 +111,8 @@ ln_tensor* ln_tensor_new(ln_ctx* ctx, int dtype, int64_t n, int64_t c, int64_t h
     if (!t->base) { delete t; return nullptr; }
     t->ptr = t->base;
     if (ln_is_f4(dtype)) {
-        t->sf = (char*)t->ptr + n * h * w * t->cstride;
-        t->sf_stride = ln_f4_sf_stride(dtype, c);
+        t->sf = (char*)t->ptr + ln_round_up(n * h * w * t->cstride, 128);
+        t->sf_words = ln_f4_sf_words(dtype, c);
     }
     return t;
 }
