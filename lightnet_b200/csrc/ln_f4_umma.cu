@@ -10,11 +10,11 @@
 // issuing thread copies both from shared memory to TMEM (tcgen05.cp, executed in order with the instructions that read them) right
 // before the k-block that they belong to.
 //
-// Roles: warp 0 loads, warp 1 issues, warps 2 to 5 gather scales (every fourth k-block each; the ring has at least four stages, so none
-// comes back to a stage whose use before is still to be filled), warps 8 to 15 are the epilogue: two groups of four that take the units
-// of 64 columns of the tiles in turn.  TMEM: 416 columns of accumulators, 2 x 48 of scales.  Two tiles of 192 filters, three of 128 or
-// six of 64 fit; two of 256 overlap by 96 columns (0..255 and 160..415), so their epilogue reads the two units that overlap first and
-// the next tile starts as soon as those are in registers.
+// Roles: warps 0 and 6 load (pixels; weights), warp 1 issues, warps 2 to 5 gather scales (every fourth k-block each; the ring has at
+// least four stages, so none comes back to a stage whose use before is still to be filled), warps 8 to 23 are the epilogue: four groups
+// of four that take the units of 32 columns of the tiles in turn.  TMEM: 416 columns of accumulators, 2 x 48 of scales.  Two tiles of
+// 192 filters, three of 128 or six of 64 fit; two of 256 overlap by 96 columns (0..255 and 160..415), so their epilogue reads the four
+// units that hold the overlap first and the next tile starts as soon as those are in registers.
 // Every wait is bounded (see ln_umma.h).
 #include <cstdlib>
 
@@ -23,13 +23,13 @@
 
 namespace {
 
-constexpr int kThreadsF4 = 32 * 16, kFirstEpilogueWarp = 8, kGatherWarps = 4;
+constexpr int kThreadsF4 = 32 * 24, kFirstEpilogueWarp = 8, kGatherWarps = 4;
 constexpr int kMaxStagesF4 = 8, kMaxBufsF4 = 6;
-constexpr int CH = 64;  // columns of an epilogue unit
+constexpr int CH = 32;  // columns of an epilogue unit
 constexpr int kOverlapBase = 160;  // first column of the second accumulator of 256
 constexpr uint32_t kScaleCols = 416, kScaleSet = 48, kScaleB = 16;  // TMEM columns: two sets of [16 pixels' | 32 filters'] scale words
 constexpr uint32_t kBarBytesF4 = 512;
-constexpr uint32_t kTabBytesF4 = 8 * 512;  // {multiplier, bias} of the columns that a warp is at
+constexpr uint32_t kTabBytesF4 = 16 * 256;  // {multiplier, bias} of the columns that a warp is at
 constexpr int kMaxSmemF4 = 227 * 1024;
 
 struct f4_params {
@@ -136,15 +136,15 @@ __global__ void __launch_bounds__(kThreadsF4, 1) f4_umma_kernel(const __grid_con
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < p.stages; ++s) {
-            mbar_init(full_bar(s), p.flat ? 1 : 2);  // the loader (with the copies' bytes) and a warp that gathers scales
+            mbar_init(full_bar(s), p.flat ? 2 : 3);  // the two loaders (with their copies' bytes) and a warp that gathers scales
             mbar_init(empty_bar(s), 1);
         }
         for (int b = 0; b < p.nbuf; ++b) {
             mbar_init(tfull_bar(b), 1);
             mbar_init(tempty_bar(b), 4 * p.subs);
         }
-        mbar_init(early_bar(0), 8);
-        mbar_init(early_bar(1), 8);
+        mbar_init(early_bar(0), 16);
+        mbar_init(early_bar(1), 16);
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -160,41 +160,63 @@ __global__ void __launch_bounds__(kThreadsF4, 1) f4_umma_kernel(const __grid_con
     const bool overlap = p.bn == 256;
 
     if (warp == 0) {
-        // ------------------------------------------------------------------ loads
-        if (lane == 0) {
-            const uint32_t sf_bytes = (uint32_t)p.words * 512u, bytes = (uint32_t)(128 + p.bn) * p.bk + (WBLOCKS + (p.flat ? 1u : 0u)) * sf_bytes;
-            int stage = 0;
-            uint32_t phase = 0;
-            bool ok = true;
-            for (int unit = (int)blockIdx.x; ok && unit < p.num_tiles; unit += step) {
-                const f4_tile t = tile_at(p, unit);
-                const uint8_t* wsf = p.wsf + (size_t)(t.f0 >> 7) * kblocks * sf_bytes;
-                const uint8_t* xsf = p.xsf + (size_t)(t.ow0 >> 7) * kblocks * sf_bytes;  // (flat)
-                int wcol = 0, kb = 0;
-                for (int r = 0; ok && r < p.R; ++r)
-                    for (int s = 0; ok && s < p.S; ++s, wcol += p.cstride) {
-                        int ty = r - p.pad, tx = s - p.pad, map = 0;
-                        if (p.stride == 2) {
-                            const int py = ty & 1, px = tx & 1;  // parity class of the tap
-                            ty = (ty - py) >> 1;
-                            tx = (tx - px) >> 1;
-                            map = py * 2 + px;
-                        }
-                        for (int c0 = 0; c0 < p.cstride; c0 += p.bk, ++kb) {
-                            if (!(ok = mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag, p.status, LN_STATUS_PRODUCER_TIMEOUT))) break;
+        // ------------------------------------------------------------------ loads of the pixels (whole warps walk these loops; one lane issues)
+        const bool leader = elect_one();
+        const uint32_t sf_bytes = (uint32_t)p.words * 512u, bytes = 128u * p.bk + (p.flat ? sf_bytes : 0u);
+        int stage = 0;
+        uint32_t phase = 0;
+        bool ok = true;
+        for (int unit = (int)blockIdx.x; ok && unit < p.num_tiles; unit += step) {
+            const f4_tile t = tile_at(p, unit);
+            const uint8_t* xsf = p.xsf + (size_t)(t.ow0 >> 7) * kblocks * sf_bytes;  // (flat)
+            for (int r = 0; ok && r < p.R; ++r)
+                for (int s = 0; ok && s < p.S; ++s) {
+                    int ty = r - p.pad, tx = s - p.pad, map = 0;
+                    if (p.stride == 2) {
+                        const int py = ty & 1, px = tx & 1;  // parity class of the tap
+                        ty = (ty - py) >> 1;
+                        tx = (tx - px) >> 1;
+                        map = py * 2 + px;
+                    }
+                    for (int c0 = 0; c0 < p.cstride; c0 += p.bk, xsf += sf_bytes) {
+                        if (!(ok = warp_wait(empty_bar(stage), phase ^ 1u, abort_flag, p.status, LN_STATUS_PRODUCER_TIMEOUT))) break;
+                        if (leader) {
                             const uint32_t at = smem_base + (uint32_t)stage * p.stage_bytes, bar = full_bar(stage);
                             mbar_arrive_expect_tx(bar, bytes);
                             tma_load_4d(at, &p.tmA[map], c0, t.ow0 + tx, t.oh0 + ty, t.n0, bar);
-                            tma_load_2d(at + p.off_b, &p.tmB, wcol + c0, t.f0, bar);
-#pragma unroll
-                            for (int b = 0; b < WBLOCKS; ++b) bulk_load(at + p.off_sfb + b * sf_bytes, wsf + ((size_t)b * kblocks + kb) * sf_bytes, sf_bytes, bar);
-                            if (p.flat) bulk_load(at + p.off_sfa, xsf + (size_t)kb * sf_bytes, sf_bytes, bar);
-                            if (++stage == p.stages) { stage = 0; phase ^= 1u; }
+                            if (p.flat) bulk_load(at + p.off_sfa, xsf, sf_bytes, bar);
                         }
+                        __syncwarp();
+                        if (++stage == p.stages) { stage = 0; phase ^= 1u; }
                     }
+                }
+        }
+    } else if (warp == 6) {
+        // ------------------------------------------------------------------ loads of the weights
+        const bool leader = elect_one();
+        const uint32_t sf_bytes = (uint32_t)p.words * 512u, bytes = (uint32_t)p.bn * p.bk + WBLOCKS * sf_bytes;
+        int stage = 0;
+        uint32_t phase = 0;
+        bool ok = true;
+        for (int unit = (int)blockIdx.x; ok && unit < p.num_tiles; unit += step) {
+            const int f0 = (unit - fast_div(unit, p.magic_f) * p.tiles_f) * p.bn;
+            const uint8_t* wsf = p.wsf + (size_t)(f0 >> 7) * kblocks * sf_bytes;
+            int col = 0, c0 = 0;  // first byte of the tap, of the k-block inside it
+            for (int kb = 0; kb < kblocks; ++kb, wsf += sf_bytes) {
+                if (!(ok = warp_wait(empty_bar(stage), phase ^ 1u, abort_flag, p.status, LN_STATUS_PRODUCER_TIMEOUT))) break;
+                if (leader) {
+                    const uint32_t at = smem_base + (uint32_t)stage * p.stage_bytes, bar = full_bar(stage);
+                    mbar_arrive_expect_tx(bar, bytes);
+                    tma_load_2d(at + p.off_b, &p.tmB, col + c0, f0, bar);
+#pragma unroll
+                    for (int b = 0; b < WBLOCKS; ++b) bulk_load(at + p.off_sfb + b * sf_bytes, wsf + (size_t)b * kblocks * sf_bytes, sf_bytes, bar);
+                }
+                __syncwarp();
+                c0 += p.bk;
+                if (c0 >= p.cstride) { c0 = 0; col += p.cstride; }
+                if (++stage == p.stages) { stage = 0; phase ^= 1u; }
             }
         }
-        __syncwarp();
     } else if (warp == 1) {
         // ------------------------------------------------------------------ instructions (the whole warp walks the loop; one lane issues)
         const bool leader = elect_one();
@@ -328,97 +350,99 @@ __global__ void __launch_bounds__(kThreadsF4, 1) f4_umma_kernel(const __grid_con
         }
     } else if (warp >= kFirstEpilogueWarp) {
         // ------------------------------------------------------------------ epilogue
-        // Group g takes the units with number % 2 == g.  (nbuf * subs >= 2: a group that waits for a tile's accumulator has finished a unit
+        // Group g takes the units with number % 4 == g.  (nbuf * subs >= 4: a group that waits for a tile's accumulator has finished a unit
         // of the tile nbuf before it or a later one, so the parity is unambiguous.)
         const int quad = warp & 3, group = (warp - kFirstEpilogueWarp) >> 2;
         const int row = quad * 32 + lane, pw = row & (p.TW - 1), ph = (row >> p.log_tw) & (p.TH - 1), pn = row >> (p.log_tw + p.log_th);
-        const uint32_t tab = tab_base + (uint32_t)(warp - kFirstEpilogueWarp) * 512u;
-        int t = 0, turn = 0;
+        const uint32_t tab = tab_base + (uint32_t)(warp - kFirstEpilogueWarp) * 256u;
+        // {multiplier, bias} of the unit's column that this lane looks after: read one unit ahead
+        auto table_of = [&](int f, float& m, float& b) {
+            m = f < p.F ? __ldg(p.wscale + f) : 0.0f;
+            b = f < p.F ? __ldg(p.bias + f) : 0.0f;
+        };
+        int t = 0, unit = (int)blockIdx.x, order = group;
+        while (order >= p.subs) { order -= p.subs; unit += step; ++t; }
+        auto filter_of = [&]() {
+            const int sub = overlap && t % p.nbuf == 0 ? order ^ 4 : order;  // (what overlaps the other accumulator first)
+            return (unit - fast_div(unit, p.magic_f) * p.tiles_f) * p.bn + sub * CH;
+        };
+        float mult = 0.0f, bias = 0.0f;
+        if (unit < p.num_tiles) table_of(filter_of() + lane, mult, bias);
         bool ok = true;
-        for (int unit = (int)blockIdx.x; ok && unit < p.num_tiles; unit += step, ++t)
-            for (int order = 0; ok && order < p.subs; ++order, turn ^= 1) {
-                if (turn != group) continue;
-                const f4_tile at = tile_at(p, unit);
-                const int buf = t % p.nbuf, sub = overlap && buf == 0 ? order ^ 2 : order;  // (what overlaps the other accumulator first)
-                const int ow = at.ow0 + pw, oh = at.oh0 + ph, n = at.n0 + pn, f0 = at.f0 + sub * CH;
-                const bool valid = ow < p.OW && oh < p.OH && n < p.N;
-                const long long pix = ((long long)n * p.OH + oh) * p.OW + ow;
-                __syncwarp();  // (the table of the unit before has been read)
+        while (unit < p.num_tiles) {
+            const f4_tile at = tile_at(p, unit);
+            const int buf = t % p.nbuf, f0 = filter_of(), sub = (f0 - at.f0) / CH, this_t = t;
+            const bool first = order < 4;
+            const int ow = at.ow0 + pw, oh = at.oh0 + ph, n = at.n0 + pn;
+            const bool valid = ow < p.OW && oh < p.OH && n < p.N;
+            const long long pix = ((long long)n * p.OH + oh) * p.OW + ow;
+            __syncwarp();  // (the table of the unit before has been read)
+            asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(tab + 8u * lane), "f"(__fmul_rn(p.xscale, mult)), "f"(bias) : "memory");
+            __syncwarp();
+            order += 4;
+            while (order >= p.subs) { order -= p.subs; unit += step; ++t; }
+            if (unit < p.num_tiles) table_of(filter_of() + lane, mult, bias);
+            if (!(ok = warp_wait(tfull_bar(buf), (uint32_t)((this_t / p.nbuf) & 1), abort_flag, p.status, LN_STATUS_EPILOGUE_TIMEOUT))) break;
+            tc_fence_after();
+            const uint32_t taddr = tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(buf * p.acc_step + sub * CH);
+            uint32_t acc[32];
+            tmem_ld_32x32(taddr, acc);
+            tmem_ld_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(tempty_bar(buf));
+                if (overlap && first) mbar_arrive(early_bar(buf));
+            }
+            // (binary16 channels are padded to 32, 4-bit ones to 64: what is behind them is not stored)
+            if (f0 >= (OUT == LN_OUT_Q ? (p.F + 63) & ~63 : p.F)) continue;
+            float v[32];
 #pragma unroll
-                for (int i = lane; i < CH; i += 32) {
-                    const int f = f0 + i;
-                    const float m = f < p.F ? __fmul_rn(p.xscale, __ldg(p.wscale + f)) : 0.0f, b = f < p.F ? __ldg(p.bias + f) : 0.0f;
-                    asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(tab + 8u * i), "f"(m), "f"(b) : "memory");
+            for (int i = 0; i < 32; i += 2) {
+                float4 e;  // (volatile: the table is another one for every unit)
+                asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(e.x), "=f"(e.y), "=f"(e.z), "=f"(e.w) : "r"(tab + 8u * i) : "memory");
+                v[i] = __fmaf_rn(__uint_as_float(acc[i]), e.x, e.y);
+                v[i + 1] = __fmaf_rn(__uint_as_float(acc[i + 1]), e.z, e.w);
+            }
+            act_all(p.act, p.exact != 0, v);
+            if (f0 + 32 > p.F) {
+#pragma unroll
+                for (int i = 0; i < 32; ++i)
+                    if (f0 + i >= p.F) v[i] = 0.0f;
+            }
+            if (OUT == LN_OUT_F32) {
+                if (valid) {
+                    const long long img = pix / p.hw;
+                    float* dst = (float*)p.y + (img * p.F + f0) * p.hw + (pix - img * p.hw);
+#pragma unroll
+                    for (int i = 0; i < 32; ++i)
+                        if (f0 + i < p.F) dst[(long long)i * p.hw] = v[i];
                 }
-                __syncwarp();
-                if (!(ok = warp_wait(tfull_bar(buf), (uint32_t)((t / p.nbuf) & 1), abort_flag, p.status, LN_STATUS_EPILOGUE_TIMEOUT))) break;
-                tc_fence_after();
-                const uint32_t taddr = tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(buf * p.acc_step + sub * CH);
-                uint32_t acc[CH / 32][32];
+            } else if (OUT == LN_OUT_F16) {
+                uint32_t h[2][8];
 #pragma unroll
-                for (int c = 0; c < CH / 32; ++c) tmem_ld_32x32(taddr + 32u * c, acc[c]);
-                tmem_ld_wait();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) {
-                    mbar_arrive(tempty_bar(buf));
-                    if (overlap && order < 2) mbar_arrive(early_bar(buf));
+                for (int i = 0; i < 16; ++i) {
+                    const __half2 q = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+                    h[i >> 3][i & 7] = *reinterpret_cast<const uint32_t*>(&q);
                 }
-                if (f0 >= p.F) continue;  // nothing but padding
-                uint32_t sf = 0;
+                if (valid) {
+                    uint8_t* dst = (uint8_t*)p.y + pix * p.ys + 2 * f0;
+                    store_32(dst, h[0]);
+                    store_32(dst + 32, h[1]);
+                }
+            } else {
+                constexpr int B = FMT == LN_F4 ? 16 : 32;
+                uint32_t q[4], sf = 0;
 #pragma unroll
-                for (int c0 = 0; c0 < CH; c0 += 32) {
-                    if (f0 + c0 >= p.F && OUT != LN_OUT_Q) break;  // (binary16 channels are padded to 32, 4-bit ones to 64)
-                    float v[32];
-#pragma unroll
-                    for (int i = 0; i < 32; i += 2) {
-                        float4 e;  // (volatile: the table is another one for every unit)
-                        asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(e.x), "=f"(e.y), "=f"(e.z), "=f"(e.w) : "r"(tab + 8u * (c0 + i)) : "memory");
-                        v[i] = __fmaf_rn(__uint_as_float(acc[c0 / 32][i]), e.x, e.y);
-                        v[i + 1] = __fmaf_rn(__uint_as_float(acc[c0 / 32][i + 1]), e.z, e.w);
-                    }
-                    act_all(p.act, p.exact != 0, v);
-                    if (f0 + c0 + 32 > p.F) {
-#pragma unroll
-                        for (int i = 0; i < 32; ++i)
-                            if (f0 + c0 + i >= p.F) v[i] = 0.0f;
-                    }
-                    if (OUT == LN_OUT_F32) {
-                        if (valid) {
-                            const long long img = pix / p.hw;
-                            float* dst = (float*)p.y + (img * p.F + f0 + c0) * p.hw + (pix - img * p.hw);
-#pragma unroll
-                            for (int i = 0; i < 32; ++i)
-                                if (f0 + c0 + i < p.F) dst[(long long)i * p.hw] = v[i];
-                        }
-                    } else if (OUT == LN_OUT_F16) {
-                        uint32_t h[2][8];
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            const __half2 q = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
-                            h[i >> 3][i & 7] = *reinterpret_cast<const uint32_t*>(&q);
-                        }
-                        if (valid) {
-                            uint8_t* dst = (uint8_t*)p.y + pix * p.ys + 2 * (f0 + c0);
-                            store_32(dst, h[0]);
-                            store_32(dst + 32, h[1]);
-                        }
-                    } else {
-                        constexpr int B = FMT == LN_F4 ? 16 : 32;
-                        uint32_t q[4];
-#pragma unroll
-                        for (int b = 0; b < 32 / B; ++b) sf |= ln_f4_quantise<FMT>(v + b * B, p.g, p.six_g, q + b * B / 8) << (8 * (c0 / B + b));
-                        if (valid) {
-                            *(uint4*)((uint8_t*)p.y + pix * p.ys + (f0 + c0) / 2) = make_uint4(q[0], q[1], q[2], q[3]);
-                            uint8_t* at_sf = p.ysf + ln_f4_sf_at(pix, f0 / (4 * B), p.ysf_words);
-                            if (c0 + 32 == CH) {
-                                if (FMT == LN_F4) *(uint32_t*)at_sf = sf;
-                                else *(uint16_t*)(at_sf + f0 / B % 4) = (uint16_t)sf;
-                            }
-                        }
-                    }
+                for (int b = 0; b < 32 / B; ++b) sf |= ln_f4_quantise<FMT>(v + b * B, p.g, p.six_g, q + b * B / 8) << (8 * b);
+                if (valid) {
+                    *(uint4*)((uint8_t*)p.y + pix * p.ys + f0 / 2) = make_uint4(q[0], q[1], q[2], q[3]);
+                    uint8_t* at_sf = p.ysf + ln_f4_sf_at(pix, f0 / (4 * B), p.ysf_words) + f0 / B % 4;
+                    if (FMT == LN_F4) *(uint16_t*)at_sf = (uint16_t)sf;
+                    else *at_sf = (uint8_t)sf;
                 }
             }
+        }
     }
 
     tc_fence_before();
