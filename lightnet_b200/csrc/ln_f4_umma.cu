@@ -15,6 +15,11 @@
 // of four that take the units of 32 columns of the tiles in turn.  TMEM: 416 columns of accumulators, 2 x 48 of scales.  Two tiles of
 // 192 filters, three of 128 or six of 64 fit; two of 256 overlap by 96 columns (0..255 and 160..415), so their epilogue reads the four
 // units that hold the overlap first and the next tile starts as soon as those are in registers.
+//
+// CTA pairs (PAIR: clusters of two CTAs on neighbouring SMs, cta_group::2): both multiply their own 128 pixels by the same filters, each
+// loads half of the filters' codes, and one instruction of the first CTA's issuing thread works in both (M = 256).  What bounds a large
+// product is the way from L2 to shared memory, about 60 bytes a cycle and SM: a k-block of 256 filters is 54 KB for 528 cycles of
+// tensor work alone and 38 KB in a pair.  The loads of both CTAs signal the first one's barriers, commits arrive in both.
 // Every wait is bounded (see ln_umma.h).
 #include <cstdlib>
 
@@ -33,8 +38,8 @@ constexpr uint32_t kTabBytesF4 = 16 * 256;  // {multiplier, bias} of the columns
 constexpr int kMaxSmemF4 = 227 * 1024;
 
 struct f4_params {
-    CUtensorMap tmA[4], tmB;
-    const uint8_t *xsf, *wsf;
+    CUtensorMap tmA[4], tmB, tmXS, tmWS;  // codes of pixels and filters; their scales as rows of 512 bytes
+    const uint8_t* xsf;
     const float *wscale, *bias;
     void* y;
     uint8_t* ysf;
@@ -44,7 +49,7 @@ struct f4_params {
     int sf_words, cstride;
     int bk, bn, cblocks, words;
     int R, S, stride, pad, H, W, N, OH, OW, F, hw;
-    int TW, TH, TN, log_tw, log_th, tiles_f, tiles_w, tiles_h, num_tiles;
+    int TW, TH, TN, log_tw, log_th, tiles_f, tiles_w, tiles_h, num_units;  // units: pixel tiles (pairs of them) x filter tiles
     unsigned long long magic_f, magic_w, magic_h;
     int stages, nbuf, acc_step, subs, act, exact, flat;
     uint32_t off_b, off_sfa, off_sfb, stage_bytes;
@@ -59,67 +64,172 @@ __device__ __forceinline__ bool elect_one() {
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status, int code) {
     return __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity, abort_flag, status, code));
 }
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+// The CTAs of a pair: rank, the first CTA's copy of a shared address, arrival on its barriers, rendezvous.
+__device__ __forceinline__ uint32_t pair_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
 }
-// 32 rows of 16 bytes -> the four 32-lane quarters of TMEM, four columns
+__device__ __forceinline__ uint32_t in_first(uint32_t addr) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(addr));
+    return r;
+}
+template <bool RELEASE>
+__device__ __forceinline__ void arrive_first(uint32_t bar) {
+    // (the epilogue hands tensor memory back, which its fence orders; a release would wait for its global stores)
+    if (RELEASE) asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(in_first(bar)) : "memory");
+    else asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(in_first(bar)) : "memory");
+}
+__device__ __forceinline__ void pair_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// The issuing thread's wait for gathered scales: in a pair also for those that the other CTA stored before it arrived.
+__device__ __forceinline__ bool mbar_wait_pair(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status) {
+    for (uint32_t it = 0; it < kWaitLimit; ++it) {
+        uint32_t there;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(there)
+            : "r"(bar), "r"(parity), "r"(kWaitHintNs)
+            : "memory");
+        if (there) return true;
+        if ((it & 255u) == 255u && *abort_flag) return false;
+    }
+    *abort_flag = 1;
+    *(volatile int*)status = LN_STATUS_MMA_TIMEOUT;
+    __threadfence_system();
+    return false;
+}
+// Loads; in a pair they signal the first CTA's barrier (`bar` is its address there).
+template <bool PAIR>
+__device__ __forceinline__ void load_4d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, int c3, uint32_t bar) {
+    if (!PAIR) { tma_load_4d(dst, map, c0, c1, c2, c3, bar); return; }
+    asm volatile("cp.async.bulk.tensor.4d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(c2),
+                 "r"(c3)
+                 : "memory");
+}
+template <bool PAIR>
+__device__ __forceinline__ void load_3d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, uint32_t bar) {
+    if (PAIR) asm volatile("cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(c2) : "memory");
+    else asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(c2) : "memory");
+}
+template <bool PAIR>
+__device__ __forceinline__ void load_2d(uint32_t dst, const CUtensorMap* map, int c0, int c1, uint32_t bar) {
+    if (!PAIR) { tma_load_2d(dst, map, c0, c1, bar); return; }
+    asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(c1) : "memory");
+}
+// arrives, in both CTAs of a pair, once everything issued so far has finished
+template <bool PAIR>
+__device__ __forceinline__ void commit(uint32_t bar) {
+    if (PAIR) asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((uint16_t)3) : "memory");
+    else tc_commit(bar);
+}
+// 32 rows of 16 bytes -> the four 32-lane quarters of TMEM, four columns (each CTA of a pair from its own shared memory)
+template <bool PAIR>
 __device__ __forceinline__ void tc_copy_scales(uint32_t taddr, uint64_t desc) {
-    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+    if (PAIR) asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+    else asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
 }
-template <int FMT>
+template <int FMT, bool PAIR>
 __device__ __forceinline__ void tc_mma_scaled(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
-    if (FMT == LN_F4)
-        asm volatile(
-            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-            "tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, [%5], [%6], p;\n\t}" ::"r"(d),
-            "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(sfa), "r"(sfb)
-            : "memory");
-    else
-        asm volatile(
-            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-            "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%5], [%6], p;\n\t}" ::"r"(d),
-            "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(sfa), "r"(sfb)
-            : "memory");
+#define LN_MMA(GROUP, KIND)                                                                                                  \
+    asm volatile(                                                                                                            \
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"                                                                    \
+        "tcgen05.mma.cta_group::" GROUP ".kind::" KIND " [%0], %1, %2, %3, [%5], [%6], p;\n\t}" ::"r"(d),                    \
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(sfa), "r"(sfb)                                                      \
+        : "memory")
+    if (FMT == LN_F4) {
+        if (PAIR) LN_MMA("2", "mxf4nvf4.block_scale.scale_vec::4X");
+        else LN_MMA("1", "mxf4nvf4.block_scale.scale_vec::4X");
+    } else {
+        if (PAIR) LN_MMA("2", "mxf4.block_scale.scale_vec::2X");
+        else LN_MMA("1", "mxf4.block_scale.scale_vec::2X");
+    }
+#undef LN_MMA
 }
 // descriptor of 32 rows of 16 bytes (no swizzle, groups of 8 rows 128 bytes apart)
 __device__ __forceinline__ uint64_t scale_desc(uint32_t addr) { return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)(128u >> 4) << 32) | (1ull << 46); }
 
+// Fast activations, two values at a time.  exp is ex2.approx, the reciprocal a seed from the exponent's bits (12 % off) and three Newton
+// steps on the FMA pipe (2e-4, then a rounding or two): with rcp.approx as well the special function unit, at a quarter of the lanes'
+// rate, bounded the epilogue of the products with short k ranges.
+__device__ __forceinline__ void reciprocal2(float& r0, float& r1, float d0, float d1) {
+    r0 = __uint_as_float(0x7EF311C7u - __float_as_uint(d0));
+    r1 = __uint_as_float(0x7EF311C7u - __float_as_uint(d1));
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+        float e0, e1;
+        ffma2(e0, e1, -d0, -d1, r0, r1, 1.0f, 1.0f);
+        ffma2(r0, r1, r0, r1, e0, e1, r0, r1);
+    }
+}
+template <int ACT>
+__device__ __forceinline__ void act2(float& v0, float& v1) {
+    if (ACT == LN_ACT_MISH) {  // v w / (w + 2), w = e^v (e^v + 2), the ratio evaluated at min(v, 20) (it is 1 from there on)
+        float e0, e1, w0, w1, d0, d1, r0, r1;
+        fmul2(e0, e1, fminf(v0, 20.0f), fminf(v1, 20.0f), 1.44269504f, 1.44269504f);
+        e0 = ln_ex2_ftz(e0);
+        e1 = ln_ex2_ftz(e1);
+        fadd2(w0, w1, e0, e1, 2.0f, 2.0f);
+        fmul2(w0, w1, w0, w1, e0, e1);
+        fadd2(d0, d1, w0, w1, 2.0f, 2.0f);
+        reciprocal2(r0, r1, d0, d1);
+        fmul2(w0, w1, w0, w1, r0, r1);
+        fmul2(v0, v1, v0, v1, w0, w1);
+    } else {  // swish, logistic: 1 / (1 + e^-v) at max(v, -60)
+        float e0, e1, r0, r1;
+        fmul2(e0, e1, fmaxf(v0, -60.0f), fmaxf(v1, -60.0f), -1.44269504f, -1.44269504f);
+        fadd2(e0, e1, ln_ex2_ftz(e0), ln_ex2_ftz(e1), 1.0f, 1.0f);
+        reciprocal2(r0, r1, e0, e1);
+        if (ACT == LN_ACT_SWISH) fmul2(v0, v1, v0, v1, r0, r1);
+        else { v0 = v0 == v0 ? r0 : v0; v1 = v1 == v1 ? r1 : v1; }  // (max drops a NaN)
+    }
+}
 __device__ __forceinline__ void act_all(int act, bool exact, float (&v)[32]) {
-#define LN_ALL(E, A)                                                       \
-    _Pragma("unroll") for (int i = 0; i < 32; ++i) v[i] = ln_epilogue_act<E>(A, v[i]); \
+#define LN_ALL(A)                                                                          \
+    _Pragma("unroll") for (int i = 0; i < 32; ++i) v[i] = ln_epilogue_act<true>(A, v[i]);  \
+    break;
+#define LN_FAST(A)                                                                         \
+    _Pragma("unroll") for (int i = 0; i < 32; i += 2) act2<A>(v[i], v[i + 1]);             \
     break;
     switch (act) {
-        case LN_ACT_LEAKY: LN_ALL(true, LN_ACT_LEAKY)
-        case LN_ACT_RELU: LN_ALL(true, LN_ACT_RELU)
+        case LN_ACT_LEAKY: LN_ALL(LN_ACT_LEAKY)
+        case LN_ACT_RELU: LN_ALL(LN_ACT_RELU)
         case LN_ACT_MISH:
-            if (exact) { LN_ALL(true, LN_ACT_MISH) }
-            LN_ALL(false, LN_ACT_MISH)
+            if (exact) { LN_ALL(LN_ACT_MISH) }
+            LN_FAST(LN_ACT_MISH)
         case LN_ACT_SWISH:
-            if (exact) { LN_ALL(true, LN_ACT_SWISH) }
-            LN_ALL(false, LN_ACT_SWISH)
+            if (exact) { LN_ALL(LN_ACT_SWISH) }
+            LN_FAST(LN_ACT_SWISH)
         case LN_ACT_LOGISTIC:
-            if (exact) { LN_ALL(true, LN_ACT_LOGISTIC) }
-            LN_ALL(false, LN_ACT_LOGISTIC)
+            if (exact) { LN_ALL(LN_ACT_LOGISTIC) }
+            LN_FAST(LN_ACT_LOGISTIC)
         default: break;
     }
 #undef LN_ALL
+#undef LN_FAST
 }
-
 __device__ __forceinline__ void store_32(uint8_t* dst, const uint32_t (&v)[8]) {  // a whole sector
     asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
 }
-// the tile's place: output box origin and first filter
+// the place of work unit `unit`: output box origin and first filter.  The CTAs of a pair take two consecutive pixel tiles (the second may
+// lie behind the last: everything there is out of range).
 struct f4_tile {
     int ow0, oh0, n0, f0;
 };
-__device__ __forceinline__ f4_tile tile_at(const f4_params& p, int unit) {
-    const int q1 = fast_div(unit, p.magic_f), tf = unit - q1 * p.tiles_f;
+template <bool PAIR>
+__device__ __forceinline__ f4_tile tile_at(const f4_params& p, int unit, int rank) {
+    const int u1 = fast_div(unit, p.magic_f), tf = unit - u1 * p.tiles_f, q1 = PAIR ? 2 * u1 + rank : u1;
     const int q2 = fast_div(q1, p.magic_w), tw = q1 - q2 * p.tiles_w;
     const int tn = fast_div(q2, p.magic_h), th = q2 - tn * p.tiles_h;
     return {tw * p.TW, th * p.TH, tn * p.TN, tf * p.bn};
 }
 
-template <int FMT, int OUT, int WBLOCKS>
+template <int FMT, int OUT, int WBLOCKS, bool PAIR>
 __global__ void __launch_bounds__(kThreadsF4, 1) f4_umma_kernel(const __grid_constant__ f4_params p) {
     extern __shared__ uint8_t smem_raw[];
     const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -133,164 +243,166 @@ __global__ void __launch_bounds__(kThreadsF4, 1) f4_umma_kernel(const __grid_con
     volatile int* abort_flag = (volatile int*)(tmem_slot + 2);
     const uint32_t tab_base = bar_base + kBarBytesF4;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = PAIR ? (int)pair_rank() : 0;
+    constexpr int kCtas = PAIR ? 2 : 1;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < p.stages; ++s) {
-            mbar_init(full_bar(s), p.flat ? 2 : 3);  // the two loaders (with their copies' bytes) and a warp that gathers scales
+            mbar_init(full_bar(s), p.flat ? 2 : 2 + kCtas);  // the two loaders (with the copies' bytes) and the warps that gather scales
             mbar_init(empty_bar(s), 1);
         }
         for (int b = 0; b < p.nbuf; ++b) {
             mbar_init(tfull_bar(b), 1);
-            mbar_init(tempty_bar(b), 4 * p.subs);
+            mbar_init(tempty_bar(b), 4 * p.subs * kCtas);
         }
-        mbar_init(early_bar(0), 16);
-        mbar_init(early_bar(1), 16);
+        mbar_init(early_bar(0), 16 * kCtas);
+        mbar_init(early_bar(1), 16 * kCtas);
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32((const void*)tmem_slot)), "r"(512u) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        if (PAIR) {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32((const void*)tmem_slot)), "r"(512u) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32((const void*)tmem_slot)), "r"(512u) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        }
     }
     tc_fence_before();
     __syncthreads();
+    if (PAIR) pair_sync();  // the other CTA's barriers are there before anything signals them
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
-    const int kblocks = p.R * p.S * p.cblocks, step = (int)gridDim.x;
+    const int kblocks = p.R * p.S * p.cblocks, first_unit = (int)blockIdx.x / kCtas, step = (int)gridDim.x / kCtas;
     const bool overlap = p.bn == 256;
 
     if (warp == 0) {
-        // ------------------------------------------------------------------ loads of the pixels (whole warps walk these loops; one lane issues)
-        const bool leader = elect_one();
-        const uint32_t sf_bytes = (uint32_t)p.words * 512u, bytes = 128u * p.bk + (p.flat ? sf_bytes : 0u);
-        int stage = 0;
-        uint32_t phase = 0;
-        bool ok = true;
-        for (int unit = (int)blockIdx.x; ok && unit < p.num_tiles; unit += step) {
-            const f4_tile t = tile_at(p, unit);
-            const uint8_t* xsf = p.xsf + (size_t)(t.ow0 >> 7) * kblocks * sf_bytes;  // (flat)
-            for (int r = 0; ok && r < p.R; ++r)
-                for (int s = 0; ok && s < p.S; ++s) {
-                    int ty = r - p.pad, tx = s - p.pad, map = 0;
-                    if (p.stride == 2) {
-                        const int py = ty & 1, px = tx & 1;  // parity class of the tap
-                        ty = (ty - py) >> 1;
-                        tx = (tx - px) >> 1;
-                        map = py * 2 + px;
-                    }
-                    for (int c0 = 0; c0 < p.cstride; c0 += p.bk, xsf += sf_bytes) {
-                        if (!(ok = warp_wait(empty_bar(stage), phase ^ 1u, abort_flag, p.status, LN_STATUS_PRODUCER_TIMEOUT))) break;
-                        if (leader) {
-                            const uint32_t at = smem_base + (uint32_t)stage * p.stage_bytes, bar = full_bar(stage);
-                            mbar_arrive_expect_tx(bar, bytes);
-                            tma_load_4d(at, &p.tmA[map], c0, t.ow0 + tx, t.oh0 + ty, t.n0, bar);
-                            if (p.flat) bulk_load(at + p.off_sfa, xsf, sf_bytes, bar);
+        // ------------------------------------------------------------------ loads of the pixels
+        if (elect_one()) {
+            const uint32_t bytes = 128u * p.bk + (p.flat ? (uint32_t)p.words * 512u : 0u);
+            const uint32_t first_full = PAIR ? in_first(full_bar(0)) : full_bar(0);
+            int stage = 0;
+            uint32_t phase = 0;
+            bool ok = true;
+            for (int unit = first_unit; ok && unit < p.num_units; unit += step) {
+                const f4_tile t = tile_at<PAIR>(p, unit, rank);
+                int sf_row = (t.ow0 >> 7) * kblocks * p.words;  // (flat)
+                for (int r = 0; ok && r < p.R; ++r)
+                    for (int s = 0; ok && s < p.S; ++s) {
+                        int ty = r - p.pad, tx = s - p.pad, map = 0;
+                        if (p.stride == 2) {
+                            const int py = ty & 1, px = tx & 1;  // parity class of the tap
+                            ty = (ty - py) >> 1;
+                            tx = (tx - px) >> 1;
+                            map = py * 2 + px;
                         }
-                        __syncwarp();
-                        if (++stage == p.stages) { stage = 0; phase ^= 1u; }
+                        for (int c0 = 0; c0 < p.cstride; c0 += p.bk, sf_row += p.words) {
+                            if (!(ok = mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag, p.status, LN_STATUS_PRODUCER_TIMEOUT))) break;
+                            const uint32_t at = smem_base + (uint32_t)stage * p.stage_bytes, bar = first_full + 8u * stage;
+                            if (rank == 0) mbar_arrive_expect_tx(full_bar(stage), kCtas * bytes);
+                            load_4d<PAIR>(at, &p.tmA[map], c0, t.ow0 + tx, t.oh0 + ty, t.n0, bar);
+                            if (p.flat) load_2d<PAIR>(at + p.off_sfa, &p.tmXS, 0, sf_row, bar);
+                            if (++stage == p.stages) { stage = 0; phase ^= 1u; }
+                        }
                     }
-                }
-        }
-    } else if (warp == 6) {
-        // ------------------------------------------------------------------ loads of the weights
-        const bool leader = elect_one();
-        const uint32_t sf_bytes = (uint32_t)p.words * 512u, bytes = (uint32_t)p.bn * p.bk + WBLOCKS * sf_bytes;
-        int stage = 0;
-        uint32_t phase = 0;
-        bool ok = true;
-        for (int unit = (int)blockIdx.x; ok && unit < p.num_tiles; unit += step) {
-            const int f0 = (unit - fast_div(unit, p.magic_f) * p.tiles_f) * p.bn;
-            const uint8_t* wsf = p.wsf + (size_t)(f0 >> 7) * kblocks * sf_bytes;
-            int col = 0, c0 = 0;  // first byte of the tap, of the k-block inside it
-            for (int kb = 0; kb < kblocks; ++kb, wsf += sf_bytes) {
-                if (!(ok = warp_wait(empty_bar(stage), phase ^ 1u, abort_flag, p.status, LN_STATUS_PRODUCER_TIMEOUT))) break;
-                if (leader) {
-                    const uint32_t at = smem_base + (uint32_t)stage * p.stage_bytes, bar = full_bar(stage);
-                    mbar_arrive_expect_tx(bar, bytes);
-                    tma_load_2d(at + p.off_b, &p.tmB, col + c0, f0, bar);
-#pragma unroll
-                    for (int b = 0; b < WBLOCKS; ++b) bulk_load(at + p.off_sfb + b * sf_bytes, wsf + (size_t)b * kblocks * sf_bytes, sf_bytes, bar);
-                }
-                __syncwarp();
-                c0 += p.bk;
-                if (c0 >= p.cstride) { c0 = 0; col += p.cstride; }
-                if (++stage == p.stages) { stage = 0; phase ^= 1u; }
             }
         }
+        __syncwarp();
+    } else if (warp == 6) {
+        // ------------------------------------------------------------------ loads of the weights (a CTA of a pair: of its half of the codes, and all scales)
+        if (elect_one()) {
+            const int rows = p.bn / kCtas;
+            const uint32_t bytes = (uint32_t)rows * p.bk + WBLOCKS * (uint32_t)p.words * 512u;
+            const uint32_t first_full = PAIR ? in_first(full_bar(0)) : full_bar(0);
+            int stage = 0;
+            uint32_t phase = 0;
+            bool ok = true;
+            for (int unit = first_unit; ok && unit < p.num_units; unit += step) {
+                const int f0 = (unit - fast_div(unit, p.magic_f) * p.tiles_f) * p.bn;
+                int col = 0, c0 = 0;  // first byte of the tap, of the k-block inside it
+                for (int kb = 0; kb < kblocks; ++kb) {
+                    if (!(ok = mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag, p.status, LN_STATUS_PRODUCER_TIMEOUT))) break;
+                    const uint32_t at = smem_base + (uint32_t)stage * p.stage_bytes, bar = first_full + 8u * stage;
+                    if (rank == 0) mbar_arrive_expect_tx(full_bar(stage), kCtas * bytes);
+                    load_2d<PAIR>(at + p.off_b, &p.tmB, col + c0, f0 + rank * rows, bar);
+                    load_3d<PAIR>(at + p.off_sfb, &p.tmWS, 0, kb * p.words, f0 >> 7, bar);
+                    c0 += p.bk;
+                    if (c0 >= p.cstride) { c0 = 0; col += p.cstride; }
+                    if (++stage == p.stages) { stage = 0; phase ^= 1u; }
+                }
+            }
+        }
+        __syncwarp();
     } else if (warp == 1) {
-        // ------------------------------------------------------------------ instructions (the whole warp walks the loop; one lane issues)
-        const bool leader = elect_one();
-        // E2M1 operands (bits 7, 10: type 1), N / 8, scale type (bit 23: 1 = E8M0), M / 128, K-major; the scale ids go to bits 4 and 29
-        const uint32_t idesc = (1u << 7) | (1u << 10) | ((uint32_t)(p.bn >> 3) << 17) | ((FMT == LN_MX4 ? 1u : 0u) << 23) | (1u << 27);
-        const uint64_t desc_base = make_smem_desc(0u, p.bk);
-        constexpr int kWords = FMT == LN_MX4 ? 2 : 4, kBlocks = WBLOCKS;  // of a whole k-block
-        const uint64_t sfa_desc = scale_desc(p.off_sfa), sfb_desc = scale_desc(p.off_sfb);
-        int stage = 0, t = 0;
-        uint32_t phase = 0, set = 0;
-        bool ok = true;
-        for (int unit = (int)blockIdx.x; ok && unit < p.num_tiles; unit += step, ++t) {
-            const int buf = t % p.nbuf;
-            if (!(ok = warp_wait(tempty_bar(buf), (uint32_t)((t / p.nbuf) & 1) ^ 1u, abort_flag, p.status, LN_STATUS_MMA_TIMEOUT))) break;
-            if (overlap && t > 0 && !(ok = warp_wait(early_bar(buf ^ 1), (uint32_t)(((t - 1) >> 1) & 1), abort_flag, p.status, LN_STATUS_MMA_TIMEOUT))) break;
-            tc_fence_after();
-            const uint32_t d = tmem_base + (uint32_t)(buf * p.acc_step);
-            const int tf = unit - fast_div(unit, p.magic_f) * p.tiles_f;
-            const uint32_t shift = (uint32_t)((tf * p.bn & 127) >> 5);  // first column of the tile's filters inside their group of 128
-            int c0 = 0;
-            for (int kb = 0; kb < kblocks; ++kb) {
-                if (!(ok = warp_wait(full_bar(stage), phase, abort_flag, p.status, LN_STATUS_MMA_TIMEOUT))) break;
+        // ------------------------------------------------------------------ instructions
+        if (rank == 0 && elect_one()) {
+            // E2M1 operands (bits 7, 10: type 1), N / 8, scale type (bit 23: 1 = E8M0), M / 128, K-major; the scale ids go to bits 4 and 29
+            const uint32_t idesc = (1u << 7) | (1u << 10) | ((uint32_t)(p.bn >> 3) << 17) | ((FMT == LN_MX4 ? 1u : 0u) << 23) | ((uint32_t)kCtas << 27);
+            const uint64_t desc_base = make_smem_desc(0u, p.bk);
+            constexpr int kWords = FMT == LN_MX4 ? 2 : 4;  // of a whole k-block
+            const uint64_t sfa_desc = scale_desc(p.off_sfa), sfb_desc = scale_desc(p.off_sfb);
+            int stage = 0, t = 0;
+            uint32_t phase = 0, set = 0;
+            bool ok = true;
+            for (int unit = first_unit; ok && unit < p.num_units; unit += step, ++t) {
+                const int buf = t % p.nbuf;
+                if (!(ok = mbar_wait(tempty_bar(buf), (uint32_t)((t / p.nbuf) & 1) ^ 1u, abort_flag, p.status, LN_STATUS_MMA_TIMEOUT))) break;
+                if (overlap && t > 0 && !(ok = mbar_wait(early_bar(buf ^ 1), (uint32_t)(((t - 1) >> 1) & 1), abort_flag, p.status, LN_STATUS_MMA_TIMEOUT))) break;
                 tc_fence_after();
-                const uint32_t at = smem_base + (uint32_t)stage * p.stage_bytes;
-                const uint32_t sfa = tmem_base + kScaleCols + set * kScaleSet, sfb = sfa + kScaleB;
-                const int left = p.cstride - c0, n = (left < p.bk ? left : p.bk) >> 5;  // instructions of this k-block
-                const uint64_t a_desc = desc_base + (at >> 4), b_desc = desc_base + ((at + p.off_b) >> 4);
-                if (n == 4) {
-                    // a whole k-block of 128 bytes, unrolled with constant offsets: as loops with run-time bounds the copies and
-                    // instructions of a k-block took their thread 1100 cycles, this way 420, less than the 530 that they run for
-                    if (leader) {
+                const uint32_t d = tmem_base + (uint32_t)(buf * p.acc_step);
+                const int tf = unit - fast_div(unit, p.magic_f) * p.tiles_f;
+                const uint32_t shift = (uint32_t)((tf * p.bn & 127) >> 5);  // first column of the tile's filters inside their group of 128
+                int c0 = 0;
+                for (int kb = 0; kb < kblocks; ++kb) {
+                    ok = PAIR && !p.flat ? mbar_wait_pair(full_bar(stage), phase, abort_flag, p.status) : mbar_wait(full_bar(stage), phase, abort_flag, p.status, LN_STATUS_MMA_TIMEOUT);
+                    if (!ok) break;
+                    const uint32_t at = smem_base + (uint32_t)stage * p.stage_bytes;
+                    const uint32_t sfa = tmem_base + kScaleCols + set * kScaleSet, sfb = sfa + kScaleB;
+                    const int left = p.cstride - c0, n = (left < p.bk ? left : p.bk) >> 5;  // instructions of this k-block
+                    const uint64_t a_desc = desc_base + (at >> 4), b_desc = desc_base + ((at + p.off_b) >> 4);
+                    if (n == 4) {
+                        // a whole k-block of 128 bytes, unrolled with constant offsets: as loops with run-time bounds the copies and
+                        // instructions of a k-block took their thread 1100 cycles, this way 390, less than the 530 that they run for
 #pragma unroll
                         for (int j = 0; j < kWords; ++j) {
-                            tc_copy_scales(sfa + 4u * j, sfa_desc + ((at + 512u * j) >> 4));
+                            tc_copy_scales<PAIR>(sfa + 4u * j, sfa_desc + ((at + 512u * j) >> 4));
 #pragma unroll
-                            for (int b = 0; b < kBlocks; ++b) tc_copy_scales(sfb + 4u * (j * kBlocks + b), sfb_desc + ((at + 512u * (b * kWords + j)) >> 4));
+                            for (int b = 0; b < WBLOCKS; ++b) tc_copy_scales<PAIR>(sfb + 4u * (j * WBLOCKS + b), sfb_desc + ((at + 512u * (b * kWords + j)) >> 4));
                         }
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             const uint32_t word = FMT == LN_MX4 ? i >> 1 : i, id = FMT == LN_MX4 ? (uint32_t)(i & 1) * 2u : 0u;
-                            tc_mma_scaled<FMT>(d, a_desc + 2u * i, b_desc + 2u * i, idesc | (id << 4) | (id << 29), sfa + 4u * word, sfb + 4u * word * kBlocks + shift, i ? 1u : (uint32_t)(kb != 0));
+                            tc_mma_scaled<FMT, PAIR>(d, a_desc + 2u * i, b_desc + 2u * i, idesc | (id << 4) | (id << 29), sfa + 4u * word, sfb + 4u * word * WBLOCKS + shift, i ? 1u : (uint32_t)(kb != 0));
                         }
-                        tc_commit(empty_bar(stage));
-                    }
-                } else if (leader) {
-                    for (int j = 0; j < p.words; ++j) {
-                        tc_copy_scales(sfa + 4u * j, scale_desc(at + p.off_sfa + 512u * j));
-                        for (int b = 0; b < WBLOCKS; ++b) tc_copy_scales(sfb + 4u * (j * WBLOCKS + b), scale_desc(at + p.off_sfb + 512u * (b * p.words + j)));
-                    }
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (i < n) {
+                    } else {
+                        for (int j = 0; j < p.words; ++j) {
+                            tc_copy_scales<PAIR>(sfa + 4u * j, sfa_desc + ((at + 512u * j) >> 4));
+                            for (int b = 0; b < WBLOCKS; ++b) tc_copy_scales<PAIR>(sfb + 4u * (j * WBLOCKS + b), sfb_desc + ((at + 512u * (b * p.words + j)) >> 4));
+                        }
+                        for (int i = 0; i < n; ++i) {
                             const uint32_t word = FMT == LN_MX4 ? i >> 1 : i, id = FMT == LN_MX4 ? (uint32_t)(i & 1) * 2u : 0u;
-                            tc_mma_scaled<FMT>(d, a_desc + 2u * i, b_desc + 2u * i, idesc | (id << 4) | (id << 29), sfa + 4u * word, sfb + 4u * word * WBLOCKS + shift, (uint32_t)((kb | i) != 0));
+                            tc_mma_scaled<FMT, PAIR>(d, a_desc + 2u * i, b_desc + 2u * i, idesc | (id << 4) | (id << 29), sfa + 4u * word, sfb + 4u * word * WBLOCKS + shift, (uint32_t)((kb | i) != 0));
                         }
-                    tc_commit(empty_bar(stage));
+                    }
+                    commit<PAIR>(empty_bar(stage));
+                    set ^= 1u;
+                    c0 += p.bk;
+                    if (c0 >= p.cstride) c0 = 0;
+                    if (++stage == p.stages) { stage = 0; phase ^= 1u; }
                 }
-                __syncwarp();
-                set ^= 1u;
-                c0 += p.bk;
-                if (c0 >= p.cstride) c0 = 0;
-                if (++stage == p.stages) { stage = 0; phase ^= 1u; }
+                if (!ok) break;
+                commit<PAIR>(tfull_bar(buf));
             }
-            if (!ok) break;
-            if (leader) tc_commit(tfull_bar(buf));
-            __syncwarp();
         }
+        __syncwarp();
     } else if (warp < 2 + kGatherWarps) {
         // ------------------------------------------------------------------ scales of the pixels under shifted taps
-        int unit = (int)blockIdx.x, r = 0, s = 0, cb = 0;
+        int unit = first_unit, r = 0, s = 0, cb = 0;
         int iy0[4], ix0[4], img[4];
         auto enter_tile = [&]() {
-            if (unit >= p.num_tiles) return;
-            const f4_tile t = tile_at(p, unit);
+            if (unit >= p.num_units) return;
+            const f4_tile t = tile_at<PAIR>(p, unit, rank);
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
                 const int row = g * 32 + lane;
@@ -325,11 +437,11 @@ __global__ void __launch_bounds__(kThreadsF4, 1) f4_umma_kernel(const __grid_con
             int stage = warp - 2;  // (fewer than stages)
             uint32_t phase = 0;
             uint32_t now[4][4], next[4][4];
-            bool more = unit < p.num_tiles, ok = true;
+            bool more = unit < p.num_units, ok = true;
             if (more) fetch(now);
             while (more && ok) {
                 for (int i = 0; i < kGatherWarps; ++i) advance();
-                more = unit < p.num_tiles;
+                more = unit < p.num_units;
                 if (more) fetch(next);
                 if (!(ok = warp_wait(empty_bar(stage), phase ^ 1u, abort_flag, p.status, LN_STATUS_PRODUCER_TIMEOUT))) break;
                 const uint32_t dst = smem_base + (uint32_t)stage * p.stage_bytes + p.off_sfa + 16u * lane;
@@ -339,7 +451,10 @@ __global__ void __launch_bounds__(kThreadsF4, 1) f4_umma_kernel(const __grid_con
                         asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + 512u * j), "r"(now[0][j]), "r"(now[1][j]), "r"(now[2][j]), "r"(now[3][j]) : "memory");
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
-                if (lane == 0) mbar_arrive(full_bar(stage));
+                if (lane == 0) {
+                    if (PAIR) arrive_first<true>(full_bar(stage));
+                    else mbar_arrive(full_bar(stage));
+                }
                 stage += kGatherWarps;
                 if (stage >= p.stages) { stage -= p.stages; phase ^= 1u; }
 #pragma unroll
@@ -355,44 +470,61 @@ __global__ void __launch_bounds__(kThreadsF4, 1) f4_umma_kernel(const __grid_con
         const int quad = warp & 3, group = (warp - kFirstEpilogueWarp) >> 2;
         const int row = quad * 32 + lane, pw = row & (p.TW - 1), ph = (row >> p.log_tw) & (p.TH - 1), pn = row >> (p.log_tw + p.log_th);
         const uint32_t tab = tab_base + (uint32_t)(warp - kFirstEpilogueWarp) * 256u;
-        // {multiplier, bias} of the unit's column that this lane looks after: read one unit ahead
-        auto table_of = [&](int f, float& m, float& b) {
-            m = f < p.F ? __ldg(p.wscale + f) : 0.0f;
-            b = f < p.F ? __ldg(p.bias + f) : 0.0f;
+        // {multiplier, bias} of the unit's column that this lane looks after, read one unit ahead (volatile: otherwise the compiler moves the
+        // loads down to their use, and every unit waits for them)
+        float wscale = 0.0f, bias = 0.0f;
+        int unit = first_unit, order = group, buf = 0;
+        uint32_t phase = 0;
+        auto settle = [&]() {  // units beyond the tile's: the next tiles
+            while (order >= p.subs) {
+                order -= p.subs;
+                unit += step;
+                if (++buf == p.nbuf) { buf = 0; phase ^= 1u; }
+            }
         };
-        int t = 0, unit = (int)blockIdx.x, order = group;
-        while (order >= p.subs) { order -= p.subs; unit += step; ++t; }
-        auto filter_of = [&]() {
-            const int sub = overlap && t % p.nbuf == 0 ? order ^ 4 : order;  // (what overlaps the other accumulator first)
-            return (unit - fast_div(unit, p.magic_f) * p.tiles_f) * p.bn + sub * CH;
+        auto sub_of = [&]() { return overlap && buf == 0 ? order ^ 4 : order; };  // (what overlaps the other accumulator first)
+        auto prefetch = [&]() {
+            if (unit >= p.num_units) return;
+            const int f = (unit - fast_div(unit, p.magic_f) * p.tiles_f) * p.bn + sub_of() * CH + lane;
+            if (f >= p.F) { wscale = bias = 0.0f; return; }
+            asm volatile("ld.global.nc.f32 %0, [%1];" : "=f"(wscale) : "l"(p.wscale + f));
+            asm volatile("ld.global.nc.f32 %0, [%1];" : "=f"(bias) : "l"(p.bias + f));
         };
-        float mult = 0.0f, bias = 0.0f;
-        if (unit < p.num_tiles) table_of(filter_of() + lane, mult, bias);
+        settle();
+        prefetch();
         bool ok = true;
-        while (unit < p.num_tiles) {
-            const f4_tile at = tile_at(p, unit);
-            const int buf = t % p.nbuf, f0 = filter_of(), sub = (f0 - at.f0) / CH, this_t = t;
+        while (unit < p.num_units) {
+            const f4_tile at = tile_at<PAIR>(p, unit, rank);
+            const int sub = sub_of(), f0 = at.f0 + sub * CH, this_buf = buf;
+            const uint32_t this_phase = phase;
             const bool first = order < 4;
             const int ow = at.ow0 + pw, oh = at.oh0 + ph, n = at.n0 + pn;
             const bool valid = ow < p.OW && oh < p.OH && n < p.N;
-            const long long pix = ((long long)n * p.OH + oh) * p.OW + ow;
-            __syncwarp();  // (the table of the unit before has been read)
-            asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(tab + 8u * lane), "f"(__fmul_rn(p.xscale, mult)), "f"(bias) : "memory");
+            const int pix = (n * p.OH + oh) * p.OW + ow;  // (of a valid row below 2^30)
+            // the table: {m 2i, m 2i + 1, b 2i, b 2i + 1}
+            __syncwarp();  // (that of the unit before has been read)
+            asm volatile("st.shared.f32 [%0], %1;" ::"r"(tab + 16u * (lane >> 1) + 4u * (lane & 1)), "f"(__fmul_rn(p.xscale, wscale)) : "memory");
+            asm volatile("st.shared.f32 [%0], %1;" ::"r"(tab + 16u * (lane >> 1) + 8u + 4u * (lane & 1)), "f"(bias) : "memory");
             __syncwarp();
             order += 4;
-            while (order >= p.subs) { order -= p.subs; unit += step; ++t; }
-            if (unit < p.num_tiles) table_of(filter_of() + lane, mult, bias);
-            if (!(ok = warp_wait(tfull_bar(buf), (uint32_t)((this_t / p.nbuf) & 1), abort_flag, p.status, LN_STATUS_EPILOGUE_TIMEOUT))) break;
+            settle();
+            prefetch();
+            if (!(ok = warp_wait(tfull_bar(this_buf), this_phase, abort_flag, p.status, LN_STATUS_EPILOGUE_TIMEOUT))) break;
             tc_fence_after();
-            const uint32_t taddr = tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(buf * p.acc_step + sub * CH);
+            const uint32_t taddr = tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(this_buf * p.acc_step + sub * CH);
             uint32_t acc[32];
             tmem_ld_32x32(taddr, acc);
             tmem_ld_wait();
             tc_fence_before();
             __syncwarp();
             if (lane == 0) {
-                mbar_arrive(tempty_bar(buf));
-                if (overlap && first) mbar_arrive(early_bar(buf));
+                if (PAIR) {
+                    arrive_first<false>(tempty_bar(this_buf));
+                    if (overlap && first) arrive_first<false>(early_bar(this_buf));
+                } else {
+                    mbar_arrive(tempty_bar(this_buf));
+                    if (overlap && first) mbar_arrive(early_bar(this_buf));
+                }
             }
             // (binary16 channels are padded to 32, 4-bit ones to 64: what is behind them is not stored)
             if (f0 >= (OUT == LN_OUT_Q ? (p.F + 63) & ~63 : p.F)) continue;
@@ -400,9 +532,8 @@ __global__ void __launch_bounds__(kThreadsF4, 1) f4_umma_kernel(const __grid_con
 #pragma unroll
             for (int i = 0; i < 32; i += 2) {
                 float4 e;  // (volatile: the table is another one for every unit)
-                asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(e.x), "=f"(e.y), "=f"(e.z), "=f"(e.w) : "r"(tab + 8u * i) : "memory");
-                v[i] = __fmaf_rn(__uint_as_float(acc[i]), e.x, e.y);
-                v[i + 1] = __fmaf_rn(__uint_as_float(acc[i + 1]), e.z, e.w);
+                asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(e.x), "=f"(e.y), "=f"(e.z), "=f"(e.w) : "r"(tab + 8u * i));
+                ffma2(v[i], v[i + 1], __uint_as_float(acc[i]), __uint_as_float(acc[i + 1]), e.x, e.y, e.z, e.w);
             }
             act_all(p.act, p.exact != 0, v);
             if (f0 + 32 > p.F) {
@@ -412,8 +543,8 @@ __global__ void __launch_bounds__(kThreadsF4, 1) f4_umma_kernel(const __grid_con
             }
             if (OUT == LN_OUT_F32) {
                 if (valid) {
-                    const long long img = pix / p.hw;
-                    float* dst = (float*)p.y + (img * p.F + f0) * p.hw + (pix - img * p.hw);
+                    const int img = pix / p.hw;
+                    float* dst = (float*)p.y + ((long long)img * p.F + f0) * p.hw + (pix - img * p.hw);
 #pragma unroll
                     for (int i = 0; i < 32; ++i)
                         if (f0 + i < p.F) dst[(long long)i * p.hw] = v[i];
@@ -426,7 +557,7 @@ __global__ void __launch_bounds__(kThreadsF4, 1) f4_umma_kernel(const __grid_con
                     h[i >> 3][i & 7] = *reinterpret_cast<const uint32_t*>(&q);
                 }
                 if (valid) {
-                    uint8_t* dst = (uint8_t*)p.y + pix * p.ys + 2 * f0;
+                    uint8_t* dst = (uint8_t*)p.y + (long long)pix * p.ys + 2 * f0;
                     store_32(dst, h[0]);
                     store_32(dst + 32, h[1]);
                 }
@@ -436,7 +567,7 @@ __global__ void __launch_bounds__(kThreadsF4, 1) f4_umma_kernel(const __grid_con
 #pragma unroll
                 for (int b = 0; b < 32 / B; ++b) sf |= ln_f4_quantise<FMT>(v + b * B, p.g, p.six_g, q + b * B / 8) << (8 * b);
                 if (valid) {
-                    *(uint4*)((uint8_t*)p.y + pix * p.ys + f0 / 2) = make_uint4(q[0], q[1], q[2], q[3]);
+                    *(uint4*)((uint8_t*)p.y + (long long)pix * p.ys + f0 / 2) = make_uint4(q[0], q[1], q[2], q[3]);
                     uint8_t* at_sf = p.ysf + ln_f4_sf_at(pix, f0 / (4 * B), p.ysf_words) + f0 / B % 4;
                     if (FMT == LN_F4) *(uint16_t*)at_sf = (uint16_t)sf;
                     else *at_sf = (uint8_t)sf;
@@ -452,9 +583,11 @@ __global__ void __launch_bounds__(kThreadsF4, 1) f4_umma_kernel(const __grid_con
         for (int i = 0; i < 64; ++i) __nanosleep(20000);
     }
     __syncthreads();
+    if (PAIR) pair_sync();  // neither CTA leaves while the other may still signal its barriers or work in its TMEM
     if (warp == 1) {
         tc_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512u) : "memory");
+        if (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512u) : "memory");
+        else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512u) : "memory");
     }
 }
 
@@ -465,17 +598,28 @@ int log2_of(int v) {
 }
 
 template <int FMT, int OUT>
-cudaError_t launch(ln_ctx* ctx, const f4_params& p, int grid, size_t smem) {
+cudaError_t launch(ln_ctx* ctx, const f4_params& p, bool pair, int grid, size_t smem) {
     auto go = [&](void (*k)(const f4_params)) -> cudaError_t {
         if (!ctx->configured_kernels.count((const void*)k)) {
             const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmemF4);
             if (e != cudaSuccess) return e;
             ctx->configured_kernels.insert((const void*)k);
         }
-        k<<<grid, kThreadsF4, smem, ctx->stream>>>(p);
-        return cudaGetLastError();
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3((unsigned)grid);
+        cfg.blockDim = dim3(kThreadsF4);
+        cfg.dynamicSmemBytes = smem;
+        cfg.stream = ctx->stream;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = pair ? 2 : 1;
+        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        return cudaLaunchKernelEx(&cfg, k, p);
     };
-    return p.bn > 128 ? go(f4_umma_kernel<FMT, OUT, 2>) : go(f4_umma_kernel<FMT, OUT, 1>);
+    if (pair) return go(f4_umma_kernel<FMT, OUT, 2, true>);
+    return p.bn > 128 ? go(f4_umma_kernel<FMT, OUT, 2, false>) : go(f4_umma_kernel<FMT, OUT, 1, false>);
 }
 
 }  // namespace
@@ -527,24 +671,26 @@ int ln_f4_umma_launch(ln_ctx* ctx, const ln_f4_conv& c) {
             if (atoi(e) == bn) p.bn = bn;
     }
     const int wblocks = p.bn > 128 ? 2 : 1;
+    bool pair = p.bn > 128 && best > 1;
+    if (const char* e = getenv("LN_F4_PAIR")) pair = pair && atoi(e) != 0;  // (A/B measurements: no CTA pairs)
     p.nbuf = p.bn == 256 ? 2 : (int)kScaleCols / p.bn;
     p.acc_step = p.bn == 256 ? kOverlapBase : p.bn;
     p.subs = p.bn / CH;
     p.flat = flat ? 1 : 0;
     p.tiles_f = (p.F + p.bn - 1) / p.bn; p.tiles_w = (p.OW + p.TW - 1) / p.TW; p.tiles_h = (p.OH + p.TH - 1) / p.TH;
-    const int64_t num_tiles = best * p.tiles_f;
-    if (num_tiles >= (1 << 20)) return ln_fail(ctx, LN_ERR_UNSUPPORTED, "%s: %lld tiles", who, (long long)num_tiles);
-    p.num_tiles = (int)num_tiles;
+    const int64_t num_units = (pair ? (best + 1) / 2 : best) * p.tiles_f;
+    if (num_units >= (1 << 19)) return ln_fail(ctx, LN_ERR_UNSUPPORTED, "%s: %lld tiles", who, (long long)num_units);
+    p.num_units = (int)num_units;
     auto magic = [](int d) { return ((1ull << 40) + (unsigned long long)d - 1) / (unsigned long long)d; };
     p.magic_f = magic(p.tiles_f); p.magic_w = magic(p.tiles_w); p.magic_h = magic(p.tiles_h);
     p.off_b = 128u * p.bk;
-    p.off_sfa = p.off_b + (uint32_t)p.bn * p.bk;
+    p.off_sfa = p.off_b + (uint32_t)(pair ? p.bn / 2 : p.bn) * p.bk;
     p.off_sfb = p.off_sfa + (uint32_t)p.words * 512u;
     p.stage_bytes = (uint32_t)ln_round_up(p.off_sfb + (uint32_t)(p.words * wblocks) * 512u, 1024);
     p.stages = (int)((kMaxSmemF4 - 1024 - kBarBytesF4 - kTabBytesF4) / p.stage_bytes);
     if (p.stages > kMaxStagesF4) p.stages = kMaxStagesF4;
     const size_t smem = 1024 + (size_t)p.stages * p.stage_bytes + kBarBytesF4 + kTabBytesF4;
-    p.xsf = (const uint8_t*)x.sf; p.wsf = (const uint8_t*)c.w->sf; p.wscale = c.w->wscale; p.bias = c.bias;
+    p.xsf = (const uint8_t*)x.sf; p.wscale = c.w->wscale; p.bias = c.bias;
     p.y = y.ptr; p.ys = y.cstride; p.ysf = (uint8_t*)y.sf; p.ysf_words = y.sf_words;
     p.xscale = x.scale; p.g = y.scale; p.six_g = 6.0f * y.scale;
     p.act = c.act; p.exact = ctx->exact_epilogue ? 1 : 0;
@@ -568,15 +714,29 @@ int ln_f4_umma_launch(ln_ctx* ctx, const ln_f4_conv& c) {
     {
         const cuuint64_t dims[2] = {(cuuint64_t)((int64_t)c.k * c.k * x.cstride), (cuuint64_t)p.F};
         const cuuint64_t strides[1] = {(cuuint64_t)((int64_t)c.k * c.k * x.cstride)};
-        const cuuint32_t box[2] = {(cuuint32_t)p.bk, (cuuint32_t)p.bn};
+        const cuuint32_t box[2] = {(cuuint32_t)p.bk, (cuuint32_t)(pair ? p.bn / 2 : p.bn)};
         const CUresult r = ctx->encode_tiled(&p.tmB, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, c.w->w, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swz, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
                                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
         if (r != CUDA_SUCCESS) return ln_fail(ctx, LN_ERR_CUDA, "%s: cuTensorMapEncodeTiled(weights) failed with %d", who, (int)r);
     }
-    const int grid = p.num_tiles < ctx->sm_count ? p.num_tiles : ctx->sm_count;
+    {
+        const int64_t rows = (int64_t)c.k * c.k * kb.cblocks * kb.words, groups = c.w->fpad / 128;
+        const cuuint64_t dims[3] = {128, (cuuint64_t)rows, (cuuint64_t)groups};
+        const cuuint64_t strides[2] = {512, (cuuint64_t)rows * 512};
+        const cuuint32_t box[3] = {128, (cuuint32_t)kb.words, (cuuint32_t)wblocks};
+        CUresult r = ctx->encode_tiled(&p.tmWS, CU_TENSOR_MAP_DATA_TYPE_UINT32, 3, c.w->sf, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
+                                       CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+        if (r == CUDA_SUCCESS && flat) {
+            const cuuint64_t xdims[2] = {128, (cuuint64_t)((pixels + 127) / 128 * x.sf_words)};
+            r = ctx->encode_tiled(&p.tmXS, CU_TENSOR_MAP_DATA_TYPE_UINT32, 2, x.sf, xdims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
+                                  CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+        }
+        if (r != CUDA_SUCCESS) return ln_fail(ctx, LN_ERR_CUDA, "%s: cuTensorMapEncodeTiled(scales) failed with %d", who, (int)r);
+    }
+    const int places = pair ? ctx->sm_count / 2 : ctx->sm_count, grid = (p.num_units < places ? p.num_units : places) * (pair ? 2 : 1);
     cudaError_t e;
 #define LN_F4_LAUNCH(FMT) \
-    (c.out_kind == LN_OUT_F32 ? launch<FMT, LN_OUT_F32>(ctx, p, grid, smem) : c.out_kind == LN_OUT_F16 ? launch<FMT, LN_OUT_F16>(ctx, p, grid, smem) : launch<FMT, LN_OUT_Q>(ctx, p, grid, smem))
+    (c.out_kind == LN_OUT_F32 ? launch<FMT, LN_OUT_F32>(ctx, p, pair, grid, smem) : c.out_kind == LN_OUT_F16 ? launch<FMT, LN_OUT_F16>(ctx, p, pair, grid, smem) : launch<FMT, LN_OUT_Q>(ctx, p, pair, grid, smem))
     e = c.dtype == LN_F4 ? LN_F4_LAUNCH(LN_F4) : LN_F4_LAUNCH(LN_MX4);
 #undef LN_F4_LAUNCH
     ctx->launches++;
