@@ -191,11 +191,16 @@ def load_library():
     return _lib
 
 
+_I64x4 = C.c_int64 * 4
+
+
 def _shape4(shape):
-    s = tuple(int(v) for v in shape)
-    if len(s) != 4:
+    if len(shape) != 4:
         raise ValueError("shapes are [batch, channels, height, width]")
-    return (C.c_int64 * 4)(*s)
+    try:
+        return _I64x4(*shape)
+    except TypeError:  # (other number types)
+        return _I64x4(*[int(v) for v in shape])
 
 
 def _ptr(a):
@@ -221,9 +226,9 @@ class Tensor:
 
     @property
     def shape(self):
-        s = (C.c_int64 * 4)()
+        s = _I64x4()
         _lib.ln_tensor_shape(self.h, s)
-        return tuple(int(v) for v in s)
+        return tuple(s)
 
     @property
     def dtype(self):
@@ -233,17 +238,21 @@ class Tensor:
     def scale(self):
         return float(_lib.ln_tensor_scale(self.h))
 
-    @property
-    def __cuda_array_interface__(self):
-        """f32 and binary16 tensors for other libraries on the same GPU (`torch.as_tensor(t, device="cuda")` shares the memory and keeps
-        the handle); order their work behind the backend's stream."""
+    def __getattr__(self, name):
+        """`__cuda_array_interface__`: f32 and binary16 tensors for other libraries on the same GPU (`torch.as_tensor(t, device="cuda")`
+        shares the memory and keeps the handle); order their work behind the backend's stream.  Made when it is first asked for."""
+        if name != "__cuda_array_interface__":
+            raise AttributeError(name)
         dtype = self.dtype
         if dtype not in (LN_F32, LN_F16):
             raise AttributeError("only f32 and binary16 tensors have an array interface")
-        size, p, s = 4 if dtype == LN_F32 else 2, C.c_void_p(), (C.c_int64 * 4)()
+        size, p, s = 4 if dtype == LN_F32 else 2, C.c_void_p(), _I64x4()
         self.backend._check(_lib.ln_tensor_device_data(self.h, C.byref(p), s))
-        return {"shape": self.shape, "typestr": "<f%d" % size, "data": (p.value, False), "strides": tuple(size * v for v in s), "version": 3,
-                "stream": int(self.backend.stream)}
+        n, c, h, w = s
+        self.__cuda_array_interface__ = d = {
+            "shape": self.shape, "typestr": "<f4" if size == 4 else "<f2", "data": (p.value, False), "strides": (size * n, size * c, size * h, size * w),
+            "version": 3, "stream": self.backend.stream}
+        return d
 
 
 class ConvWeights:
@@ -280,7 +289,9 @@ class B200Backend:
 
     def _out(self, fn, *args):
         h = C.c_void_p()
-        self._check(fn(self.ctx, *args, C.byref(h)))
+        rc = fn(self.ctx, *args, C.byref(h))
+        if rc:
+            self._check(rc)
         return Tensor(self, h)
 
     def sync(self):

@@ -12,7 +12,7 @@
 
 #include <cstdint>
 
-#include "ln_common.h"
+#include "ln_umma.h"
 
 inline bool ln_is_f4(int dtype) { return dtype == LN_F4 || dtype == LN_MX4; }
 inline int ln_f4_block(int dtype) { return dtype == LN_MX4 ? 32 : 16; }
@@ -43,6 +43,13 @@ __host__ __device__ __forceinline__ int64_t ln_f4_sf_at(int64_t q, int64_t w, in
 }
 
 // ---- the number formats -----------------------------------------------------------------------------------------------------------
+
+// The 4-bit kernels are launched as programmatic dependents: they may start, and set up what is their own, while the kernel in front of
+// them still runs.  Every thread comes by here before it reads or writes global memory.
+__device__ __forceinline__ void ln_f4_after_predecessor() {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+}
 
 // max that hands a NaN on
 __device__ __forceinline__ float ln_max_nan(float a, float b) {
@@ -122,9 +129,11 @@ __device__ __forceinline__ uint32_t ln_f4_quantise(const float* x, float g, floa
             // The result is the rounded quotient but where that is within 2^-22 steps of the middle of two numbers.
             const float r = scale ? __frcp_rn(d) : 0.0f;
 #pragma unroll
-            for (int i = 0; i < B; ++i) {
-                const float q = __fmul_rn(x[i], r);
-                t[i] = __fmaf_rn(__fmaf_rn(-q, d, x[i]), r, q);
+            for (int i = 0; i < B; i += 2) {
+                float q0, q1, e0, e1;
+                fmul2(q0, q1, x[i], x[i + 1], r, r);
+                ffma2(e0, e1, -q0, -q1, d, d, x[i], x[i + 1]);
+                ffma2(t[i], t[i + 1], e0, e1, r, r, q0, q1);
             }
         }
     } else {
@@ -148,5 +157,20 @@ struct ln_f4_conv {  // one convolution: operands, geometry, output
     ln_tensor* y = nullptr;
     int k = 1, stride = 1, pad = 0, act = 0, out_kind = LN_OUT_F32;
 };
+// launches a 4-bit kernel (all begin with ln_f4_after_predecessor) on the ctx stream
+template <typename... P, typename... A>
+inline cudaError_t ln_f4_launch(ln_ctx* ctx, void (*kernel)(P...), int grid, int threads, A... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)grid);
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.stream = ctx->stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    ctx->launches++;
+    return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+}
 bool ln_f4_umma_takes(const ln_f4_conv& c, int64_t stride_x, int64_t stride_y);
 int ln_f4_umma_launch(ln_ctx* ctx, const ln_f4_conv& c);

@@ -11,14 +11,17 @@ namespace {
 
 constexpr int kThreads = 256;
 
+// 16 bytes that are read once
+__device__ __forceinline__ uint4 ln_ldg_stream(const __half* p) { return __ldcs(reinterpret_cast<const uint4*>(p)); }
+
 int grid_for(ln_ctx* ctx, int64_t n) {
     const int64_t b = (n + kThreads - 1) / kThreads, cap = (int64_t)ctx->sm_count * 16;
     return (int)(b < 1 ? 1 : (b > cap ? cap : b));
 }
-int check_launch(ln_ctx* ctx, const char* what) {
-    ctx->launches++;
-    const cudaError_t e = cudaGetLastError();
-    return e == cudaSuccess ? LN_OK : ln_fail(ctx, LN_ERR_CUDA, "%s: kernel launch failed: %s", what, cudaGetErrorString(e));
+int check_launch(ln_ctx* ctx, const char* what, cudaError_t e) {
+    if (e == cudaSuccess) return LN_OK;
+    (void)cudaGetLastError();  // (the next launch is checked for its own error)
+    return ln_fail(ctx, LN_ERR_CUDA, "%s: kernel launch failed: %s", what, cudaGetErrorString(e));
 }
 // A new tensor, or the status of why there is none.
 int new_tensor(ln_ctx* ctx, int dtype, int64_t n, int64_t c, int64_t h, int64_t w, ln_tensor** out) {
@@ -37,66 +40,98 @@ int32_t guarded(ln_ctx* ctx, const char* who, F&& body) {
 // Tensor scales that keep 6 g, every product of g with a block scale and its reciprocal normal numbers.
 bool usable_scale(int dtype, float s) { return dtype == LN_MX4 ? s == 1.0f : s >= 0x1p-100f && s <= 0x1p100f; }
 
-// ---- narrow ---------------------------------------------------------------------------------------------------------------------
-// One thread per block of 16 or 32 channels.
+// ---- narrow and widen -----------------------------------------------------------------------------------------------------------
+// binary16 NHWC: a thread takes 32 channels of a pixel, consecutive threads consecutive groups of them, so that all accesses of a warp are
+// contiguous; two neighbours, which always belong to one pixel (its channels are padded to 64), put their scale bytes together.
+// f32 NCHW: the 32 lanes of a warp are 8 pixels x 4 blocks, so that a row of 8 pixels is a sector of a plane on one side and the four
+// blocks of a pixel (32 or 64 bytes of codes, one word of scales) are contiguous on the other.
+// I: 32-bit indexes where they suffice (a division per thread).
 
 template <int FMT>
-__device__ __forceinline__ void store_block(const float* x, float g, float six_g, uint8_t* codes, uint8_t* scale) {
+__device__ __forceinline__ uint32_t store_block(const float* x, float g, float six_g, uint8_t* codes) {
     constexpr int B = FMT == LN_F4 ? 16 : 32;
     uint32_t w[B / 8];
-    *scale = (uint8_t)ln_f4_quantise<FMT>(x, g, six_g, w);
+    const uint32_t scale = ln_f4_quantise<FMT>(x, g, six_g, w);
     if (FMT == LN_F4) *reinterpret_cast<uint2*>(codes) = make_uint2(w[0], w[1]);
     else *reinterpret_cast<uint4*>(codes) = make_uint4(w[0], w[1], w[B / 8 - 2], w[B / 8 - 1]);
+    return scale;
 }
-
-// f32 NCHW: consecutive threads take consecutive pixels, so that the reads are contiguous.
-template <int FMT>
-__global__ void narrow_f32_kernel(const float* __restrict__ x, uint8_t* __restrict__ codes, uint8_t* __restrict__ sf, int64_t pixels, int64_t hw, int C, int blocks,
-                                  int64_t cstride, int64_t sf_words, float g, float six_g) {
+template <int FMT, typename I>
+__global__ void __launch_bounds__(kThreads) narrow_f16_kernel(const __half* __restrict__ x, int64_t xs, uint8_t* __restrict__ codes, uint8_t* __restrict__ sf, int64_t pixels, int C, int groups,
+                                                              int64_t cstride, int64_t sf_words, float g, float six_g) {
+    ln_f4_after_predecessor();
     constexpr int B = FMT == LN_F4 ? 16 : 32;
-    for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < pixels * blocks; i += (int64_t)gridDim.x * blockDim.x) {
-        const int64_t pix = i % pixels;
-        const int b = (int)(i / pixels);
-        const float* src = x + (pix / hw * C + b * B) * hw + pix % hw;
-        float v[B];
+    const I total = (I)(pixels * groups), step = (I)(gridDim.x * blockDim.x);
+    for (I i = (I)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += step) {  // (total is even: the lanes of a pair leave together)
+        const I pix = i / (I)groups;
+        const int c0 = (int)(i - pix * (I)groups) * 32;
+        uint4 q[4];
 #pragma unroll
-        for (int j = 0; j < B; ++j) v[j] = b * B + j < C ? src[j * hw] : 0.0f;
-        store_block<FMT>(v, g, six_g, codes + pix * cstride + b * (B / 2), sf + ln_f4_sf_at(pix, b >> 2, sf_words) + (b & 3));
-    }
-}
-// binary16 NHWC: consecutive threads take consecutive blocks of a pixel.
-template <int FMT>
-__global__ void narrow_f16_kernel(const __half* __restrict__ x, int64_t xs, uint8_t* __restrict__ codes, uint8_t* __restrict__ sf, int64_t pixels, int C, int blocks,
-                                  int64_t cstride, int64_t sf_words, float g, float six_g) {
-    constexpr int B = FMT == LN_F4 ? 16 : 32;
-    for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < pixels * blocks; i += (int64_t)gridDim.x * blockDim.x) {
-        const int64_t pix = i / blocks;
-        const int b = (int)(i - pix * blocks);
-        float v[B];
+        for (int j = 0; j < 4; ++j) q[j] = c0 < C ? ln_ldg_stream(x + (int64_t)pix * xs + c0 + 8 * j) : make_uint4(0, 0, 0, 0);  // (a pixel's channels are padded to 32)
+        float v[32];
 #pragma unroll
-        for (int j = 0; j < B; j += 8) {
-            uint4 q = make_uint4(0, 0, 0, 0);
-            if (b * B + j < C) q = *reinterpret_cast<const uint4*>(x + pix * xs + b * B + j);  // (a pixel's channels are padded to 32)
-            const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+        for (int j = 0; j < 4; ++j) {
+            const uint32_t w[4] = {q[j].x, q[j].y, q[j].z, q[j].w};
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[k]));
-                v[j + 2 * k] = b * B + j + 2 * k < C ? f.x : 0.0f;
-                v[j + 2 * k + 1] = b * B + j + 2 * k + 1 < C ? f.y : 0.0f;
+                v[8 * j + 2 * k] = f.x;
+                v[8 * j + 2 * k + 1] = f.y;
             }
         }
-        store_block<FMT>(v, g, six_g, codes + pix * cstride + b * (B / 2), sf + ln_f4_sf_at(pix, b >> 2, sf_words) + (b & 3));
+        if (c0 + 32 > C) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+                if (c0 + j >= C) v[j] = 0.0f;
+        }
+        uint32_t w[4], s = 0;
+#pragma unroll
+        for (int b = 0; b < 32 / B; ++b) s |= ln_f4_quantise<FMT>(v + b * B, g, six_g, w + b * B / 8) << (8 * b);
+        *reinterpret_cast<uint4*>(codes + (int64_t)pix * cstride + c0 / 2) = make_uint4(w[0], w[1], w[2], w[3]);
+        const uint32_t other = __shfl_down_sync(__activemask(), s, 1);
+        if ((c0 & 32) == 0) {
+            uint8_t* dst = sf + ln_f4_sf_at(pix, c0 / (4 * B), sf_words) + c0 / B % 4;
+            if (FMT == LN_F4) *reinterpret_cast<uint32_t*>(dst) = s | other << 16;
+            else *reinterpret_cast<uint16_t*>(dst) = (uint16_t)(s | other << 8);
+        }
+    }
+}
+template <int FMT, typename I>
+__global__ void __launch_bounds__(kThreads) narrow_f32_kernel(const float* __restrict__ x, uint8_t* __restrict__ codes, uint8_t* __restrict__ sf, int64_t pixels, int64_t hw, int C, int blocks,
+                                                              int64_t cstride, int64_t sf_words, float g, float six_g) {
+    ln_f4_after_predecessor();
+    constexpr int B = FMT == LN_F4 ? 16 : 32;
+    const I rows = (I)((pixels + 7) / 8), warps = rows * (I)((blocks + 3) / 4), step = (I)(gridDim.x * (blockDim.x / 32));
+    const int lane = threadIdx.x & 31;
+    for (I w = (I)blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32; w < warps; w += step) {
+        const I quad = w / rows;
+        const I pix = (w - quad * rows) * 8 + (lane >> 2);
+        const int b = (int)quad * 4 + (lane & 3);
+        uint32_t s = 0;
+        if (pix < (I)pixels && b < blocks) {
+            const I img = pix / (I)hw;
+            const float* src = x + ((int64_t)img * C + b * B) * hw + (pix - img * (I)hw);
+            float v[B];
+            if (b * B + B <= C) {
+#pragma unroll
+                for (int j = 0; j < B; ++j) v[j] = __ldg(src + j * hw);
+            } else {
+#pragma unroll
+                for (int j = 0; j < B; ++j) v[j] = b * B + j < C ? __ldg(src + j * hw) : 0.0f;
+            }
+            s = store_block<FMT>(v, g, six_g, codes + (int64_t)pix * cstride + b * (B / 2));
+        }
+        s |= __shfl_down_sync(0xFFFFFFFFu, s, 1) << 8;
+        s |= __shfl_down_sync(0xFFFFFFFFu, s, 2) << 16;
+        // (behind the last block of LN_MX4 a word may have two bytes that nothing uses)
+        if ((lane & 3) == 0 && pix < (I)pixels) *reinterpret_cast<uint32_t*>(sf + ln_f4_sf_at(pix, b >> 2, sf_words)) = s;
     }
 }
 
-// ---- widen ----------------------------------------------------------------------------------------------------------------------
-// One thread per 16 channels of a pixel.
-
+// 16 channels
 template <int FMT>
-__device__ __forceinline__ void load_16(const uint8_t* codes, const uint8_t* sf, int64_t pix, int64_t sf_words, int b16, float g, float (&v)[16]) {
-    const int b = FMT == LN_F4 ? b16 : b16 >> 1;
-    const float d = ln_f4_factor<FMT>(sf[ln_f4_sf_at(pix, b >> 2, sf_words) + (b & 3)], g);
-    const uint2 w = *reinterpret_cast<const uint2*>(codes + b16 * 8);
+__device__ __forceinline__ void widen_16(uint2 w, uint32_t scale, float g, float (&v)[16]) {
+    const float d = ln_f4_factor<FMT>(scale, g);
     uint32_t h[8];
     ln_e2m1x8_to_h2(w.x, *reinterpret_cast<uint32_t(*)[4]>(h));
     ln_e2m1x8_to_h2(w.y, *reinterpret_cast<uint32_t(*)[4]>(h + 4));
@@ -107,43 +142,68 @@ __device__ __forceinline__ void load_16(const uint8_t* codes, const uint8_t* sf,
         v[2 * k + 1] = __fmul_rn(f.y, d);
     }
 }
-template <int FMT>
-__global__ void widen_f32_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ sf, float* __restrict__ y, int64_t pixels, int64_t hw, int C, int blocks,
-                                 int64_t cstride, int64_t sf_words, float g) {
-    for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < pixels * blocks; i += (int64_t)gridDim.x * blockDim.x) {
-        const int64_t pix = i % pixels;
-        const int b = (int)(i / pixels);
-        float v[16];
-        load_16<FMT>(codes + pix * cstride, sf, pix, sf_words, b, g, v);
-        float* dst = y + (pix / hw * C + b * 16) * hw + pix % hw;
+template <int FMT, typename I>
+__global__ void __launch_bounds__(kThreads) widen_f16_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ sf, __half* __restrict__ y, int64_t ys, int64_t pixels, int C, int groups,
+                                                             int64_t cstride, int64_t sf_words, float g) {
+    ln_f4_after_predecessor();
+    constexpr int B = FMT == LN_F4 ? 16 : 32;
+    const I total = (I)(pixels * groups), step = (I)(gridDim.x * blockDim.x);
+    for (I i = (I)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += step) {
+        const I pix = i / (I)groups;
+        const int c0 = (int)(i - pix * (I)groups) * 32;
+        const uint4 q = __ldg(reinterpret_cast<const uint4*>(codes + (int64_t)pix * cstride + c0 / 2));
+        const uint8_t* s = sf + ln_f4_sf_at(pix, c0 / (4 * B), sf_words) + c0 / B % 4;
+        const uint32_t scale = FMT == LN_F4 ? __ldg(reinterpret_cast<const uint16_t*>(s)) : __ldg(s);
+        float v[2][16];
+        widen_16<FMT>(make_uint2(q.x, q.y), scale & 0xFFu, g, v[0]);
+        widen_16<FMT>(make_uint2(q.z, q.w), FMT == LN_F4 ? scale >> 8 : scale, g, v[1]);
+        if (c0 + 32 > C) {  // (a NaN block that ends inside the padding must not reach it)
 #pragma unroll
-        for (int j = 0; j < 16; ++j)
-            if (b * 16 + j < C) dst[j * hw] = v[j];
+            for (int j = 0; j < 32; ++j)
+                if (c0 + j >= C) v[j >> 4][j & 15] = 0.0f;
+        }
+        uint4* dst = reinterpret_cast<uint4*>(y + (int64_t)pix * ys + c0);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            uint32_t h[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const __half2 p = __floats2half2_rn(v[j >> 1][(j & 1) * 8 + 2 * k], v[j >> 1][(j & 1) * 8 + 2 * k + 1]);
+                h[k] = *reinterpret_cast<const uint32_t*>(&p);
+            }
+            dst[j] = make_uint4(h[0], h[1], h[2], h[3]);
+        }
     }
 }
-template <int FMT>
-__global__ void widen_f16_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ sf, __half* __restrict__ y, int64_t ys, int64_t pixels, int C, int blocks,
-                                 int64_t cstride, int64_t sf_words, float g) {
-    for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < pixels * blocks; i += (int64_t)gridDim.x * blockDim.x) {
-        const int64_t pix = i / blocks;
-        const int b = (int)(i - pix * blocks);
+template <int FMT, typename I>
+__global__ void __launch_bounds__(kThreads) widen_f32_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ sf, float* __restrict__ y, int64_t pixels, int64_t hw, int C, int blocks,
+                                                             int64_t cstride, int64_t sf_words, float g) {
+    ln_f4_after_predecessor();  // (blocks of 16 channels for both types)
+    const I rows = (I)((pixels + 7) / 8), warps = rows * (I)((blocks + 3) / 4), step = (I)(gridDim.x * (blockDim.x / 32));
+    const int lane = threadIdx.x & 31;
+    for (I w = (I)blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32; w < warps; w += step) {
+        const I quad = w / rows;
+        const I pix = (w - quad * rows) * 8 + (lane >> 2);
+        const int b16 = (int)quad * 4 + (lane & 3), b = FMT == LN_F4 ? b16 : b16 >> 1;
+        if (pix >= (I)pixels || b16 >= blocks) continue;
         float v[16];
-        load_16<FMT>(codes + pix * cstride, sf, pix, sf_words, b, g, v);
-        uint32_t h[8];
+        widen_16<FMT>(__ldg(reinterpret_cast<const uint2*>(codes + (int64_t)pix * cstride + b16 * 8)), __ldg(sf + ln_f4_sf_at(pix, b >> 2, sf_words) + (b & 3)), g, v);
+        const I img = pix / (I)hw;
+        float* dst = y + ((int64_t)img * C + b16 * 16) * hw + (pix - img * (I)hw);
+        if (b16 * 16 + 16 <= C) {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            // (a NaN block that ends inside the padding must not reach it)
-            const __half2 p = __floats2half2_rn(b * 16 + 2 * k < C ? v[2 * k] : 0.0f, b * 16 + 2 * k + 1 < C ? v[2 * k + 1] : 0.0f);
-            h[k] = *reinterpret_cast<const uint32_t*>(&p);
+            for (int j = 0; j < 16; ++j) dst[j * hw] = v[j];
+        } else {
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+                if (b16 * 16 + j < C) dst[j * hw] = v[j];
         }
-        uint4* dst = reinterpret_cast<uint4*>(y + pix * ys + b * 16);
-        dst[0] = make_uint4(h[0], h[1], h[2], h[3]);
-        dst[1] = make_uint4(h[4], h[5], h[6], h[7]);
     }
 }
 // codes (one per byte) and scales in NCHW order
 __global__ void unpack_f4_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ sf, uint8_t* __restrict__ out_codes, uint8_t* __restrict__ out_sf, int64_t n, int64_t hw,
                                  int C, int sf_blocks, int64_t cstride, int64_t sf_words) {
+    ln_f4_after_predecessor();
     const int64_t first = n * C * hw, total = first + n * sf_blocks * hw;
     for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
         const int64_t k = i < first ? i : i - first;
@@ -160,6 +220,7 @@ __global__ void unpack_f4_kernel(const uint8_t* __restrict__ codes, const uint8_
 template <int FMT>
 __global__ void pack_weights_f4_kernel(const float* __restrict__ w, int C, int k2, int64_t cstride, uint8_t* __restrict__ codes, uint8_t* __restrict__ sf, float* __restrict__ wscale,
                                        int64_t sf_words) {
+    ln_f4_after_predecessor();
     constexpr int B = FMT == LN_F4 ? 16 : 32;
     const int f = blockIdx.x;
     const float* src = w + (int64_t)f * C * k2;
@@ -182,7 +243,7 @@ __global__ void pack_weights_f4_kernel(const float* __restrict__ w, int C, int k
 #pragma unroll
         for (int j = 0; j < B; ++j) v[j] = b * B + j < C ? src[(int64_t)(b * B + j) * k2 + tap] : 0.0f;
         const int64_t at = ln_f4_sf_at(f, (int64_t)tap * sf_words + (b >> 2), k2 * sf_words) + (b & 3);
-        store_block<FMT>(v, g, 6.0f * g, codes + ((int64_t)f * k2 + tap) * cstride + b * (B / 2), sf + at);
+        sf[at] = (uint8_t)store_block<FMT>(v, g, 6.0f * g, codes + ((int64_t)f * k2 + tap) * cstride + b * (B / 2));
     }
 }
 
@@ -198,6 +259,7 @@ struct simt_params {
 // One thread per output value, filters fastest.  Takes every geometry.
 template <int FMT, bool EXACT>
 __global__ void conv_f4_simt_kernel(const simt_params p) {
+    ln_f4_after_predecessor();
     constexpr int B = FMT == LN_F4 ? 16 : 32;
     for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < p.total; i += (int64_t)gridDim.x * blockDim.x) {
         const int f = (int)(i % p.F);
@@ -242,21 +304,42 @@ __global__ void conv_f4_simt_kernel(const simt_params p) {
     }
 }
 
+// one launch with 32-bit indexes where every index, and the step behind the last one, stays below 2^31
+#define LN_F4_CALL(KERNEL, FMT, SMALL, GRID, ...) \
+    ((FMT) == LN_F4 ? ((SMALL) ? ln_f4_launch(ctx, KERNEL<LN_F4, uint32_t>, GRID, kThreads, __VA_ARGS__) : ln_f4_launch(ctx, KERNEL<LN_F4, int64_t>, GRID, kThreads, __VA_ARGS__)) \
+                    : ((SMALL) ? ln_f4_launch(ctx, KERNEL<LN_MX4, uint32_t>, GRID, kThreads, __VA_ARGS__) : ln_f4_launch(ctx, KERNEL<LN_MX4, int64_t>, GRID, kThreads, __VA_ARGS__)))
+
 int narrow_into(ln_ctx* ctx, const ln_tensor* t, ln_tensor* q) {
     const int64_t pixels = t->n * t->h * t->w, hw = t->h * t->w;
-    const int blocks = (int)(q->cstride * 2 / ln_f4_block(q->dtype));
-    const int grid = grid_for(ctx, pixels * blocks);
     uint8_t *codes = (uint8_t*)q->ptr, *sf = (uint8_t*)q->sf;
     const float g = q->scale, six_g = 6.0f * g;
+    const bool small = q->cstride * pixels < (1ll << 30);
+    cudaError_t e;
     if (t->dtype == LN_F32) {
-        if (q->dtype == LN_F4) narrow_f32_kernel<LN_F4><<<grid, kThreads, 0, ctx->stream>>>((const float*)t->ptr, codes, sf, pixels, hw, (int)t->c, blocks, q->cstride, q->sf_words, g, six_g);
-        else narrow_f32_kernel<LN_MX4><<<grid, kThreads, 0, ctx->stream>>>((const float*)t->ptr, codes, sf, pixels, hw, (int)t->c, blocks, q->cstride, q->sf_words, g, six_g);
+        const int blocks = (int)(q->cstride * 2 / ln_f4_block(q->dtype));
+        e = LN_F4_CALL(narrow_f32_kernel, q->dtype, small, grid_for(ctx, (pixels + 7) / 8 * ((blocks + 3) / 4) * 32), (const float*)t->ptr, codes, sf, pixels, hw, (int)t->c, blocks, q->cstride, q->sf_words, g,
+                       six_g);
     } else {
-        if (q->dtype == LN_F4) narrow_f16_kernel<LN_F4><<<grid, kThreads, 0, ctx->stream>>>((const __half*)t->ptr, t->cstride / 2, codes, sf, pixels, (int)t->c, blocks, q->cstride, q->sf_words, g, six_g);
-        else narrow_f16_kernel<LN_MX4><<<grid, kThreads, 0, ctx->stream>>>((const __half*)t->ptr, t->cstride / 2, codes, sf, pixels, (int)t->c, blocks, q->cstride, q->sf_words, g, six_g);
+        const int groups = (int)(q->cstride / 16);
+        e = LN_F4_CALL(narrow_f16_kernel, q->dtype, small, grid_for(ctx, pixels * groups), (const __half*)t->ptr, t->cstride / 2, codes, sf, pixels, (int)t->c, groups, q->cstride, q->sf_words, g, six_g);
     }
-    return check_launch(ctx, "ln_tensor_narrow_f4");
+    return check_launch(ctx, "ln_tensor_narrow_f4", e);
 }
+int widen_into(ln_ctx* ctx, const ln_tensor* t, ln_tensor* y) {
+    const int64_t pixels = t->n * t->h * t->w, hw = t->h * t->w;
+    const uint8_t *codes = (const uint8_t*)t->ptr, *sf = (const uint8_t*)t->sf;
+    const bool small = t->cstride * pixels < (1ll << 30);
+    cudaError_t e;
+    if (y->dtype == LN_F32) {
+        const int blocks = (int)((t->c + 15) / 16);
+        e = LN_F4_CALL(widen_f32_kernel, t->dtype, small, grid_for(ctx, (pixels + 7) / 8 * ((blocks + 3) / 4) * 32), codes, sf, (float*)y->ptr, pixels, hw, (int)t->c, blocks, t->cstride, t->sf_words, t->scale);
+    } else {
+        const int groups = (int)(y->cstride / 64);
+        e = LN_F4_CALL(widen_f16_kernel, t->dtype, small, grid_for(ctx, pixels * groups), codes, sf, (__half*)y->ptr, y->cstride / 2, pixels, (int)t->c, groups, t->cstride, t->sf_words, t->scale);
+    }
+    return check_launch(ctx, "ln_tensor_widen_f4", e);
+}
+#undef LN_F4_CALL
 
 }  // namespace
 
@@ -293,18 +376,7 @@ int32_t ln_tensor_widen_f4(ln_ctx* ctx, const ln_tensor* t, int32_t dtype, ln_te
         ln_tensor* y = nullptr;
         int rc = new_tensor(ctx, dtype, t->n, t->c, t->h, t->w, &y);
         if (rc) return rc;
-        const int64_t pixels = t->n * t->h * t->w, hw = t->h * t->w;
-        const uint8_t *codes = (const uint8_t*)t->ptr, *sf = (const uint8_t*)t->sf;
-        if (dtype == LN_F32) {
-            const int blocks = (int)((t->c + 15) / 16), grid = grid_for(ctx, pixels * blocks);
-            if (t->dtype == LN_F4) widen_f32_kernel<LN_F4><<<grid, kThreads, 0, ctx->stream>>>(codes, sf, (float*)y->ptr, pixels, hw, (int)t->c, blocks, t->cstride, t->sf_words, t->scale);
-            else widen_f32_kernel<LN_MX4><<<grid, kThreads, 0, ctx->stream>>>(codes, sf, (float*)y->ptr, pixels, hw, (int)t->c, blocks, t->cstride, t->sf_words, 1.0f);
-        } else {
-            const int blocks = (int)(y->cstride / 32), grid = grid_for(ctx, pixels * blocks);
-            if (t->dtype == LN_F4) widen_f16_kernel<LN_F4><<<grid, kThreads, 0, ctx->stream>>>(codes, sf, (__half*)y->ptr, y->cstride / 2, pixels, (int)t->c, blocks, t->cstride, t->sf_words, t->scale);
-            else widen_f16_kernel<LN_MX4><<<grid, kThreads, 0, ctx->stream>>>(codes, sf, (__half*)y->ptr, y->cstride / 2, pixels, (int)t->c, blocks, t->cstride, t->sf_words, 1.0f);
-        }
-        rc = check_launch(ctx, who);
+        rc = widen_into(ctx, t, y);
         if (rc) { ln_tensor_release(y); return rc; }
         *out = y;
         return LN_OK;
@@ -324,10 +396,9 @@ int32_t ln_tensor_download_f4(ln_ctx* ctx, const ln_tensor* t, uint8_t* host_cod
         cudaSetDevice(ctx->device);
         uint8_t* tmp = (uint8_t*)ln_pool_alloc(ctx, (size_t)(code_count + scales));
         if (!tmp) return LN_ERR_CUDA;
-        unpack_f4_kernel<<<grid_for(ctx, code_count + scales), kThreads, 0, ctx->stream>>>((const uint8_t*)t->ptr, (const uint8_t*)t->sf, tmp, tmp + code_count, t->n, hw, (int)t->c, sf_blocks,
+        cudaError_t e = ln_f4_launch(ctx, unpack_f4_kernel, grid_for(ctx, code_count + scales), kThreads, (const uint8_t*)t->ptr, (const uint8_t*)t->sf, tmp, tmp + code_count, t->n, hw, (int)t->c, sf_blocks,
                                                                                          t->cstride, t->sf_words);
-        int rc = check_launch(ctx, who);
-        cudaError_t e = cudaSuccess;
+        int rc = check_launch(ctx, who, e);
         if (rc == LN_OK) {
             e = cudaMemcpyAsync(host_codes, tmp, (size_t)code_count, cudaMemcpyDeviceToHost, ctx->stream);
             if (e == cudaSuccess) e = cudaMemcpyAsync(host_scales, tmp + code_count, (size_t)scales, cudaMemcpyDeviceToHost, ctx->stream);
@@ -363,12 +434,12 @@ int32_t ln_conv_weights_f4(ln_ctx* ctx, const ln_tensor* weights_f32, int64_t fi
         w->wscale = (float*)ln_pool_alloc(ctx, (size_t)filters * 4);
         if (!w->w || !w->sf || !w->wscale) { ln_conv_weights_release(w); return LN_ERR_CUDA; }
         int rc = LN_OK;
-        const cudaError_t e = cudaMemsetAsync(w->sf, 0, sf_bytes, ctx->stream);
+        cudaError_t e = cudaMemsetAsync(w->sf, 0, sf_bytes, ctx->stream);
         if (e != cudaSuccess) rc = ln_fail(ctx, LN_ERR_CUDA, "%s: %s", who, cudaGetErrorString(e));
         if (rc == LN_OK) {
-            if (dtype == LN_F4) pack_weights_f4_kernel<LN_F4><<<(int)filters, 256, 0, ctx->stream>>>((const float*)weights_f32->ptr, (int)channels, (int)k2, w->cpad, (uint8_t*)w->w, (uint8_t*)w->sf, w->wscale, sf_words);
-            else pack_weights_f4_kernel<LN_MX4><<<(int)filters, 256, 0, ctx->stream>>>((const float*)weights_f32->ptr, (int)channels, (int)k2, w->cpad, (uint8_t*)w->w, (uint8_t*)w->sf, w->wscale, sf_words);
-            rc = check_launch(ctx, who);
+            if (dtype == LN_F4) e = ln_f4_launch(ctx, pack_weights_f4_kernel<LN_F4>, (int)filters, 256, (const float*)weights_f32->ptr, (int)channels, (int)k2, w->cpad, (uint8_t*)w->w, (uint8_t*)w->sf, w->wscale, sf_words);
+            else e = ln_f4_launch(ctx, pack_weights_f4_kernel<LN_MX4>, (int)filters, 256, (const float*)weights_f32->ptr, (int)channels, (int)k2, w->cpad, (uint8_t*)w->w, (uint8_t*)w->sf, w->wscale, sf_words);
+            rc = check_launch(ctx, who, e);
         }
         if (rc) { ln_conv_weights_release(w); return rc; }
         *out = w;
@@ -428,14 +499,15 @@ int32_t ln_conv2d_bias_act_f4(ln_ctx* ctx, const ln_tensor* x, const ln_conv_wei
             p.OH = (int)oh; p.OW = (int)ow; p.blocks = (int)(x->cstride * 2 / ln_f4_block(x->dtype));
             p.act = activation; p.out_f16 = dst->dtype == LN_F16; p.xscale = x->scale;
             const int grid = grid_for(ctx, p.total);
+            cudaError_t e;
             if (x->dtype == LN_F4) {
-                if (ctx->exact_epilogue) conv_f4_simt_kernel<LN_F4, true><<<grid, kThreads, 0, ctx->stream>>>(p);
-                else conv_f4_simt_kernel<LN_F4, false><<<grid, kThreads, 0, ctx->stream>>>(p);
+                if (ctx->exact_epilogue) e = ln_f4_launch(ctx, conv_f4_simt_kernel<LN_F4, true>, grid, kThreads, p);
+                else e = ln_f4_launch(ctx, conv_f4_simt_kernel<LN_F4, false>, grid, kThreads, p);
             } else {
-                if (ctx->exact_epilogue) conv_f4_simt_kernel<LN_MX4, true><<<grid, kThreads, 0, ctx->stream>>>(p);
-                else conv_f4_simt_kernel<LN_MX4, false><<<grid, kThreads, 0, ctx->stream>>>(p);
+                if (ctx->exact_epilogue) e = ln_f4_launch(ctx, conv_f4_simt_kernel<LN_MX4, true>, grid, kThreads, p);
+                else e = ln_f4_launch(ctx, conv_f4_simt_kernel<LN_MX4, false>, grid, kThreads, p);
             }
-            rc = check_launch(ctx, who);
+            rc = check_launch(ctx, who, e);
             if (rc == LN_OK && wide) rc = narrow_into(ctx, wide, y);
         }
         if (wide) ln_tensor_release(wide);

@@ -36,6 +36,7 @@ constexpr uint32_t kScaleCols = 416, kScaleSet = 48, kScaleB = 16;  // TMEM colu
 constexpr uint32_t kBarBytesF4 = 512;
 constexpr uint32_t kTabBytesF4 = 16 * 256;  // {multiplier, bias} of the columns that a warp is at
 constexpr int kMaxSmemF4 = 227 * 1024;
+constexpr size_t kLeastSmemF4 = 118 * 1024;
 
 struct f4_params {
     CUtensorMap tmA[4], tmB, tmXS, tmWS;  // codes of pixels and filters; their scales as rows of 512 bytes
@@ -273,6 +274,7 @@ __global__ void __launch_bounds__(kThreadsF4, 1) f4_umma_kernel(const __grid_con
     __syncthreads();
     if (PAIR) pair_sync();  // the other CTA's barriers are there before anything signals them
     tc_fence_after();
+    ln_f4_after_predecessor();
     const uint32_t tmem_base = *tmem_slot;
     const int kblocks = p.R * p.S * p.cblocks, first_unit = (int)blockIdx.x / kCtas, step = (int)gridDim.x / kCtas;
     const bool overlap = p.bn == 256;
@@ -610,12 +612,14 @@ cudaError_t launch(ln_ctx* ctx, const f4_params& p, bool pair, int grid, size_t 
         cfg.blockDim = dim3(kThreadsF4);
         cfg.dynamicSmemBytes = smem;
         cfg.stream = ctx->stream;
-        cudaLaunchAttribute attr[1];
-        attr[0].id = cudaLaunchAttributeClusterDimension;
-        attr[0].val.clusterDim.x = pair ? 2 : 1;
-        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+        cudaLaunchAttribute attr[2];
+        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[0].val.programmaticStreamSerializationAllowed = 1;
+        attr[1].id = cudaLaunchAttributeClusterDimension;
+        attr[1].val.clusterDim.x = 2;
+        attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
         cfg.attrs = attr;
-        cfg.numAttrs = 1;
+        cfg.numAttrs = pair ? 2 : 1;
         return cudaLaunchKernelEx(&cfg, k, p);
     };
     if (pair) return go(f4_umma_kernel<FMT, OUT, 2, true>);
@@ -689,7 +693,10 @@ int ln_f4_umma_launch(ln_ctx* ctx, const ln_f4_conv& c) {
     p.stage_bytes = (uint32_t)ln_round_up(p.off_sfb + (uint32_t)(p.words * wblocks) * 512u, 1024);
     p.stages = (int)((kMaxSmemF4 - 1024 - kBarBytesF4 - kTabBytesF4) / p.stage_bytes);
     if (p.stages > kMaxStagesF4) p.stages = kMaxStagesF4;
-    const size_t smem = 1024 + (size_t)p.stages * p.stage_bytes + kBarBytesF4 + kTabBytesF4;
+    size_t smem = 1024 + (size_t)p.stages * p.stage_bytes + kBarBytesF4 + kTabBytesF4;
+    // One CTA per SM, whatever else runs: a CTA takes all of TMEM and waits while another one has it, and of two pairs on the same two SMs
+    // each could hold what the other waits for.  So none asks for less than half of an SM's shared memory.
+    if (smem < kLeastSmemF4) smem = kLeastSmemF4;
     p.xsf = (const uint8_t*)x.sf; p.wscale = c.w->wscale; p.bias = c.bias;
     p.y = y.ptr; p.ys = y.cstride; p.ysf = (uint8_t*)y.sf; p.ysf_words = y.sf_words;
     p.xscale = x.scale; p.g = y.scale; p.six_g = 6.0f * y.scale;
