@@ -438,19 +438,16 @@ __global__ void __launch_bounds__(kThreadsF4, 1) f4_umma_kernel(const __grid_con
             for (int i = 2; i < warp; ++i) advance();
             int stage = warp - 2;  // (fewer than stages)
             uint32_t phase = 0;
-            uint32_t now[4][4], next[4][4];
-            bool more = unit < p.num_units, ok = true;
-            if (more) fetch(now);
-            while (more && ok) {
-                for (int i = 0; i < kGatherWarps; ++i) advance();
-                more = unit < p.num_units;
-                if (more) fetch(next);
+            uint32_t v[4][4];
+            bool ok = true;
+            if (unit < p.num_units) fetch(v);
+            while (ok && unit < p.num_units) {
                 if (!(ok = warp_wait(empty_bar(stage), phase ^ 1u, abort_flag, p.status, LN_STATUS_PRODUCER_TIMEOUT))) break;
                 const uint32_t dst = smem_base + (uint32_t)stage * p.stage_bytes + p.off_sfa + 16u * lane;
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
                     if (j < p.words)
-                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + 512u * j), "r"(now[0][j]), "r"(now[1][j]), "r"(now[2][j]), "r"(now[3][j]) : "memory");
+                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + 512u * j), "r"(v[0][j]), "r"(v[1][j]), "r"(v[2][j]), "r"(v[3][j]) : "memory");
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) {
@@ -459,10 +456,9 @@ __global__ void __launch_bounds__(kThreadsF4, 1) f4_umma_kernel(const __grid_con
                 }
                 stage += kGatherWarps;
                 if (stage >= p.stages) { stage -= p.stages; phase ^= 1u; }
-#pragma unroll
-                for (int g = 0; g < 4; ++g)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) now[g][j] = next[g][j];
+                // (behind the fence, which would wait for the reads; the other warps' k-blocks cover their latency)
+                for (int i = 0; i < kGatherWarps; ++i) advance();
+                if (unit < p.num_units) fetch(v);
             }
         }
     } else if (warp >= kFirstEpilogueWarp) {
