@@ -190,12 +190,13 @@ __device__ __forceinline__ void act2(float& v0, float& v1) {
         else { v0 = v0 == v0 ? r0 : v0; v1 = v1 == v1 ? r1 : v1; }  // (max drops a NaN)
     }
 }
-__device__ __forceinline__ void act_all(int act, bool exact, float (&v)[32]) {
+template <int W>
+__device__ __forceinline__ void act_all(int act, bool exact, float (&v)[W]) {
 #define LN_ALL(A)                                                                          \
-    _Pragma("unroll") for (int i = 0; i < 32; ++i) v[i] = ln_epilogue_act<true>(A, v[i]);  \
+    _Pragma("unroll") for (int i = 0; i < W; ++i) v[i] = ln_epilogue_act<true>(A, v[i]);   \
     break;
 #define LN_FAST(A)                                                                         \
-    _Pragma("unroll") for (int i = 0; i < 32; i += 2) act2<A>(v[i], v[i + 1]);             \
+    _Pragma("unroll") for (int i = 0; i < W; i += 2) act2<A>(v[i], v[i + 1]);              \
     break;
     switch (act) {
         case LN_ACT_LEAKY: LN_ALL(LN_ACT_LEAKY)
@@ -214,6 +215,8 @@ __device__ __forceinline__ void act_all(int act, bool exact, float (&v)[32]) {
 #undef LN_ALL
 #undef LN_FAST
 }
+__device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[16]) { tmem_ld_32x16(taddr, r); tmem_ld_wait(); }
+__device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[32]) { tmem_ld_32x32(taddr, r); tmem_ld_wait(); }
 __device__ __forceinline__ void store_32(uint8_t* dst, const uint32_t (&v)[8]) {  // a whole sector
     asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
 }
@@ -465,6 +468,7 @@ __global__ void __launch_bounds__(kThreadsF4, 1) f4_umma_kernel(const __grid_con
         // ------------------------------------------------------------------ epilogue
         // Group g takes the units with number % 4 == g.  (nbuf * subs >= 4: a group that waits for a tile's accumulator has finished a unit
         // of the tile nbuf before it or a later one, so the parity is unambiguous.)
+        constexpr int W = OUT == LN_OUT_Q && FMT == LN_MX4 ? 32 : 16;  // columns at a time (a block of a 4-bit output)
         const int quad = warp & 3, group = (warp - kFirstEpilogueWarp) >> 2;
         const int row = quad * 32 + lane, pw = row & (p.TW - 1), ph = (row >> p.log_tw) & (p.TH - 1), pn = row >> (p.log_tw + p.log_th);
         const uint32_t tab = tab_base + (uint32_t)(warp - kFirstEpilogueWarp) * 256u;
@@ -510,65 +514,64 @@ __global__ void __launch_bounds__(kThreadsF4, 1) f4_umma_kernel(const __grid_con
             if (!(ok = warp_wait(tfull_bar(this_buf), this_phase, abort_flag, p.status, LN_STATUS_EPILOGUE_TIMEOUT))) break;
             tc_fence_after();
             const uint32_t taddr = tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(this_buf * p.acc_step + sub * CH);
-            uint32_t acc[32];
-            tmem_ld_32x32(taddr, acc);
-            tmem_ld_wait();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) {
-                if (PAIR) {
-                    arrive_first<false>(tempty_bar(this_buf));
-                    if (overlap && first) arrive_first<false>(early_bar(this_buf));
-                } else {
-                    mbar_arrive(tempty_bar(this_buf));
-                    if (overlap && first) mbar_arrive(early_bar(this_buf));
+            // A loop, not unrolled: 32 columns in one piece are more code than the instruction caches of four warps at different places of
+            // it keep, and the epilogue then waited for instructions most of the time.
+#pragma unroll 1
+            for (int c0 = 0; c0 < CH; c0 += W) {
+                uint32_t acc[W];
+                tmem_ld(taddr + c0, acc);
+                if (c0 + W == CH) {
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) {
+                        if (PAIR) {
+                            arrive_first<false>(tempty_bar(this_buf));
+                            if (overlap && first) arrive_first<false>(early_bar(this_buf));
+                        } else {
+                            mbar_arrive(tempty_bar(this_buf));
+                            if (overlap && first) mbar_arrive(early_bar(this_buf));
+                        }
+                    }
+                    __syncwarp();
                 }
-            }
-            // (binary16 channels are padded to 32, 4-bit ones to 64: what is behind them is not stored)
-            if (f0 >= (OUT == LN_OUT_Q ? (p.F + 63) & ~63 : p.F)) continue;
-            float v[32];
+                const int f = f0 + c0;
+                // (binary16 channels are padded to 32, 4-bit ones to 64: what is behind them is not stored)
+                if (f0 >= (OUT == LN_OUT_Q ? (p.F + 63) & ~63 : p.F)) continue;
+                float v[W];
 #pragma unroll
-            for (int i = 0; i < 32; i += 2) {
-                float4 e;  // (volatile: the table is another one for every unit)
-                asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(e.x), "=f"(e.y), "=f"(e.z), "=f"(e.w) : "r"(tab + 8u * i));
-                ffma2(v[i], v[i + 1], __uint_as_float(acc[i]), __uint_as_float(acc[i + 1]), e.x, e.y, e.z, e.w);
-            }
-            act_all(p.act, p.exact != 0, v);
-            if (f0 + 32 > p.F) {
+                for (int i = 0; i < W; i += 2) {
+                    float4 e;  // (volatile: the table is another one for every unit)
+                    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(e.x), "=f"(e.y), "=f"(e.z), "=f"(e.w) : "r"(tab + 8u * (c0 + i)));
+                    ffma2(v[i], v[i + 1], __uint_as_float(acc[i]), __uint_as_float(acc[i + 1]), e.x, e.y, e.z, e.w);
+                }
+                act_all<W>(p.act, p.exact != 0, v);
+                if (f + W > p.F) {
 #pragma unroll
-                for (int i = 0; i < 32; ++i)
-                    if (f0 + i >= p.F) v[i] = 0.0f;
-            }
-            if (OUT == LN_OUT_F32) {
-                if (valid) {
+                    for (int i = 0; i < W; ++i)
+                        if (f + i >= p.F) v[i] = 0.0f;
+                }
+                if (!valid) continue;
+                if (OUT == LN_OUT_F32) {
                     const int img = pix / p.hw;
-                    float* dst = (float*)p.y + ((long long)img * p.F + f0) * p.hw + (pix - img * p.hw);
+                    float* dst = (float*)p.y + ((long long)img * p.F + f) * p.hw + (pix - img * p.hw);
 #pragma unroll
-                    for (int i = 0; i < 32; ++i)
-                        if (f0 + i < p.F) dst[(long long)i * p.hw] = v[i];
-                }
-            } else if (OUT == LN_OUT_F16) {
-                uint32_t h[2][8];
+                    for (int i = 0; i < W; ++i)
+                        if (f + i < p.F) dst[(long long)i * p.hw] = v[i];
+                } else if (OUT == LN_OUT_F16) {
+                    uint32_t h[8];
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const __half2 q = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
-                    h[i >> 3][i & 7] = *reinterpret_cast<const uint32_t*>(&q);
-                }
-                if (valid) {
-                    uint8_t* dst = (uint8_t*)p.y + (long long)pix * p.ys + 2 * f0;
-                    store_32(dst, h[0]);
-                    store_32(dst + 32, h[1]);
-                }
-            } else {
-                constexpr int B = FMT == LN_F4 ? 16 : 32;
-                uint32_t q[4], sf = 0;
-#pragma unroll
-                for (int b = 0; b < 32 / B; ++b) sf |= ln_f4_quantise<FMT>(v + b * B, p.g, p.six_g, q + b * B / 8) << (8 * b);
-                if (valid) {
-                    *(uint4*)((uint8_t*)p.y + (long long)pix * p.ys + f0 / 2) = make_uint4(q[0], q[1], q[2], q[3]);
-                    uint8_t* at_sf = p.ysf + ln_f4_sf_at(pix, f0 / (4 * B), p.ysf_words) + f0 / B % 4;
-                    if (FMT == LN_F4) *(uint16_t*)at_sf = (uint16_t)sf;
-                    else *at_sf = (uint8_t)sf;
+                    for (int i = 0; i < 8; ++i) {
+                        const __half2 q = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+                        h[i] = *reinterpret_cast<const uint32_t*>(&q);
+                    }
+                    store_32((uint8_t*)p.y + (long long)pix * p.ys + 2 * f, h);
+                } else {
+                    uint32_t q[W / 8];
+                    const uint32_t sf = ln_f4_quantise<FMT>(v, p.g, p.six_g, q);
+                    uint8_t* dst = (uint8_t*)p.y + (long long)pix * p.ys + f / 2;
+                    if (W == 16) *(uint2*)dst = make_uint2(q[0], q[1]);
+                    else *(uint4*)dst = make_uint4(q[0], q[1], q[W / 8 - 2], q[W / 8 - 1]);
+                    p.ysf[ln_f4_sf_at(pix, f / (4 * W), p.ysf_words) + f / W % 4] = (uint8_t)sf;
                 }
             }
         }
