@@ -89,10 +89,10 @@ int32_t ln_tensor_zeros_f32(ln_ctx* ctx, const int64_t shape[4], ln_tensor** out
 int32_t ln_tensor_download_f32(ln_ctx* ctx, const ln_tensor* t, float* host, int64_t count);
 int32_t ln_tensor_shape(const ln_tensor* t, int64_t shape[4]);
 int32_t ln_tensor_dtype(const ln_tensor* t);
-/* Device address of an f32 or binary16 tensor's first value, and the distance in values between neighbours along each axis, for a
+/* Device address of an f32 or binary16 tensor's first value, its shape and the distance in values between neighbours along each axis, for a
    program that hands the tensor to another library on the same GPU.  The handle keeps the memory; work on another stream has to be
    ordered behind the ctx stream (ln_ctx_stream) by the caller, and in front of it again before the handle is released. */
-int32_t ln_tensor_device_data(const ln_tensor* t, void** data, int64_t strides[4]);
+int32_t ln_tensor_device_data(const ln_tensor* t, void** data, int64_t shape[4], int64_t strides[4]);
 int32_t ln_tensor_retain(ln_tensor* t);
 int32_t ln_tensor_release(ln_tensor* t);
 

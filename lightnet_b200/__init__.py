@@ -85,7 +85,7 @@ SYMBOLS = {
     "ln_tensor_download_f32": (C.c_int32, [_VP, _VP, _VP, C.c_int64]),
     "ln_tensor_shape": (C.c_int32, [_VP, _I64P]),
     "ln_tensor_dtype": (C.c_int32, [_VP]),
-    "ln_tensor_device_data": (C.c_int32, [_VP, _PP, _I64P]),
+    "ln_tensor_device_data": (C.c_int32, [_VP, _PP, _I64P, _I64P]),
     "ln_tensor_retain": (C.c_int32, [_VP]),
     "ln_tensor_release": (C.c_int32, [_VP]),
     "ln_conv2d_f32": (C.c_int32, [_VP, _VP, _VP, _I64P] + [C.c_int64] * 10 + [_PP]),
@@ -243,15 +243,17 @@ class Tensor:
         shares the memory and keeps the handle); order their work behind the backend's stream.  Made when it is first asked for."""
         if name != "__cuda_array_interface__":
             raise AttributeError(name)
-        dtype = self.dtype
-        if dtype not in (LN_F32, LN_F16):
+        dtype = _lib.ln_tensor_dtype(self.h)
+        if dtype != LN_F32 and dtype != LN_F16:
             raise AttributeError("only f32 and binary16 tensors have an array interface")
-        size, p, s = 4 if dtype == LN_F32 else 2, C.c_void_p(), _I64x4()
-        self.backend._check(_lib.ln_tensor_device_data(self.h, C.byref(p), s))
+        backend, size, p, shape, s = self.backend, 4 if dtype == LN_F32 else 2, C.c_void_p(), _I64x4(), _I64x4()
+        rc = _lib.ln_tensor_device_data(self.h, p, shape, s)
+        if rc:
+            backend._check(rc)
         n, c, h, w = s
         self.__cuda_array_interface__ = d = {
-            "shape": self.shape, "typestr": "<f4" if size == 4 else "<f2", "data": (p.value, False), "strides": (size * n, size * c, size * h, size * w),
-            "version": 3, "stream": self.backend.stream}
+            "shape": tuple(shape), "typestr": "<f4" if size == 4 else "<f2", "data": (p.value, False), "strides": (size * n, size * c, size * h, size * w),
+            "version": 3, "stream": backend.stream}
         return d
 
 

@@ -159,10 +159,11 @@ struct ln_f4_conv {  // one convolution: operands, geometry, output
 };
 // launches a 4-bit kernel (all begin with ln_f4_after_predecessor) on the ctx stream
 template <typename... P, typename... A>
-inline cudaError_t ln_f4_launch(ln_ctx* ctx, void (*kernel)(P...), int grid, int threads, A... args) {
+inline cudaError_t ln_f4_launch(ln_ctx* ctx, void (*kernel)(P...), int grid, int threads, size_t smem, const A&... args) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)grid);
     cfg.blockDim = dim3((unsigned)threads);
+    cfg.dynamicSmemBytes = smem;
     cfg.stream = ctx->stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

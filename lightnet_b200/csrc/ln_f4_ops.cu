@@ -306,8 +306,8 @@ __global__ void conv_f4_simt_kernel(const simt_params p) {
 
 // one launch with 32-bit indexes where every index, and the step behind the last one, stays below 2^31
 #define LN_F4_CALL(KERNEL, FMT, SMALL, GRID, ...) \
-    ((FMT) == LN_F4 ? ((SMALL) ? ln_f4_launch(ctx, KERNEL<LN_F4, uint32_t>, GRID, kThreads, __VA_ARGS__) : ln_f4_launch(ctx, KERNEL<LN_F4, int64_t>, GRID, kThreads, __VA_ARGS__)) \
-                    : ((SMALL) ? ln_f4_launch(ctx, KERNEL<LN_MX4, uint32_t>, GRID, kThreads, __VA_ARGS__) : ln_f4_launch(ctx, KERNEL<LN_MX4, int64_t>, GRID, kThreads, __VA_ARGS__)))
+    ((FMT) == LN_F4 ? ((SMALL) ? ln_f4_launch(ctx, KERNEL<LN_F4, uint32_t>, GRID, kThreads, 0, __VA_ARGS__) : ln_f4_launch(ctx, KERNEL<LN_F4, int64_t>, GRID, kThreads, 0, __VA_ARGS__)) \
+                    : ((SMALL) ? ln_f4_launch(ctx, KERNEL<LN_MX4, uint32_t>, GRID, kThreads, 0, __VA_ARGS__) : ln_f4_launch(ctx, KERNEL<LN_MX4, int64_t>, GRID, kThreads, 0, __VA_ARGS__)))
 
 int narrow_into(ln_ctx* ctx, const ln_tensor* t, ln_tensor* q) {
     const int64_t pixels = t->n * t->h * t->w, hw = t->h * t->w;
@@ -396,7 +396,7 @@ int32_t ln_tensor_download_f4(ln_ctx* ctx, const ln_tensor* t, uint8_t* host_cod
         cudaSetDevice(ctx->device);
         uint8_t* tmp = (uint8_t*)ln_pool_alloc(ctx, (size_t)(code_count + scales));
         if (!tmp) return LN_ERR_CUDA;
-        cudaError_t e = ln_f4_launch(ctx, unpack_f4_kernel, grid_for(ctx, code_count + scales), kThreads, (const uint8_t*)t->ptr, (const uint8_t*)t->sf, tmp, tmp + code_count, t->n, hw, (int)t->c, sf_blocks,
+        cudaError_t e = ln_f4_launch(ctx, unpack_f4_kernel, grid_for(ctx, code_count + scales), kThreads, 0, (const uint8_t*)t->ptr, (const uint8_t*)t->sf, tmp, tmp + code_count, t->n, hw, (int)t->c, sf_blocks,
                                                                                          t->cstride, t->sf_words);
         int rc = check_launch(ctx, who, e);
         if (rc == LN_OK) {
@@ -437,8 +437,8 @@ int32_t ln_conv_weights_f4(ln_ctx* ctx, const ln_tensor* weights_f32, int64_t fi
         cudaError_t e = cudaMemsetAsync(w->sf, 0, sf_bytes, ctx->stream);
         if (e != cudaSuccess) rc = ln_fail(ctx, LN_ERR_CUDA, "%s: %s", who, cudaGetErrorString(e));
         if (rc == LN_OK) {
-            if (dtype == LN_F4) e = ln_f4_launch(ctx, pack_weights_f4_kernel<LN_F4>, (int)filters, 256, (const float*)weights_f32->ptr, (int)channels, (int)k2, w->cpad, (uint8_t*)w->w, (uint8_t*)w->sf, w->wscale, sf_words);
-            else e = ln_f4_launch(ctx, pack_weights_f4_kernel<LN_MX4>, (int)filters, 256, (const float*)weights_f32->ptr, (int)channels, (int)k2, w->cpad, (uint8_t*)w->w, (uint8_t*)w->sf, w->wscale, sf_words);
+            if (dtype == LN_F4) e = ln_f4_launch(ctx, pack_weights_f4_kernel<LN_F4>, (int)filters, 256, 0, (const float*)weights_f32->ptr, (int)channels, (int)k2, w->cpad, (uint8_t*)w->w, (uint8_t*)w->sf, w->wscale, sf_words);
+            else e = ln_f4_launch(ctx, pack_weights_f4_kernel<LN_MX4>, (int)filters, 256, 0, (const float*)weights_f32->ptr, (int)channels, (int)k2, w->cpad, (uint8_t*)w->w, (uint8_t*)w->sf, w->wscale, sf_words);
             rc = check_launch(ctx, who, e);
         }
         if (rc) { ln_conv_weights_release(w); return rc; }
@@ -501,11 +501,11 @@ int32_t ln_conv2d_bias_act_f4(ln_ctx* ctx, const ln_tensor* x, const ln_conv_wei
             const int grid = grid_for(ctx, p.total);
             cudaError_t e;
             if (x->dtype == LN_F4) {
-                if (ctx->exact_epilogue) e = ln_f4_launch(ctx, conv_f4_simt_kernel<LN_F4, true>, grid, kThreads, p);
-                else e = ln_f4_launch(ctx, conv_f4_simt_kernel<LN_F4, false>, grid, kThreads, p);
+                if (ctx->exact_epilogue) e = ln_f4_launch(ctx, conv_f4_simt_kernel<LN_F4, true>, grid, kThreads, 0, p);
+                else e = ln_f4_launch(ctx, conv_f4_simt_kernel<LN_F4, false>, grid, kThreads, 0, p);
             } else {
-                if (ctx->exact_epilogue) e = ln_f4_launch(ctx, conv_f4_simt_kernel<LN_MX4, true>, grid, kThreads, p);
-                else e = ln_f4_launch(ctx, conv_f4_simt_kernel<LN_MX4, false>, grid, kThreads, p);
+                if (ctx->exact_epilogue) e = ln_f4_launch(ctx, conv_f4_simt_kernel<LN_MX4, true>, grid, kThreads, 0, p);
+                else e = ln_f4_launch(ctx, conv_f4_simt_kernel<LN_MX4, false>, grid, kThreads, 0, p);
             }
             rc = check_launch(ctx, who, e);
             if (rc == LN_OK && wide) rc = narrow_into(ctx, wide, y);

@@ -12,14 +12,12 @@
 //
 // Roles: warps 0 and 6 load (pixels; weights), warp 1 issues, warps 2 to 5 gather scales (every fourth k-block each; the ring has at
 // least four stages, so none comes back to a stage whose use before is still to be filled), warps 8 to 23 are the epilogue: four groups
-// of four that take the units of 32 columns of the tiles in turn.  TMEM: 416 columns of accumulators, 2 x 48 of scales.  Two tiles of
-// 192 filters, three of 128 or six of 64 fit; two of 256 overlap by 96 columns (0..255 and 160..415), so their epilogue reads the four
-// units that hold the overlap first and the next tile starts as soon as those are in registers.
-//
-// CTA pairs (PAIR: clusters of two CTAs on neighbouring SMs, cta_group::2): both multiply their own 128 pixels by the same filters, each
-// loads half of the filters' codes, and one instruction of the first CTA's issuing thread works in both (M = 256).  What bounds a large
-// product is the way from L2 to shared memory, about 60 bytes a cycle and SM: a k-block of 256 filters is 54 KB for 528 cycles of
-// tensor work alone and 38 KB in a pair.  The loads of both CTAs signal the first one's barriers, commits arrive in both.
+// of four that take the units of 32 columns of the tiles in turn.  TMEM: 416 columns of accumulators, 2 x 48 of scales.  Three tiles of
+// 128 filters or six of 64 fit; two of 256 overlap by 96 columns (0..255 and 160..415), so their epilogue reads the four units that hold
+// the overlap first, and the next tile starts when those have been read.
+// What bounds it: large k ranges the way from L2 to shared memory (54 KB per k-block of 256 filters at 64 bytes a cycle are 844 cycles, the
+// instructions take 528; measured 830), short ones the epilogue.  CTA pairs (cta_group::2, half of the filters' codes per CTA) were built and
+// gave the same 64 us on 8192 x 4096 x 4096: a tcgen05.cp of a pair takes its thread 50 cycles and more, and twelve go with four instructions.
 // Every wait is bounded (see ln_umma.h).
 #include <cstdlib>
 
@@ -50,7 +48,7 @@ struct f4_params {
     int sf_words, cstride;
     int bk, bn, cblocks, words;
     int R, S, stride, pad, H, W, N, OH, OW, F, hw;
-    int TW, TH, TN, log_tw, log_th, tiles_f, tiles_w, tiles_h, num_units;  // units: pixel tiles (pairs of them) x filter tiles
+    int TW, TH, TN, log_tw, log_th, tiles_f, tiles_w, tiles_h, num_units;  // units: pixel tiles x filter tiles
     unsigned long long magic_f, magic_w, magic_h;
     int stages, nbuf, acc_step, subs, act, exact, flat;
     uint32_t off_b, off_sfa, off_sfb, stage_bytes;
@@ -65,91 +63,23 @@ __device__ __forceinline__ bool elect_one() {
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status, int code) {
     return __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity, abort_flag, status, code));
 }
-// The CTAs of a pair: rank, the first CTA's copy of a shared address, arrival on its barriers, rendezvous.
-__device__ __forceinline__ uint32_t pair_rank() {
-    uint32_t r;
-    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-    return r;
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(c2) : "memory");
 }
-__device__ __forceinline__ uint32_t in_first(uint32_t addr) {
-    uint32_t r;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(addr));
-    return r;
-}
-template <bool RELEASE>
-__device__ __forceinline__ void arrive_first(uint32_t bar) {
-    // (the epilogue hands tensor memory back, which its fence orders; a release would wait for its global stores)
-    if (RELEASE) asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(in_first(bar)) : "memory");
-    else asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(in_first(bar)) : "memory");
-}
-__device__ __forceinline__ void pair_sync() {
-    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-// The issuing thread's wait for gathered scales: in a pair also for those that the other CTA stored before it arrived.
-__device__ __forceinline__ bool mbar_wait_pair(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status) {
-    for (uint32_t it = 0; it < kWaitLimit; ++it) {
-        uint32_t there;
-        asm volatile(
-            "{\n\t.reg .pred p;\n\t"
-            "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n\t"
-            "selp.u32 %0, 1, 0, p;\n\t}"
-            : "=r"(there)
-            : "r"(bar), "r"(parity), "r"(kWaitHintNs)
-            : "memory");
-        if (there) return true;
-        if ((it & 255u) == 255u && *abort_flag) return false;
-    }
-    *abort_flag = 1;
-    *(volatile int*)status = LN_STATUS_MMA_TIMEOUT;
-    __threadfence_system();
-    return false;
-}
-// Loads; in a pair they signal the first CTA's barrier (`bar` is its address there).
-template <bool PAIR>
-__device__ __forceinline__ void load_4d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, int c3, uint32_t bar) {
-    if (!PAIR) { tma_load_4d(dst, map, c0, c1, c2, c3, bar); return; }
-    asm volatile("cp.async.bulk.tensor.4d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(c2),
-                 "r"(c3)
-                 : "memory");
-}
-template <bool PAIR>
-__device__ __forceinline__ void load_3d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, uint32_t bar) {
-    if (PAIR) asm volatile("cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(c2) : "memory");
-    else asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(c2) : "memory");
-}
-template <bool PAIR>
-__device__ __forceinline__ void load_2d(uint32_t dst, const CUtensorMap* map, int c0, int c1, uint32_t bar) {
-    if (!PAIR) { tma_load_2d(dst, map, c0, c1, bar); return; }
-    asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(c1) : "memory");
-}
-// arrives, in both CTAs of a pair, once everything issued so far has finished
-template <bool PAIR>
-__device__ __forceinline__ void commit(uint32_t bar) {
-    if (PAIR) asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((uint16_t)3) : "memory");
-    else tc_commit(bar);
-}
-// 32 rows of 16 bytes -> the four 32-lane quarters of TMEM, four columns (each CTA of a pair from its own shared memory)
-template <bool PAIR>
+// 32 rows of 16 bytes -> the four 32-lane quarters of TMEM, four columns
 __device__ __forceinline__ void tc_copy_scales(uint32_t taddr, uint64_t desc) {
-    if (PAIR) asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
-    else asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
 }
-template <int FMT, bool PAIR>
+template <int FMT>
 __device__ __forceinline__ void tc_mma_scaled(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
-#define LN_MMA(GROUP, KIND)                                                                                                  \
+#define LN_MMA(KIND)                                                                                                         \
     asm volatile(                                                                                                            \
         "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"                                                                    \
-        "tcgen05.mma.cta_group::" GROUP ".kind::" KIND " [%0], %1, %2, %3, [%5], [%6], p;\n\t}" ::"r"(d),                    \
+        "tcgen05.mma.cta_group::1.kind::" KIND " [%0], %1, %2, %3, [%5], [%6], p;\n\t}" ::"r"(d),                            \
         "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(sfa), "r"(sfb)                                                      \
         : "memory")
-    if (FMT == LN_F4) {
-        if (PAIR) LN_MMA("2", "mxf4nvf4.block_scale.scale_vec::4X");
-        else LN_MMA("1", "mxf4nvf4.block_scale.scale_vec::4X");
-    } else {
-        if (PAIR) LN_MMA("2", "mxf4.block_scale.scale_vec::2X");
-        else LN_MMA("1", "mxf4.block_scale.scale_vec::2X");
-    }
+    if (FMT == LN_F4) LN_MMA("mxf4nvf4.block_scale.scale_vec::4X");
+    else LN_MMA("mxf4.block_scale.scale_vec::2X");
 #undef LN_MMA
 }
 // descriptor of 32 rows of 16 bytes (no swizzle, groups of 8 rows 128 bytes apart)
@@ -220,20 +150,19 @@ __device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[32]) { tme
 __device__ __forceinline__ void store_32(uint8_t* dst, const uint32_t (&v)[8]) {  // a whole sector
     asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
 }
-// the place of work unit `unit`: output box origin and first filter.  The CTAs of a pair take two consecutive pixel tiles (the second may
-// lie behind the last: everything there is out of range).
+// the place of a tile: output box origin and first filter
 struct f4_tile {
     int ow0, oh0, n0, f0;
 };
-template <bool PAIR>
-__device__ __forceinline__ f4_tile tile_at(const f4_params& p, int unit, int rank) {
-    const int u1 = fast_div(unit, p.magic_f), tf = unit - u1 * p.tiles_f, q1 = PAIR ? 2 * u1 + rank : u1;
+__device__ __forceinline__ f4_tile tile_at(const f4_params& p, int unit) {
+    const int q1 = fast_div(unit, p.magic_f), tf = unit - q1 * p.tiles_f;
     const int q2 = fast_div(q1, p.magic_w), tw = q1 - q2 * p.tiles_w;
     const int tn = fast_div(q2, p.magic_h), th = q2 - tn * p.tiles_h;
     return {tw * p.TW, th * p.TH, tn * p.TN, tf * p.bn};
 }
 
-template <int FMT, int OUT, int WBLOCKS, bool PAIR>
+// WBLOCKS: groups of 128 filters that a tile's scales are in
+template <int FMT, int OUT, int WBLOCKS>
 __global__ void __launch_bounds__(kThreadsF4, 1) f4_umma_kernel(const __grid_constant__ f4_params p) {
     extern __shared__ uint8_t smem_raw[];
     const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -247,51 +176,42 @@ __global__ void __launch_bounds__(kThreadsF4, 1) f4_umma_kernel(const __grid_con
     volatile int* abort_flag = (volatile int*)(tmem_slot + 2);
     const uint32_t tab_base = bar_base + kBarBytesF4;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int rank = PAIR ? (int)pair_rank() : 0;
-    constexpr int kCtas = PAIR ? 2 : 1;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < p.stages; ++s) {
-            mbar_init(full_bar(s), p.flat ? 2 : 2 + kCtas);  // the two loaders (with the copies' bytes) and the warps that gather scales
+            mbar_init(full_bar(s), p.flat ? 2 : 3);  // the two loaders (with the copies' bytes) and the warps that gather scales
             mbar_init(empty_bar(s), 1);
         }
         for (int b = 0; b < p.nbuf; ++b) {
             mbar_init(tfull_bar(b), 1);
-            mbar_init(tempty_bar(b), 4 * p.subs * kCtas);
+            mbar_init(tempty_bar(b), 4 * p.subs);
         }
-        mbar_init(early_bar(0), 16 * kCtas);
-        mbar_init(early_bar(1), 16 * kCtas);
+        mbar_init(early_bar(0), 16);
+        mbar_init(early_bar(1), 16);
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) {
-        if (PAIR) {
-            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32((const void*)tmem_slot)), "r"(512u) : "memory");
-            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
-        } else {
-            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32((const void*)tmem_slot)), "r"(512u) : "memory");
-            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-        }
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32((const void*)tmem_slot)), "r"(512u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     tc_fence_before();
     __syncthreads();
-    if (PAIR) pair_sync();  // the other CTA's barriers are there before anything signals them
     tc_fence_after();
     ln_f4_after_predecessor();
     const uint32_t tmem_base = *tmem_slot;
-    const int kblocks = p.R * p.S * p.cblocks, first_unit = (int)blockIdx.x / kCtas, step = (int)gridDim.x / kCtas;
-    const bool overlap = p.bn == 256;
+    const int kblocks = p.R * p.S * p.cblocks, first_unit = (int)blockIdx.x, step = (int)gridDim.x;
+    constexpr bool overlap = WBLOCKS == 2;
 
     if (warp == 0) {
         // ------------------------------------------------------------------ loads of the pixels
         if (elect_one()) {
             const uint32_t bytes = 128u * p.bk + (p.flat ? (uint32_t)p.words * 512u : 0u);
-            const uint32_t first_full = PAIR ? in_first(full_bar(0)) : full_bar(0);
             int stage = 0;
             uint32_t phase = 0;
             bool ok = true;
             for (int unit = first_unit; ok && unit < p.num_units; unit += step) {
-                const f4_tile t = tile_at<PAIR>(p, unit, rank);
+                const f4_tile t = tile_at(p, unit);
                 int sf_row = (t.ow0 >> 7) * kblocks * p.words;  // (flat)
                 for (int r = 0; ok && r < p.R; ++r)
                     for (int s = 0; ok && s < p.S; ++s) {
@@ -304,10 +224,10 @@ __global__ void __launch_bounds__(kThreadsF4, 1) f4_umma_kernel(const __grid_con
                         }
                         for (int c0 = 0; c0 < p.cstride; c0 += p.bk, sf_row += p.words) {
                             if (!(ok = mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag, p.status, LN_STATUS_PRODUCER_TIMEOUT))) break;
-                            const uint32_t at = smem_base + (uint32_t)stage * p.stage_bytes, bar = first_full + 8u * stage;
-                            if (rank == 0) mbar_arrive_expect_tx(full_bar(stage), kCtas * bytes);
-                            load_4d<PAIR>(at, &p.tmA[map], c0, t.ow0 + tx, t.oh0 + ty, t.n0, bar);
-                            if (p.flat) load_2d<PAIR>(at + p.off_sfa, &p.tmXS, 0, sf_row, bar);
+                            const uint32_t at = smem_base + (uint32_t)stage * p.stage_bytes, bar = full_bar(stage);
+                            mbar_arrive_expect_tx(bar, bytes);
+                            tma_load_4d(at, &p.tmA[map], c0, t.ow0 + tx, t.oh0 + ty, t.n0, bar);
+                            if (p.flat) tma_load_2d(at + p.off_sfa, &p.tmXS, 0, sf_row, bar);
                             if (++stage == p.stages) { stage = 0; phase ^= 1u; }
                         }
                     }
@@ -315,11 +235,9 @@ __global__ void __launch_bounds__(kThreadsF4, 1) f4_umma_kernel(const __grid_con
         }
         __syncwarp();
     } else if (warp == 6) {
-        // ------------------------------------------------------------------ loads of the weights (a CTA of a pair: of its half of the codes, and all scales)
+        // ------------------------------------------------------------------ loads of the weights
         if (elect_one()) {
-            const int rows = p.bn / kCtas;
-            const uint32_t bytes = (uint32_t)rows * p.bk + WBLOCKS * (uint32_t)p.words * 512u;
-            const uint32_t first_full = PAIR ? in_first(full_bar(0)) : full_bar(0);
+            const uint32_t bytes = (uint32_t)p.bn * p.bk + WBLOCKS * (uint32_t)p.words * 512u;
             int stage = 0;
             uint32_t phase = 0;
             bool ok = true;
@@ -328,10 +246,10 @@ __global__ void __launch_bounds__(kThreadsF4, 1) f4_umma_kernel(const __grid_con
                 int col = 0, c0 = 0;  // first byte of the tap, of the k-block inside it
                 for (int kb = 0; kb < kblocks; ++kb) {
                     if (!(ok = mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag, p.status, LN_STATUS_PRODUCER_TIMEOUT))) break;
-                    const uint32_t at = smem_base + (uint32_t)stage * p.stage_bytes, bar = first_full + 8u * stage;
-                    if (rank == 0) mbar_arrive_expect_tx(full_bar(stage), kCtas * bytes);
-                    load_2d<PAIR>(at + p.off_b, &p.tmB, col + c0, f0 + rank * rows, bar);
-                    load_3d<PAIR>(at + p.off_sfb, &p.tmWS, 0, kb * p.words, f0 >> 7, bar);
+                    const uint32_t at = smem_base + (uint32_t)stage * p.stage_bytes, bar = full_bar(stage);
+                    mbar_arrive_expect_tx(bar, bytes);
+                    tma_load_2d(at + p.off_b, &p.tmB, col + c0, f0, bar);
+                    tma_load_3d(at + p.off_sfb, &p.tmWS, 0, kb * p.words, f0 >> 7, bar);
                     c0 += p.bk;
                     if (c0 >= p.cstride) { c0 = 0; col += p.cstride; }
                     if (++stage == p.stages) { stage = 0; phase ^= 1u; }
@@ -341,9 +259,9 @@ __global__ void __launch_bounds__(kThreadsF4, 1) f4_umma_kernel(const __grid_con
         __syncwarp();
     } else if (warp == 1) {
         // ------------------------------------------------------------------ instructions
-        if (rank == 0 && elect_one()) {
+        if (elect_one()) {
             // E2M1 operands (bits 7, 10: type 1), N / 8, scale type (bit 23: 1 = E8M0), M / 128, K-major; the scale ids go to bits 4 and 29
-            const uint32_t idesc = (1u << 7) | (1u << 10) | ((uint32_t)(p.bn >> 3) << 17) | ((FMT == LN_MX4 ? 1u : 0u) << 23) | ((uint32_t)kCtas << 27);
+            const uint32_t idesc = (1u << 7) | (1u << 10) | ((uint32_t)(p.bn >> 3) << 17) | ((FMT == LN_MX4 ? 1u : 0u) << 23) | (1u << 27);
             const uint64_t desc_base = make_smem_desc(0u, p.bk);
             constexpr int kWords = FMT == LN_MX4 ? 2 : 4;  // of a whole k-block
             const uint64_t sfa_desc = scale_desc(p.off_sfa), sfb_desc = scale_desc(p.off_sfb);
@@ -360,8 +278,7 @@ __global__ void __launch_bounds__(kThreadsF4, 1) f4_umma_kernel(const __grid_con
                 const uint32_t shift = (uint32_t)((tf * p.bn & 127) >> 5);  // first column of the tile's filters inside their group of 128
                 int c0 = 0;
                 for (int kb = 0; kb < kblocks; ++kb) {
-                    ok = PAIR && !p.flat ? mbar_wait_pair(full_bar(stage), phase, abort_flag, p.status) : mbar_wait(full_bar(stage), phase, abort_flag, p.status, LN_STATUS_MMA_TIMEOUT);
-                    if (!ok) break;
+                    if (!(ok = mbar_wait(full_bar(stage), phase, abort_flag, p.status, LN_STATUS_MMA_TIMEOUT))) break;
                     const uint32_t at = smem_base + (uint32_t)stage * p.stage_bytes;
                     const uint32_t sfa = tmem_base + kScaleCols + set * kScaleSet, sfb = sfa + kScaleB;
                     const int left = p.cstride - c0, n = (left < p.bk ? left : p.bk) >> 5;  // instructions of this k-block
@@ -371,33 +288,33 @@ __global__ void __launch_bounds__(kThreadsF4, 1) f4_umma_kernel(const __grid_con
                         // instructions of a k-block took their thread 1100 cycles, this way 390, less than the 530 that they run for
 #pragma unroll
                         for (int j = 0; j < kWords; ++j) {
-                            tc_copy_scales<PAIR>(sfa + 4u * j, sfa_desc + ((at + 512u * j) >> 4));
+                            tc_copy_scales(sfa + 4u * j, sfa_desc + ((at + 512u * j) >> 4));
 #pragma unroll
-                            for (int b = 0; b < WBLOCKS; ++b) tc_copy_scales<PAIR>(sfb + 4u * (j * WBLOCKS + b), sfb_desc + ((at + 512u * (b * kWords + j)) >> 4));
+                            for (int b = 0; b < WBLOCKS; ++b) tc_copy_scales(sfb + 4u * (j * WBLOCKS + b), sfb_desc + ((at + 512u * (b * kWords + j)) >> 4));
                         }
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             const uint32_t word = FMT == LN_MX4 ? i >> 1 : i, id = FMT == LN_MX4 ? (uint32_t)(i & 1) * 2u : 0u;
-                            tc_mma_scaled<FMT, PAIR>(d, a_desc + 2u * i, b_desc + 2u * i, idesc | (id << 4) | (id << 29), sfa + 4u * word, sfb + 4u * word * WBLOCKS + shift, i ? 1u : (uint32_t)(kb != 0));
+                            tc_mma_scaled<FMT>(d, a_desc + 2u * i, b_desc + 2u * i, idesc | (id << 4) | (id << 29), sfa + 4u * word, sfb + 4u * word * WBLOCKS + shift, i ? 1u : (uint32_t)(kb != 0));
                         }
                     } else {
                         for (int j = 0; j < p.words; ++j) {
-                            tc_copy_scales<PAIR>(sfa + 4u * j, sfa_desc + ((at + 512u * j) >> 4));
-                            for (int b = 0; b < WBLOCKS; ++b) tc_copy_scales<PAIR>(sfb + 4u * (j * WBLOCKS + b), sfb_desc + ((at + 512u * (b * p.words + j)) >> 4));
+                            tc_copy_scales(sfa + 4u * j, sfa_desc + ((at + 512u * j) >> 4));
+                            for (int b = 0; b < WBLOCKS; ++b) tc_copy_scales(sfb + 4u * (j * WBLOCKS + b), sfb_desc + ((at + 512u * (b * p.words + j)) >> 4));
                         }
                         for (int i = 0; i < n; ++i) {
                             const uint32_t word = FMT == LN_MX4 ? i >> 1 : i, id = FMT == LN_MX4 ? (uint32_t)(i & 1) * 2u : 0u;
-                            tc_mma_scaled<FMT, PAIR>(d, a_desc + 2u * i, b_desc + 2u * i, idesc | (id << 4) | (id << 29), sfa + 4u * word, sfb + 4u * word * WBLOCKS + shift, (uint32_t)((kb | i) != 0));
+                            tc_mma_scaled<FMT>(d, a_desc + 2u * i, b_desc + 2u * i, idesc | (id << 4) | (id << 29), sfa + 4u * word, sfb + 4u * word * WBLOCKS + shift, (uint32_t)((kb | i) != 0));
                         }
                     }
-                    commit<PAIR>(empty_bar(stage));
+                    tc_commit(empty_bar(stage));
                     set ^= 1u;
                     c0 += p.bk;
                     if (c0 >= p.cstride) c0 = 0;
                     if (++stage == p.stages) { stage = 0; phase ^= 1u; }
                 }
                 if (!ok) break;
-                commit<PAIR>(tfull_bar(buf));
+                tc_commit(tfull_bar(buf));
             }
         }
         __syncwarp();
@@ -407,7 +324,7 @@ __global__ void __launch_bounds__(kThreadsF4, 1) f4_umma_kernel(const __grid_con
         int iy0[4], ix0[4], img[4];
         auto enter_tile = [&]() {
             if (unit >= p.num_units) return;
-            const f4_tile t = tile_at<PAIR>(p, unit, rank);
+            const f4_tile t = tile_at(p, unit);
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
                 const int row = g * 32 + lane;
@@ -453,10 +370,7 @@ __global__ void __launch_bounds__(kThreadsF4, 1) f4_umma_kernel(const __grid_con
                         asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + 512u * j), "r"(v[0][j]), "r"(v[1][j]), "r"(v[2][j]), "r"(v[3][j]) : "memory");
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
-                if (lane == 0) {
-                    if (PAIR) arrive_first<true>(full_bar(stage));
-                    else mbar_arrive(full_bar(stage));
-                }
+                if (lane == 0) mbar_arrive(full_bar(stage));
                 stage += kGatherWarps;
                 if (stage >= p.stages) { stage -= p.stages; phase ^= 1u; }
                 // (behind the fence, which would wait for the reads; the other warps' k-blocks cover their latency)
@@ -496,7 +410,7 @@ __global__ void __launch_bounds__(kThreadsF4, 1) f4_umma_kernel(const __grid_con
         prefetch();
         bool ok = true;
         while (unit < p.num_units) {
-            const f4_tile at = tile_at<PAIR>(p, unit, rank);
+            const f4_tile at = tile_at(p, unit);
             const int sub = sub_of(), f0 = at.f0 + sub * CH, this_buf = buf;
             const uint32_t this_phase = phase;
             const bool first = order < 4;
@@ -524,13 +438,8 @@ __global__ void __launch_bounds__(kThreadsF4, 1) f4_umma_kernel(const __grid_con
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) {
-                        if (PAIR) {
-                            arrive_first<false>(tempty_bar(this_buf));
-                            if (overlap && first) arrive_first<false>(early_bar(this_buf));
-                        } else {
-                            mbar_arrive(tempty_bar(this_buf));
-                            if (overlap && first) mbar_arrive(early_bar(this_buf));
-                        }
+                        mbar_arrive(tempty_bar(this_buf));
+                        if (overlap && first) mbar_arrive(early_bar(this_buf));
                     }
                     __syncwarp();
                 }
@@ -584,11 +493,9 @@ __global__ void __launch_bounds__(kThreadsF4, 1) f4_umma_kernel(const __grid_con
         for (int i = 0; i < 64; ++i) __nanosleep(20000);
     }
     __syncthreads();
-    if (PAIR) pair_sync();  // neither CTA leaves while the other may still signal its barriers or work in its TMEM
     if (warp == 1) {
         tc_fence_after();
-        if (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512u) : "memory");
-        else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512u) : "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512u) : "memory");
     }
 }
 
@@ -599,30 +506,14 @@ int log2_of(int v) {
 }
 
 template <int FMT, int OUT>
-cudaError_t launch(ln_ctx* ctx, const f4_params& p, bool pair, int grid, size_t smem) {
-    auto go = [&](void (*k)(const f4_params)) -> cudaError_t {
-        if (!ctx->configured_kernels.count((const void*)k)) {
-            const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmemF4);
-            if (e != cudaSuccess) return e;
-            ctx->configured_kernels.insert((const void*)k);
-        }
-        cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3((unsigned)grid);
-        cfg.blockDim = dim3(kThreadsF4);
-        cfg.dynamicSmemBytes = smem;
-        cfg.stream = ctx->stream;
-        cudaLaunchAttribute attr[2];
-        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attr[0].val.programmaticStreamSerializationAllowed = 1;
-        attr[1].id = cudaLaunchAttributeClusterDimension;
-        attr[1].val.clusterDim.x = 2;
-        attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
-        cfg.attrs = attr;
-        cfg.numAttrs = pair ? 2 : 1;
-        return cudaLaunchKernelEx(&cfg, k, p);
-    };
-    if (pair) return go(f4_umma_kernel<FMT, OUT, 2, true>);
-    return p.bn > 128 ? go(f4_umma_kernel<FMT, OUT, 2, false>) : go(f4_umma_kernel<FMT, OUT, 1, false>);
+cudaError_t launch(ln_ctx* ctx, const f4_params& p, int grid, size_t smem) {
+    void (*k)(const f4_params) = p.bn > 128 ? f4_umma_kernel<FMT, OUT, 2> : f4_umma_kernel<FMT, OUT, 1>;
+    if (!ctx->configured_kernels.count((const void*)k)) {
+        const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmemF4);
+        if (e != cudaSuccess) return e;
+        ctx->configured_kernels.insert((const void*)k);
+    }
+    return ln_f4_launch(ctx, k, grid, kThreadsF4, smem, p);
 }
 
 }  // namespace
@@ -660,41 +551,41 @@ int ln_f4_umma_launch(ln_ctx* ctx, const ln_f4_conv& c) {
         }
     p.log_tw = log2_of(p.TW); p.log_th = log2_of(p.TH);
     // filter tile
-    const int64_t instructions = (int64_t)c.k * c.k * x.cstride / 32;
+    // A launch takes about start + (k-blocks of a tile + (rounds - 1) x the longer of k-blocks and epilogue), rounds = tiles per SM, in ns
+    // as measured over 27 shapes of both types with binary16 output (leaky), 3 to 76 us, each with every tile; the choice was the best one or
+    // within 4 % of it on all of them.  Where most SMs have nothing to do, a k-block of 256 filters comes faster.
+    const int64_t kblocks = (int64_t)c.k * c.k * kb.cblocks;
+    const int cand[3] = {256, 128, 64}, start[3] = {5400, 3650, 3300}, out[3] = {3300, 1750, 900}, flat_k[3] = {490, 360, 320}, tap_k[3] = {640, 520, 420};
     int64_t least = -1;
-    const int cand[4] = {256, 192, 128, 64};
-    for (int bn : cand) {
-        const int64_t rounds = (best * ((p.F + bn - 1) / bn) + ctx->sm_count - 1) / ctx->sm_count;
-        const int64_t chain = instructions * (bn >= 128 ? bn / 2 + 8 : 100), out = (int64_t)bn * 12;
-        const int64_t cost = rounds * (bn == 256 ? chain + 500 + (out > chain ? out - chain : 0) : (chain > out ? chain : out)) + out;
-        if (least < 0 || cost < least) { least = cost; p.bn = bn; }
+    for (int i = 0; i < 3; ++i) {
+        const int64_t units = best * ((p.F + cand[i] - 1) / cand[i]), rounds = (units + ctx->sm_count - 1) / ctx->sm_count;
+        const int64_t chain = kblocks * (!flat ? tap_k[i] : (i == 0 && 2 * units <= ctx->sm_count ? 330 : flat_k[i]));
+        const int64_t cost = start[i] + chain + (rounds - 1) * (chain > out[i] ? chain : out[i]);
+        if (least < 0 || cost < least) { least = cost; p.bn = cand[i]; }
     }
     if (const char* e = getenv("LN_F4_BN")) {  // (A/B measurements: another filter tile)
         for (int bn : cand)
             if (atoi(e) == bn) p.bn = bn;
     }
     const int wblocks = p.bn > 128 ? 2 : 1;
-    bool pair = p.bn > 128 && best > 1;
-    if (const char* e = getenv("LN_F4_PAIR")) pair = pair && atoi(e) != 0;  // (A/B measurements: no CTA pairs)
     p.nbuf = p.bn == 256 ? 2 : (int)kScaleCols / p.bn;
     p.acc_step = p.bn == 256 ? kOverlapBase : p.bn;
     p.subs = p.bn / CH;
     p.flat = flat ? 1 : 0;
     p.tiles_f = (p.F + p.bn - 1) / p.bn; p.tiles_w = (p.OW + p.TW - 1) / p.TW; p.tiles_h = (p.OH + p.TH - 1) / p.TH;
-    const int64_t num_units = (pair ? (best + 1) / 2 : best) * p.tiles_f;
+    const int64_t num_units = best * p.tiles_f;
     if (num_units >= (1 << 19)) return ln_fail(ctx, LN_ERR_UNSUPPORTED, "%s: %lld tiles", who, (long long)num_units);
     p.num_units = (int)num_units;
     auto magic = [](int d) { return ((1ull << 40) + (unsigned long long)d - 1) / (unsigned long long)d; };
     p.magic_f = magic(p.tiles_f); p.magic_w = magic(p.tiles_w); p.magic_h = magic(p.tiles_h);
     p.off_b = 128u * p.bk;
-    p.off_sfa = p.off_b + (uint32_t)(pair ? p.bn / 2 : p.bn) * p.bk;
+    p.off_sfa = p.off_b + (uint32_t)p.bn * p.bk;
     p.off_sfb = p.off_sfa + (uint32_t)p.words * 512u;
     p.stage_bytes = (uint32_t)ln_round_up(p.off_sfb + (uint32_t)(p.words * wblocks) * 512u, 1024);
     p.stages = (int)((kMaxSmemF4 - 1024 - kBarBytesF4 - kTabBytesF4) / p.stage_bytes);
     if (p.stages > kMaxStagesF4) p.stages = kMaxStagesF4;
     size_t smem = 1024 + (size_t)p.stages * p.stage_bytes + kBarBytesF4 + kTabBytesF4;
-    // One CTA per SM, whatever else runs: a CTA takes all of TMEM and waits while another one has it, and of two pairs on the same two SMs
-    // each could hold what the other waits for.  So none asks for less than half of an SM's shared memory.
+    // One CTA per SM: it takes all of TMEM and would wait while another one has it, so none asks for less than half of an SM's shared memory.
     if (smem < kLeastSmemF4) smem = kLeastSmemF4;
     p.xsf = (const uint8_t*)x.sf; p.wscale = c.w->wscale; p.bias = c.bias;
     p.y = y.ptr; p.ys = y.cstride; p.ysf = (uint8_t*)y.sf; p.ysf_words = y.sf_words;
@@ -720,7 +611,7 @@ int ln_f4_umma_launch(ln_ctx* ctx, const ln_f4_conv& c) {
     {
         const cuuint64_t dims[2] = {(cuuint64_t)((int64_t)c.k * c.k * x.cstride), (cuuint64_t)p.F};
         const cuuint64_t strides[1] = {(cuuint64_t)((int64_t)c.k * c.k * x.cstride)};
-        const cuuint32_t box[2] = {(cuuint32_t)p.bk, (cuuint32_t)(pair ? p.bn / 2 : p.bn)};
+        const cuuint32_t box[2] = {(cuuint32_t)p.bk, (cuuint32_t)p.bn};
         const CUresult r = ctx->encode_tiled(&p.tmB, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, c.w->w, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swz, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
                                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
         if (r != CUDA_SUCCESS) return ln_fail(ctx, LN_ERR_CUDA, "%s: cuTensorMapEncodeTiled(weights) failed with %d", who, (int)r);
@@ -739,13 +630,12 @@ int ln_f4_umma_launch(ln_ctx* ctx, const ln_f4_conv& c) {
         }
         if (r != CUDA_SUCCESS) return ln_fail(ctx, LN_ERR_CUDA, "%s: cuTensorMapEncodeTiled(scales) failed with %d", who, (int)r);
     }
-    const int places = pair ? ctx->sm_count / 2 : ctx->sm_count, grid = (p.num_units < places ? p.num_units : places) * (pair ? 2 : 1);
+    const int grid = p.num_units < ctx->sm_count ? p.num_units : ctx->sm_count;
     cudaError_t e;
 #define LN_F4_LAUNCH(FMT) \
-    (c.out_kind == LN_OUT_F32 ? launch<FMT, LN_OUT_F32>(ctx, p, pair, grid, smem) : c.out_kind == LN_OUT_F16 ? launch<FMT, LN_OUT_F16>(ctx, p, pair, grid, smem) : launch<FMT, LN_OUT_Q>(ctx, p, pair, grid, smem))
+    (c.out_kind == LN_OUT_F32 ? launch<FMT, LN_OUT_F32>(ctx, p, grid, smem) : c.out_kind == LN_OUT_F16 ? launch<FMT, LN_OUT_F16>(ctx, p, grid, smem) : launch<FMT, LN_OUT_Q>(ctx, p, grid, smem))
     e = c.dtype == LN_F4 ? LN_F4_LAUNCH(LN_F4) : LN_F4_LAUNCH(LN_MX4);
 #undef LN_F4_LAUNCH
-    ctx->launches++;
     if (e != cudaSuccess) {
         (void)cudaGetLastError();
         return ln_fail(ctx, LN_ERR_CUDA, "%s: launch failed: %s", who, cudaGetErrorString(e));

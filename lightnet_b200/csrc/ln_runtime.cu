@@ -305,8 +305,9 @@ int32_t ln_tensor_shape(const ln_tensor* t, int64_t shape[4]) {
 
 int32_t ln_tensor_dtype(const ln_tensor* t) { return t ? t->dtype : -1; }
 
-int32_t ln_tensor_device_data(const ln_tensor* t, void** data, int64_t strides[4]) {
-    if (!t || !data || !strides) return LN_ERR_ARG;
+int32_t ln_tensor_device_data(const ln_tensor* t, void** data, int64_t shape[4], int64_t strides[4]) {
+    if (!t || !data || !shape || !strides) return LN_ERR_ARG;
+    ln_tensor_shape(t, shape);
     if (t->dtype == LN_F32) {
         strides[3] = 1; strides[2] = t->w; strides[1] = t->h * t->w; strides[0] = t->c * t->h * t->w;
     } else if (t->dtype == LN_F16) {

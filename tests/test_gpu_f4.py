@@ -340,8 +340,8 @@ def test_array_interface_shares_the_memory(be):
     assert np.array_equal(a.cpu().numpy(), x)
     q = be.narrow_f4(be.upload_f32(x.shape, x), 0.01)
     assert not hasattr(q, "__cuda_array_interface__")
-    p, s = C.c_void_p(), (C.c_int64 * 4)()
-    assert be.lib.ln_tensor_device_data(q.h, C.byref(p), s) == 5
+    p, shape, s = C.c_void_p(), (C.c_int64 * 4)(), (C.c_int64 * 4)()
+    assert be.lib.ln_tensor_device_data(q.h, C.byref(p), shape, s) == 5
 
 
 def refused(kind, fn, *args):
