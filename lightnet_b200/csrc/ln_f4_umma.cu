@@ -120,30 +120,17 @@ __device__ __forceinline__ void act2(float& v0, float& v1) {
         else { v0 = v0 == v0 ? r0 : v0; v1 = v1 == v1 ? r1 : v1; }  // (max drops a NaN)
     }
 }
-template <int W>
-__device__ __forceinline__ void act_all(int act, bool exact, float (&v)[W]) {
-#define LN_ALL(A)                                                                          \
-    _Pragma("unroll") for (int i = 0; i < W; ++i) v[i] = ln_epilogue_act<true>(A, v[i]);   \
-    break;
-#define LN_FAST(A)                                                                         \
-    _Pragma("unroll") for (int i = 0; i < W; i += 2) act2<A>(v[i], v[i + 1]);              \
-    break;
-    switch (act) {
-        case LN_ACT_LEAKY: LN_ALL(LN_ACT_LEAKY)
-        case LN_ACT_RELU: LN_ALL(LN_ACT_RELU)
-        case LN_ACT_MISH:
-            if (exact) { LN_ALL(LN_ACT_MISH) }
-            LN_FAST(LN_ACT_MISH)
-        case LN_ACT_SWISH:
-            if (exact) { LN_ALL(LN_ACT_SWISH) }
-            LN_FAST(LN_ACT_SWISH)
-        case LN_ACT_LOGISTIC:
-            if (exact) { LN_ALL(LN_ACT_LOGISTIC) }
-            LN_FAST(LN_ACT_LOGISTIC)
-        default: break;
+template <int ACT, bool EXACT, int W>
+__device__ __forceinline__ void act_all(float (&v)[W]) {
+    constexpr bool fast = !EXACT && (ACT == LN_ACT_MISH || ACT == LN_ACT_SWISH || ACT == LN_ACT_LOGISTIC);
+#pragma unroll
+    for (int i = 0; i < W; i += 2) {
+        if (fast) act2<ACT>(v[i], v[i + 1]);
+        else {
+            v[i] = ln_epilogue_act<true>(ACT, v[i]);
+            v[i + 1] = ln_epilogue_act<true>(ACT, v[i + 1]);
+        }
     }
-#undef LN_ALL
-#undef LN_FAST
 }
 __device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[16]) { tmem_ld_32x16(taddr, r); tmem_ld_wait(); }
 __device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[32]) { tmem_ld_32x32(taddr, r); tmem_ld_wait(); }
@@ -159,6 +146,123 @@ __device__ __forceinline__ f4_tile tile_at(const f4_params& p, int unit) {
     const int q2 = fast_div(q1, p.magic_w), tw = q1 - q2 * p.tiles_w;
     const int tn = fast_div(q2, p.magic_h), th = q2 - tn * p.tiles_h;
     return {tw * p.TW, th * p.TH, tn * p.TN, tf * p.bn};
+}
+
+// what the epilogue shares with the other roles: shared addresses of its table and barriers
+struct f4_epilogue_at {
+    uint32_t tmem, tab, tfull, tempty, early;
+    volatile int* abort_flag;
+};
+template <int FMT, int OUT, int WBLOCKS, int ACT, bool EXACT>
+__device__ __forceinline__ void f4_epilogue(const f4_params& p, const f4_epilogue_at& e) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, first_unit = (int)blockIdx.x, step = (int)gridDim.x;
+    constexpr bool overlap = WBLOCKS == 2;
+    // Group g takes the units with number % 4 == g.  (nbuf * subs >= 4: a group that waits for a tile's accumulator has finished a unit
+    // of the tile nbuf before it or a later one, so the parity is unambiguous.)
+    constexpr int W = OUT == LN_OUT_Q && FMT == LN_MX4 ? 32 : 16;  // columns at a time (a block of a 4-bit output)
+    const int quad = warp & 3, group = (warp - kFirstEpilogueWarp) >> 2;
+    const int row = quad * 32 + lane, pw = row & (p.TW - 1), ph = (row >> p.log_tw) & (p.TH - 1), pn = row >> (p.log_tw + p.log_th);
+    const uint32_t tab = e.tab;
+    // {multiplier, bias} of the unit's column that this lane looks after, read one unit ahead (volatile: otherwise the compiler moves the
+    // loads down to their use, and every unit waits for them)
+    float wscale = 0.0f, bias = 0.0f;
+    int unit = first_unit, order = group, buf = 0;
+    uint32_t phase = 0;
+    auto settle = [&]() {  // units beyond the tile's: the next tiles
+        while (order >= p.subs) {
+            order -= p.subs;
+            unit += step;
+            if (++buf == p.nbuf) { buf = 0; phase ^= 1u; }
+        }
+    };
+    auto sub_of = [&]() { return overlap && buf == 0 ? order ^ 4 : order; };  // (what overlaps the other accumulator first)
+    auto prefetch = [&]() {
+        if (unit >= p.num_units) return;
+        const int f = (unit - fast_div(unit, p.magic_f) * p.tiles_f) * p.bn + sub_of() * CH + lane;
+        if (f >= p.F) { wscale = bias = 0.0f; return; }
+        asm volatile("ld.global.nc.f32 %0, [%1];" : "=f"(wscale) : "l"(p.wscale + f));
+        asm volatile("ld.global.nc.f32 %0, [%1];" : "=f"(bias) : "l"(p.bias + f));
+    };
+    settle();
+    prefetch();
+    bool ok = true;
+    while (unit < p.num_units) {
+        const f4_tile at = tile_at(p, unit);
+        const int sub = sub_of(), f0 = at.f0 + sub * CH, this_buf = buf;
+        const uint32_t this_phase = phase;
+        const bool first = order < 4;
+        const int ow = at.ow0 + pw, oh = at.oh0 + ph, n = at.n0 + pn;
+        const bool valid = ow < p.OW && oh < p.OH && n < p.N;
+        const int pix = (n * p.OH + oh) * p.OW + ow;  // (of a valid row below 2^30)
+        // the table: {m 2i, m 2i + 1, b 2i, b 2i + 1}
+        __syncwarp();  // (that of the unit before has been read)
+        asm volatile("st.shared.f32 [%0], %1;" ::"r"(tab + 16u * (lane >> 1) + 4u * (lane & 1)), "f"(__fmul_rn(p.xscale, wscale)) : "memory");
+        asm volatile("st.shared.f32 [%0], %1;" ::"r"(tab + 16u * (lane >> 1) + 8u + 4u * (lane & 1)), "f"(bias) : "memory");
+        __syncwarp();
+        order += 4;
+        settle();
+        prefetch();
+        if (!(ok = warp_wait(e.tfull + 8u * this_buf, this_phase, e.abort_flag, p.status, LN_STATUS_EPILOGUE_TIMEOUT))) break;
+        tc_fence_after();
+        const uint32_t taddr = e.tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(this_buf * p.acc_step + sub * CH);
+        // A loop, not unrolled: 32 columns in one piece are more code than the instruction caches of four warps at different places of
+        // it keep, and the epilogue then waited for instructions most of the time.
+#pragma unroll 1
+        for (int c0 = 0; c0 < CH; c0 += W) {
+            uint32_t acc[W];
+            __syncwarp();  // (rows behind the last pixel store nothing)
+            tmem_ld(taddr + c0, acc);
+            if (c0 + W == CH) {
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(e.tempty + 8u * this_buf);
+                    if (overlap && first) mbar_arrive(e.early + 8u * this_buf);
+                }
+                __syncwarp();
+            }
+            const int f = f0 + c0;
+            // (binary16 channels are padded to 32, 4-bit ones to 64: what is behind them is not stored)
+            if (f0 >= (OUT == LN_OUT_Q ? (p.F + 63) & ~63 : p.F)) continue;
+            float v[W];
+#pragma unroll
+            for (int i = 0; i < W; i += 2) {
+                float4 t;  // (volatile: the table is another one for every unit)
+                asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(t.x), "=f"(t.y), "=f"(t.z), "=f"(t.w) : "r"(tab + 8u * (c0 + i)));
+                ffma2(v[i], v[i + 1], __uint_as_float(acc[i]), __uint_as_float(acc[i + 1]), t.x, t.y, t.z, t.w);
+            }
+            act_all<ACT, EXACT>(v);
+            if (f + W > p.F) {
+#pragma unroll
+                for (int i = 0; i < W; ++i)
+                    if (f + i >= p.F) v[i] = 0.0f;
+            }
+            if (OUT == LN_OUT_F32) {
+                if (!valid) continue;
+                const int img = pix / p.hw;
+                float* dst = (float*)p.y + ((long long)img * p.F + f) * p.hw + (pix - img * p.hw);
+#pragma unroll
+                for (int i = 0; i < W; ++i)
+                    if (f + i < p.F) dst[(long long)i * p.hw] = v[i];
+            } else if (OUT == LN_OUT_F16) {
+                uint32_t h[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const __half2 q = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+                    h[i] = *reinterpret_cast<const uint32_t*>(&q);
+                }
+                if (valid) store_32((uint8_t*)p.y + (long long)pix * p.ys + 2 * f, h);
+            } else {
+                uint32_t q[W / 8];
+                const uint32_t sf = ln_f4_quantise<FMT>(v, p.g, p.six_g, q);
+                if (!valid) continue;
+                uint8_t* dst = (uint8_t*)p.y + (long long)pix * p.ys + f / 2;
+                if (W == 16) *(uint2*)dst = make_uint2(q[0], q[1]);
+                else *(uint4*)dst = make_uint4(q[0], q[1], q[W / 8 - 2], q[W / 8 - 1]);
+                p.ysf[ln_f4_sf_at(pix, f / (4 * W), p.ysf_words) + f / W % 4] = (uint8_t)sf;
+            }
+        }
+    }
 }
 
 // WBLOCKS: groups of 128 filters that a tile's scales are in
@@ -380,109 +484,18 @@ __global__ void __launch_bounds__(kThreadsF4, 1) f4_umma_kernel(const __grid_con
         }
     } else if (warp >= kFirstEpilogueWarp) {
         // ------------------------------------------------------------------ epilogue
-        // Group g takes the units with number % 4 == g.  (nbuf * subs >= 4: a group that waits for a tile's accumulator has finished a unit
-        // of the tile nbuf before it or a later one, so the parity is unambiguous.)
-        constexpr int W = OUT == LN_OUT_Q && FMT == LN_MX4 ? 32 : 16;  // columns at a time (a block of a 4-bit output)
-        const int quad = warp & 3, group = (warp - kFirstEpilogueWarp) >> 2;
-        const int row = quad * 32 + lane, pw = row & (p.TW - 1), ph = (row >> p.log_tw) & (p.TH - 1), pn = row >> (p.log_tw + p.log_th);
-        const uint32_t tab = tab_base + (uint32_t)(warp - kFirstEpilogueWarp) * 256u;
-        // {multiplier, bias} of the unit's column that this lane looks after, read one unit ahead (volatile: otherwise the compiler moves the
-        // loads down to their use, and every unit waits for them)
-        float wscale = 0.0f, bias = 0.0f;
-        int unit = first_unit, order = group, buf = 0;
-        uint32_t phase = 0;
-        auto settle = [&]() {  // units beyond the tile's: the next tiles
-            while (order >= p.subs) {
-                order -= p.subs;
-                unit += step;
-                if (++buf == p.nbuf) { buf = 0; phase ^= 1u; }
-            }
-        };
-        auto sub_of = [&]() { return overlap && buf == 0 ? order ^ 4 : order; };  // (what overlaps the other accumulator first)
-        auto prefetch = [&]() {
-            if (unit >= p.num_units) return;
-            const int f = (unit - fast_div(unit, p.magic_f) * p.tiles_f) * p.bn + sub_of() * CH + lane;
-            if (f >= p.F) { wscale = bias = 0.0f; return; }
-            asm volatile("ld.global.nc.f32 %0, [%1];" : "=f"(wscale) : "l"(p.wscale + f));
-            asm volatile("ld.global.nc.f32 %0, [%1];" : "=f"(bias) : "l"(p.bias + f));
-        };
-        settle();
-        prefetch();
-        bool ok = true;
-        while (unit < p.num_units) {
-            const f4_tile at = tile_at(p, unit);
-            const int sub = sub_of(), f0 = at.f0 + sub * CH, this_buf = buf;
-            const uint32_t this_phase = phase;
-            const bool first = order < 4;
-            const int ow = at.ow0 + pw, oh = at.oh0 + ph, n = at.n0 + pn;
-            const bool valid = ow < p.OW && oh < p.OH && n < p.N;
-            const int pix = (n * p.OH + oh) * p.OW + ow;  // (of a valid row below 2^30)
-            // the table: {m 2i, m 2i + 1, b 2i, b 2i + 1}
-            __syncwarp();  // (that of the unit before has been read)
-            asm volatile("st.shared.f32 [%0], %1;" ::"r"(tab + 16u * (lane >> 1) + 4u * (lane & 1)), "f"(__fmul_rn(p.xscale, wscale)) : "memory");
-            asm volatile("st.shared.f32 [%0], %1;" ::"r"(tab + 16u * (lane >> 1) + 8u + 4u * (lane & 1)), "f"(bias) : "memory");
-            __syncwarp();
-            order += 4;
-            settle();
-            prefetch();
-            if (!(ok = warp_wait(tfull_bar(this_buf), this_phase, abort_flag, p.status, LN_STATUS_EPILOGUE_TIMEOUT))) break;
-            tc_fence_after();
-            const uint32_t taddr = tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(this_buf * p.acc_step + sub * CH);
-            // A loop, not unrolled: 32 columns in one piece are more code than the instruction caches of four warps at different places of
-            // it keep, and the epilogue then waited for instructions most of the time.
-#pragma unroll 1
-            for (int c0 = 0; c0 < CH; c0 += W) {
-                uint32_t acc[W];
-                tmem_ld(taddr + c0, acc);
-                if (c0 + W == CH) {
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) {
-                        mbar_arrive(tempty_bar(this_buf));
-                        if (overlap && first) mbar_arrive(early_bar(this_buf));
-                    }
-                    __syncwarp();
-                }
-                const int f = f0 + c0;
-                // (binary16 channels are padded to 32, 4-bit ones to 64: what is behind them is not stored)
-                if (f0 >= (OUT == LN_OUT_Q ? (p.F + 63) & ~63 : p.F)) continue;
-                float v[W];
-#pragma unroll
-                for (int i = 0; i < W; i += 2) {
-                    float4 e;  // (volatile: the table is another one for every unit)
-                    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(e.x), "=f"(e.y), "=f"(e.z), "=f"(e.w) : "r"(tab + 8u * (c0 + i)));
-                    ffma2(v[i], v[i + 1], __uint_as_float(acc[i]), __uint_as_float(acc[i + 1]), e.x, e.y, e.z, e.w);
-                }
-                act_all<W>(p.act, p.exact != 0, v);
-                if (f + W > p.F) {
-#pragma unroll
-                    for (int i = 0; i < W; ++i)
-                        if (f + i >= p.F) v[i] = 0.0f;
-                }
-                if (!valid) continue;
-                if (OUT == LN_OUT_F32) {
-                    const int img = pix / p.hw;
-                    float* dst = (float*)p.y + ((long long)img * p.F + f) * p.hw + (pix - img * p.hw);
-#pragma unroll
-                    for (int i = 0; i < W; ++i)
-                        if (f + i < p.F) dst[(long long)i * p.hw] = v[i];
-                } else if (OUT == LN_OUT_F16) {
-                    uint32_t h[8];
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const __half2 q = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
-                        h[i] = *reinterpret_cast<const uint32_t*>(&q);
-                    }
-                    store_32((uint8_t*)p.y + (long long)pix * p.ys + 2 * f, h);
-                } else {
-                    uint32_t q[W / 8];
-                    const uint32_t sf = ln_f4_quantise<FMT>(v, p.g, p.six_g, q);
-                    uint8_t* dst = (uint8_t*)p.y + (long long)pix * p.ys + f / 2;
-                    if (W == 16) *(uint2*)dst = make_uint2(q[0], q[1]);
-                    else *(uint4*)dst = make_uint4(q[0], q[1], q[W / 8 - 2], q[W / 8 - 1]);
-                    p.ysf[ln_f4_sf_at(pix, f / (4 * W), p.ysf_words) + f / W % 4] = (uint8_t)sf;
-                }
-            }
+        // (one loop per activation: a choice inside it put the code of a unit in pieces far apart, and its warps waited for instructions)
+        const f4_epilogue_at at = {tmem_base, tab_base + (uint32_t)(warp - kFirstEpilogueWarp) * 256u, tfull_bar(0), tempty_bar(0), early_bar(0), abort_flag};
+        switch (p.act + (p.exact ? 8 : 0)) {
+            case LN_ACT_LEAKY: case LN_ACT_LEAKY + 8: f4_epilogue<FMT, OUT, WBLOCKS, LN_ACT_LEAKY, true>(p, at); break;
+            case LN_ACT_RELU: case LN_ACT_RELU + 8: f4_epilogue<FMT, OUT, WBLOCKS, LN_ACT_RELU, true>(p, at); break;
+            case LN_ACT_MISH: f4_epilogue<FMT, OUT, WBLOCKS, LN_ACT_MISH, false>(p, at); break;
+            case LN_ACT_SWISH: f4_epilogue<FMT, OUT, WBLOCKS, LN_ACT_SWISH, false>(p, at); break;
+            case LN_ACT_LOGISTIC: f4_epilogue<FMT, OUT, WBLOCKS, LN_ACT_LOGISTIC, false>(p, at); break;
+            case LN_ACT_MISH + 8: f4_epilogue<FMT, OUT, WBLOCKS, LN_ACT_MISH, true>(p, at); break;
+            case LN_ACT_SWISH + 8: f4_epilogue<FMT, OUT, WBLOCKS, LN_ACT_SWISH, true>(p, at); break;
+            case LN_ACT_LOGISTIC + 8: f4_epilogue<FMT, OUT, WBLOCKS, LN_ACT_LOGISTIC, true>(p, at); break;
+            default: f4_epilogue<FMT, OUT, WBLOCKS, LN_ACT_LINEAR, true>(p, at); break;
         }
     }
 
