@@ -33,6 +33,7 @@ constexpr int kOverlapBase = 160;  // first column of the second accumulator of 
 constexpr uint32_t kScaleCols = 416, kScaleSet = 48, kScaleB = 16;  // TMEM columns: two sets of [16 pixels' | 32 filters'] scale words
 constexpr uint32_t kBarBytesF4 = 512;
 constexpr uint32_t kTabBytesF4 = 16 * 256;  // {multiplier, bias} of the columns that a warp is at
+constexpr uint32_t kRowBytesF4 = 32 * 17 * 4;  // of a warp, where f32 rows are stored through shared memory
 constexpr int kMaxSmemF4 = 227 * 1024;
 constexpr size_t kLeastSmemF4 = 118 * 1024;
 
@@ -150,7 +151,7 @@ __device__ __forceinline__ f4_tile tile_at(const f4_params& p, int unit) {
 
 // what the epilogue shares with the other roles: shared addresses of its table and barriers
 struct f4_epilogue_at {
-    uint32_t tmem, tab, tfull, tempty, early;
+    uint32_t tmem, tab, rows, tfull, tempty, early;  // rows: 32 rows of 17 words
     volatile int* abort_flag;
 };
 template <int FMT, int OUT, int WBLOCKS, int ACT, bool EXACT>
@@ -164,9 +165,12 @@ __device__ __forceinline__ void f4_epilogue(const f4_params& p, const f4_epilogu
     const int row = quad * 32 + lane, pw = row & (p.TW - 1), ph = (row >> p.log_tw) & (p.TH - 1), pn = row >> (p.log_tw + p.log_th);
     const uint32_t tab = e.tab;
     // {multiplier, bias} of the unit's column that this lane looks after, read one unit ahead (volatile: otherwise the compiler moves the
-    // loads down to their use, and every unit waits for them)
+    // loads down to their use, and every unit waits for them); LN_MX4 has no multiplier.  They go through a table in shared memory, 8
+    // bytes per column and warp: 1024 cycles of its port for 128 x 128 outputs, which with 512 of binary16 stores is what bounds the
+    // epilogue (measured 2400).
+    constexpr bool scaled = FMT == LN_F4;
     float wscale = 0.0f, bias = 0.0f;
-    int unit = first_unit, order = group, buf = 0;
+    int unit = first_unit, order = group, buf = 0, pixel_tile = 0, f0 = 0;  // of the next unit
     uint32_t phase = 0;
     auto settle = [&]() {  // units beyond the tile's: the next tiles
         while (order >= p.subs) {
@@ -175,36 +179,44 @@ __device__ __forceinline__ void f4_epilogue(const f4_params& p, const f4_epilogu
             if (++buf == p.nbuf) { buf = 0; phase ^= 1u; }
         }
     };
-    auto sub_of = [&]() { return overlap && buf == 0 ? order ^ 4 : order; };  // (what overlaps the other accumulator first)
     auto prefetch = [&]() {
         if (unit >= p.num_units) return;
-        const int f = (unit - fast_div(unit, p.magic_f) * p.tiles_f) * p.bn + sub_of() * CH + lane;
-        if (f >= p.F) { wscale = bias = 0.0f; return; }
-        asm volatile("ld.global.nc.f32 %0, [%1];" : "=f"(wscale) : "l"(p.wscale + f));
+        pixel_tile = fast_div(unit, p.magic_f);
+        f0 = (unit - pixel_tile * p.tiles_f) * p.bn + (overlap && buf == 0 ? order ^ 4 : order) * CH;  // (what overlaps the other accumulator first)
+        const int f = f0 + lane;
+        wscale = bias = 0.0f;
+        if (f >= p.F) return;
+        if (scaled) asm volatile("ld.global.nc.f32 %0, [%1];" : "=f"(wscale) : "l"(p.wscale + f));
         asm volatile("ld.global.nc.f32 %0, [%1];" : "=f"(bias) : "l"(p.bias + f));
     };
     settle();
     prefetch();
     bool ok = true;
     while (unit < p.num_units) {
-        const f4_tile at = tile_at(p, unit);
-        const int sub = sub_of(), f0 = at.f0 + sub * CH, this_buf = buf;
-        const uint32_t this_phase = phase;
+        const int this_f0 = f0, this_buf = buf;
+        const uint32_t this_phase = phase, taddr = e.tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(this_buf * p.acc_step + (overlap && buf == 0 ? order ^ 4 : order) * CH);
         const bool first = order < 4;
-        const int ow = at.ow0 + pw, oh = at.oh0 + ph, n = at.n0 + pn;
-        const bool valid = ow < p.OW && oh < p.OH && n < p.N;
-        const int pix = (n * p.OH + oh) * p.OW + ow;  // (of a valid row below 2^30)
-        // the table: {m 2i, m 2i + 1, b 2i, b 2i + 1}
+        int pix = pixel_tile * 128 + row;  // (of a valid row below 2^30)
+        bool valid = pix < p.OW;
+        if (!p.flat) {
+            const int q2 = fast_div(pixel_tile, p.magic_w), q3 = fast_div(q2, p.magic_h);
+            const int ow = (pixel_tile - q2 * p.tiles_w) * p.TW + pw, oh = (q2 - q3 * p.tiles_h) * p.TH + ph, n = q3 * p.TN + pn;
+            valid = ow < p.OW && oh < p.OH && n < p.N;
+            pix = (n * p.OH + oh) * p.OW + ow;
+        }
+        // the table: {m 2i, m 2i + 1, b 2i, b 2i + 1}, or the biases alone
         __syncwarp();  // (that of the unit before has been read)
-        asm volatile("st.shared.f32 [%0], %1;" ::"r"(tab + 16u * (lane >> 1) + 4u * (lane & 1)), "f"(__fmul_rn(p.xscale, wscale)) : "memory");
-        asm volatile("st.shared.f32 [%0], %1;" ::"r"(tab + 16u * (lane >> 1) + 8u + 4u * (lane & 1)), "f"(bias) : "memory");
+        if (scaled) {
+            asm volatile("st.shared.f32 [%0], %1;" ::"r"(tab + 16u * (lane >> 1) + 4u * (lane & 1)), "f"(__fmul_rn(p.xscale, wscale)) : "memory");
+            asm volatile("st.shared.f32 [%0], %1;" ::"r"(tab + 16u * (lane >> 1) + 8u + 4u * (lane & 1)), "f"(bias) : "memory");
+        } else
+            asm volatile("st.shared.f32 [%0], %1;" ::"r"(tab + 4u * lane), "f"(bias) : "memory");
         __syncwarp();
         order += 4;
         settle();
         prefetch();
         if (!(ok = warp_wait(e.tfull + 8u * this_buf, this_phase, e.abort_flag, p.status, LN_STATUS_EPILOGUE_TIMEOUT))) break;
         tc_fence_after();
-        const uint32_t taddr = e.tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(this_buf * p.acc_step + sub * CH);
         // A loop, not unrolled: 32 columns in one piece are more code than the instruction caches of four warps at different places of
         // it keep, and the epilogue then waited for instructions most of the time.
 #pragma unroll 1
@@ -221,15 +233,19 @@ __device__ __forceinline__ void f4_epilogue(const f4_params& p, const f4_epilogu
                 }
                 __syncwarp();
             }
-            const int f = f0 + c0;
+            const int f = this_f0 + c0;
             // (binary16 channels are padded to 32, 4-bit ones to 64: what is behind them is not stored)
-            if (f0 >= (OUT == LN_OUT_Q ? (p.F + 63) & ~63 : p.F)) continue;
+            if (this_f0 >= (OUT == LN_OUT_Q ? (p.F + 63) & ~63 : p.F)) continue;
             float v[W];
 #pragma unroll
-            for (int i = 0; i < W; i += 2) {
+            for (int i = 0; i < W; i += scaled ? 2 : 4) {
                 float4 t;  // (volatile: the table is another one for every unit)
-                asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(t.x), "=f"(t.y), "=f"(t.z), "=f"(t.w) : "r"(tab + 8u * (c0 + i)));
-                ffma2(v[i], v[i + 1], __uint_as_float(acc[i]), __uint_as_float(acc[i + 1]), t.x, t.y, t.z, t.w);
+                asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(t.x), "=f"(t.y), "=f"(t.z), "=f"(t.w) : "r"(tab + (scaled ? 8u : 4u) * (c0 + i)));
+                if (scaled) ffma2(v[i], v[i + 1], __uint_as_float(acc[i]), __uint_as_float(acc[i + 1]), t.x, t.y, t.z, t.w);
+                else {
+                    fadd2(v[i], v[i + 1], __uint_as_float(acc[i]), __uint_as_float(acc[i + 1]), t.x, t.y);
+                    fadd2(v[(i + 2) % W], v[(i + 3) % W], __uint_as_float(acc[(i + 2) % W]), __uint_as_float(acc[(i + 3) % W]), t.z, t.w);
+                }
             }
             act_all<ACT, EXACT>(v);
             if (f + W > p.F) {
@@ -238,6 +254,30 @@ __device__ __forceinline__ void f4_epilogue(const f4_params& p, const f4_epilogu
                     if (f + i >= p.F) v[i] = 0.0f;
             }
             if (OUT == LN_OUT_F32) {
+                if (p.flat && p.hw == 1) {  // rows of F values
+                    if (p.F % 8 == 0) {  // a lane's are consecutive and fill sectors
+                        float* dst = (float*)p.y + (long long)pix * p.F + f;
+#pragma unroll
+                        for (int i = 0; i < W; i += 8) {
+                            const uint32_t (&h)[8] = *reinterpret_cast<const uint32_t(*)[8]>(v + i);
+                            if (valid && f + i < p.F) store_32((uint8_t*)(dst + i), h);
+                        }
+                        continue;
+                    }
+                    // Rows begin anywhere: two rows at a time through shared memory (17 words apart: no bank twice), so that the 16 values of
+                    // one go out together.  (65536 x 128 -> 255: 94 us with a lane writing its own row.)
+                    const uint32_t rows = e.rows + 68u * lane;
+#pragma unroll
+                    for (int i = 0; i < W; ++i) asm volatile("st.shared.f32 [%0], %1;" ::"r"(rows + 4u * i), "f"(v[i]) : "memory");
+                    __syncwarp();
+                    const int c = lane & 15, first_row = pix - lane;  // (the rows of a warp are consecutive)
+                    for (int r = lane >> 4; r < 32; r += 2) {
+                        float one;
+                        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(one) : "r"(e.rows + 68u * r + 4u * c));
+                        if (first_row + r < p.OW && f + c < p.F) ((float*)p.y)[(long long)(first_row + r) * p.F + f + c] = one;
+                    }
+                    continue;  // (the lanes meet before the next columns)
+                }
                 if (!valid) continue;
                 const int img = pix / p.hw;
                 float* dst = (float*)p.y + ((long long)img * p.F + f) * p.hw + (pix - img * p.hw);
@@ -485,7 +525,7 @@ __global__ void __launch_bounds__(kThreadsF4, 1) f4_umma_kernel(const __grid_con
     } else if (warp >= kFirstEpilogueWarp) {
         // ------------------------------------------------------------------ epilogue
         // (one loop per activation: a choice inside it put the code of a unit in pieces far apart, and its warps waited for instructions)
-        const f4_epilogue_at at = {tmem_base, tab_base + (uint32_t)(warp - kFirstEpilogueWarp) * 256u, tfull_bar(0), tempty_bar(0), early_bar(0), abort_flag};
+        const f4_epilogue_at at = {tmem_base, tab_base + (uint32_t)(warp - kFirstEpilogueWarp) * 256u, tab_base + kTabBytesF4 + (uint32_t)(warp - kFirstEpilogueWarp) * kRowBytesF4, tfull_bar(0), tempty_bar(0), early_bar(0), abort_flag};
         switch (p.act + (p.exact ? 8 : 0)) {
             case LN_ACT_LEAKY: case LN_ACT_LEAKY + 8: f4_epilogue<FMT, OUT, WBLOCKS, LN_ACT_LEAKY, true>(p, at); break;
             case LN_ACT_RELU: case LN_ACT_RELU + 8: f4_epilogue<FMT, OUT, WBLOCKS, LN_ACT_RELU, true>(p, at); break;
@@ -570,7 +610,8 @@ int ln_f4_umma_launch(ln_ctx* ctx, const ln_f4_conv& c) {
     const int64_t kblocks = (int64_t)c.k * c.k * kb.cblocks;
     const int cand[3] = {256, 128, 64}, start[3] = {5400, 3650, 3300}, out[3] = {3300, 1750, 900}, flat_k[3] = {490, 360, 320}, tap_k[3] = {640, 520, 420};
     int64_t least = -1;
-    for (int i = 0; i < 3; ++i) {
+    const bool rows = c.out_kind == LN_OUT_F32 && flat && p.hw == 1 && p.F % 8 != 0;  // (their way through shared memory leaves no four stages of the widest tile)
+    for (int i = rows ? 1 : 0; i < 3; ++i) {
         const int64_t units = best * ((p.F + cand[i] - 1) / cand[i]), rounds = (units + ctx->sm_count - 1) / ctx->sm_count;
         const int64_t chain = kblocks * (!flat ? tap_k[i] : (i == 0 && 2 * units <= ctx->sm_count ? 330 : flat_k[i]));
         const int64_t cost = start[i] + chain + (rounds - 1) * (chain > out[i] ? chain : out[i]);
@@ -578,7 +619,7 @@ int ln_f4_umma_launch(ln_ctx* ctx, const ln_f4_conv& c) {
     }
     if (const char* e = getenv("LN_F4_BN")) {  // (A/B measurements: another filter tile)
         for (int bn : cand)
-            if (atoi(e) == bn) p.bn = bn;
+            if (atoi(e) == bn && !(rows && bn == 256)) p.bn = bn;
     }
     const int wblocks = p.bn > 128 ? 2 : 1;
     p.nbuf = p.bn == 256 ? 2 : (int)kScaleCols / p.bn;
@@ -595,9 +636,10 @@ int ln_f4_umma_launch(ln_ctx* ctx, const ln_f4_conv& c) {
     p.off_sfa = p.off_b + (uint32_t)p.bn * p.bk;
     p.off_sfb = p.off_sfa + (uint32_t)p.words * 512u;
     p.stage_bytes = (uint32_t)ln_round_up(p.off_sfb + (uint32_t)(p.words * wblocks) * 512u, 1024);
-    p.stages = (int)((kMaxSmemF4 - 1024 - kBarBytesF4 - kTabBytesF4) / p.stage_bytes);
+    const size_t rest = 1024 + kBarBytesF4 + kTabBytesF4 + (rows ? 16 * kRowBytesF4 : 0);
+    p.stages = (int)((kMaxSmemF4 - rest) / p.stage_bytes);
     if (p.stages > kMaxStagesF4) p.stages = kMaxStagesF4;
-    size_t smem = 1024 + (size_t)p.stages * p.stage_bytes + kBarBytesF4 + kTabBytesF4;
+    size_t smem = rest + (size_t)p.stages * p.stage_bytes;
     // One CTA per SM: it takes all of TMEM and would wait while another one has it, so none asks for less than half of an SM's shared memory.
     if (smem < kLeastSmemF4) smem = kLeastSmemF4;
     p.xsf = (const uint8_t*)x.sf; p.wscale = c.w->wscale; p.bias = c.bias;
