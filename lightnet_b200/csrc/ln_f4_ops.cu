@@ -11,6 +11,9 @@ namespace {
 
 constexpr int kThreads = 256;
 
+__device__ __forceinline__ void ln_store_32(void* dst, const uint32_t (&v)[8]) {  // a whole sector
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
+}
 // 16 bytes that are read once
 __device__ __forceinline__ uint4 ln_ldg_stream(const __half* p) { return __ldcs(reinterpret_cast<const uint4*>(p)); }
 
@@ -41,7 +44,7 @@ int32_t guarded(ln_ctx* ctx, const char* who, F&& body) {
 bool usable_scale(int dtype, float s) { return dtype == LN_MX4 ? s == 1.0f : s >= 0x1p-100f && s <= 0x1p100f; }
 
 // ---- narrow and widen -----------------------------------------------------------------------------------------------------------
-// binary16 NHWC: a thread takes 32 channels of a pixel, consecutive threads consecutive groups of them, so that all accesses of a warp are
+// binary16 NHWC (narrow): a thread takes 32 channels of a pixel, consecutive threads consecutive groups of them, so that all accesses of a warp are
 // contiguous; two neighbours, which always belong to one pixel (its channels are padded to 64), put their scale bytes together.
 // f32 NCHW: the 32 lanes of a warp are 8 pixels x 4 blocks, so that a row of 8 pixels is a sector of a plane on one side and the four
 // blocks of a pixel (32 or 64 bytes of codes, one word of scales) are contiguous on the other.
@@ -143,36 +146,27 @@ __device__ __forceinline__ void widen_16(uint2 w, uint32_t scale, float g, float
     }
 }
 template <int FMT, typename I>
-__global__ void __launch_bounds__(kThreads) widen_f16_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ sf, __half* __restrict__ y, int64_t ys, int64_t pixels, int C, int groups,
+__global__ void __launch_bounds__(kThreads) widen_f16_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ sf, __half* __restrict__ y, int64_t ys, int64_t pixels, int C, int blocks,
                                                              int64_t cstride, int64_t sf_words, float g) {
-    ln_f4_after_predecessor();
-    constexpr int B = FMT == LN_F4 ? 16 : 32;
-    const I total = (I)(pixels * groups), step = (I)(gridDim.x * blockDim.x);
+    ln_f4_after_predecessor();  // (16 channels a thread: its 32 bytes are a sector of the output)
+    const I total = (I)(pixels * blocks), step = (I)(gridDim.x * blockDim.x);
     for (I i = (I)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += step) {
-        const I pix = i / (I)groups;
-        const int c0 = (int)(i - pix * (I)groups) * 32;
-        const uint4 q = __ldg(reinterpret_cast<const uint4*>(codes + (int64_t)pix * cstride + c0 / 2));
-        const uint8_t* s = sf + ln_f4_sf_at(pix, c0 / (4 * B), sf_words) + c0 / B % 4;
-        const uint32_t scale = FMT == LN_F4 ? __ldg(reinterpret_cast<const uint16_t*>(s)) : __ldg(s);
-        float v[2][16];
-        widen_16<FMT>(make_uint2(q.x, q.y), scale & 0xFFu, g, v[0]);
-        widen_16<FMT>(make_uint2(q.z, q.w), FMT == LN_F4 ? scale >> 8 : scale, g, v[1]);
-        if (c0 + 32 > C) {  // (a NaN block that ends inside the padding must not reach it)
+        const I pix = i / (I)blocks;
+        const int b16 = (int)(i - pix * (I)blocks), b = FMT == LN_F4 ? b16 : b16 >> 1;
+        float v[16];
+        widen_16<FMT>(__ldg(reinterpret_cast<const uint2*>(codes + (int64_t)pix * cstride + b16 * 8)), __ldg(sf + ln_f4_sf_at(pix, b >> 2, sf_words) + (b & 3)), g, v);
+        if (b16 * 16 + 16 > C) {  // (a NaN block that ends inside the padding must not reach it)
 #pragma unroll
-            for (int j = 0; j < 32; ++j)
-                if (c0 + j >= C) v[j >> 4][j & 15] = 0.0f;
+            for (int j = 0; j < 16; ++j)
+                if (b16 * 16 + j >= C) v[j] = 0.0f;
         }
-        uint4* dst = reinterpret_cast<uint4*>(y + (int64_t)pix * ys + c0);
+        uint32_t h[8];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            uint32_t h[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const __half2 p = __floats2half2_rn(v[j >> 1][(j & 1) * 8 + 2 * k], v[j >> 1][(j & 1) * 8 + 2 * k + 1]);
-                h[k] = *reinterpret_cast<const uint32_t*>(&p);
-            }
-            dst[j] = make_uint4(h[0], h[1], h[2], h[3]);
+        for (int k = 0; k < 8; ++k) {
+            const __half2 p = __floats2half2_rn(v[2 * k], v[2 * k + 1]);
+            h[k] = *reinterpret_cast<const uint32_t*>(&p);
         }
+        ln_store_32(y + (int64_t)pix * ys + b16 * 16, h);
     }
 }
 template <int FMT, typename I>
@@ -198,6 +192,61 @@ __global__ void __launch_bounds__(kThreads) widen_f32_kernel(const uint8_t* __re
             for (int j = 0; j < 16; ++j)
                 if (b16 * 16 + j < C) dst[j * hw] = v[j];
         }
+    }
+}
+// f32 rows of tokens (1 x 1 images: a row is the channels of one).  A warp takes 32 consecutive blocks, whose values are one contiguous
+// range wherever rows begin; it goes through shared memory (17 words per 16: no bank twice) so that every access to it is coalesced.
+template <int FMT>
+__global__ void __launch_bounds__(kThreads) narrow_rows_kernel(const float* __restrict__ x, uint8_t* __restrict__ codes, uint8_t* __restrict__ sf, int64_t rows, int C, int blocks, int64_t cstride,
+                                                               int64_t sf_words, float g, float six_g) {
+    ln_f4_after_predecessor();
+    constexpr int B = FMT == LN_F4 ? 16 : 32;
+    __shared__ float stage[kThreads / 32][34 * B];
+    float* mine = stage[threadIdx.x / 32];
+    const int lane = threadIdx.x & 31;
+    const int64_t total = rows * blocks;
+    for (int64_t first = (blockIdx.x * (int64_t)(kThreads / 32) + threadIdx.x / 32) * 32; first < total; first += (int64_t)gridDim.x * kThreads) {
+        const int64_t u = first + lane < total ? first + lane : total - 1, row = u / blocks;
+        const int b = (int)(u - row * blocks), have = C - b * B < 0 ? 0 : (C - b * B < B ? C - b * B : B);
+        const int64_t at = row * C + (b * B < C ? b * B : C), from = __shfl_sync(0xFFFFFFFFu, at, 0);
+        const int o = (int)(at - from), end = __shfl_sync(0xFFFFFFFFu, o + have, 31);
+        __syncwarp();
+        for (int i = lane; i < end; i += 32) mine[i + (i >> 4)] = __ldcs(x + from + i);
+        __syncwarp();
+        float v[B];
+#pragma unroll
+        for (int j = 0; j < B; ++j) v[j] = j < have ? mine[o + j + ((o + j) >> 4)] : 0.0f;
+        const bool real = first + lane < total;
+        uint32_t s = real ? store_block<FMT>(v, g, six_g, codes + row * cstride + b * (B / 2)) : 0u;
+        s |= __shfl_down_sync(0xFFFFFFFFu, s, 1) << 8;
+        if (FMT == LN_F4) {  // (a row's blocks are a multiple of four, of LN_MX4 of two)
+            s |= __shfl_down_sync(0xFFFFFFFFu, s, 2) << 16;
+            if (real && (lane & 3) == 0) *reinterpret_cast<uint32_t*>(sf + ln_f4_sf_at(row, b >> 2, sf_words)) = s;
+        } else if (real && (lane & 1) == 0)
+            *reinterpret_cast<uint16_t*>(sf + ln_f4_sf_at(row, b >> 2, sf_words) + (b & 3)) = (uint16_t)s;
+    }
+}
+template <int FMT>
+__global__ void __launch_bounds__(kThreads) widen_rows_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ sf, float* __restrict__ y, int64_t rows, int C, int blocks, int64_t cstride,
+                                                              int64_t sf_words, float g) {
+    ln_f4_after_predecessor();  // (blocks of 16 channels for both types)
+    __shared__ float stage[kThreads / 32][34 * 16];
+    float* mine = stage[threadIdx.x / 32];
+    const int lane = threadIdx.x & 31;
+    const int64_t total = rows * blocks;
+    for (int64_t first = (blockIdx.x * (int64_t)(kThreads / 32) + threadIdx.x / 32) * 32; first < total; first += (int64_t)gridDim.x * kThreads) {
+        const int64_t u = first + lane < total ? first + lane : total - 1, row = u / blocks;
+        const int b16 = (int)(u - row * blocks), b = FMT == LN_F4 ? b16 : b16 >> 1, have = C - b16 * 16 < 16 ? C - b16 * 16 : 16;
+        const int64_t at = row * C + b16 * 16, from = __shfl_sync(0xFFFFFFFFu, at, 0);
+        const int o = (int)(at - from), end = __shfl_sync(0xFFFFFFFFu, o + have, 31);
+        float v[16];
+        widen_16<FMT>(__ldg(reinterpret_cast<const uint2*>(codes + row * cstride + b16 * 8)), __ldg(sf + ln_f4_sf_at(row, b >> 2, sf_words) + (b & 3)), g, v);
+        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+            if (j < have) mine[o + j + ((o + j) >> 4)] = v[j];
+        __syncwarp();
+        for (int i = lane; i < end; i += 32) y[from + i] = mine[i + (i >> 4)];
     }
 }
 // codes (one per byte) and scales in NCHW order
@@ -315,8 +364,12 @@ int narrow_into(ln_ctx* ctx, const ln_tensor* t, ln_tensor* q) {
     const float g = q->scale, six_g = 6.0f * g;
     const bool small = q->cstride * pixels < (1ll << 30);
     cudaError_t e;
-    if (t->dtype == LN_F32) {
-        const int blocks = (int)(q->cstride * 2 / ln_f4_block(q->dtype));
+    const int blocks = (int)(q->cstride * 2 / ln_f4_block(q->dtype));
+    if (t->dtype == LN_F32 && hw == 1) {
+        const int grid = grid_for(ctx, pixels * blocks);
+        e = q->dtype == LN_F4 ? ln_f4_launch(ctx, narrow_rows_kernel<LN_F4>, grid, kThreads, 0, (const float*)t->ptr, codes, sf, pixels, (int)t->c, blocks, q->cstride, q->sf_words, g, six_g)
+                              : ln_f4_launch(ctx, narrow_rows_kernel<LN_MX4>, grid, kThreads, 0, (const float*)t->ptr, codes, sf, pixels, (int)t->c, blocks, q->cstride, q->sf_words, g, six_g);
+    } else if (t->dtype == LN_F32) {
         e = LN_F4_CALL(narrow_f32_kernel, q->dtype, small, grid_for(ctx, (pixels + 7) / 8 * ((blocks + 3) / 4) * 32), (const float*)t->ptr, codes, sf, pixels, hw, (int)t->c, blocks, q->cstride, q->sf_words, g,
                        six_g);
     } else {
@@ -330,12 +383,16 @@ int widen_into(ln_ctx* ctx, const ln_tensor* t, ln_tensor* y) {
     const uint8_t *codes = (const uint8_t*)t->ptr, *sf = (const uint8_t*)t->sf;
     const bool small = t->cstride * pixels < (1ll << 30);
     cudaError_t e;
-    if (y->dtype == LN_F32) {
-        const int blocks = (int)((t->c + 15) / 16);
+    const int blocks = (int)((t->c + 15) / 16);
+    if (y->dtype == LN_F32 && hw == 1) {
+        const int grid = grid_for(ctx, pixels * blocks);
+        e = t->dtype == LN_F4 ? ln_f4_launch(ctx, widen_rows_kernel<LN_F4>, grid, kThreads, 0, codes, sf, (float*)y->ptr, pixels, (int)t->c, blocks, t->cstride, t->sf_words, t->scale)
+                              : ln_f4_launch(ctx, widen_rows_kernel<LN_MX4>, grid, kThreads, 0, codes, sf, (float*)y->ptr, pixels, (int)t->c, blocks, t->cstride, t->sf_words, t->scale);
+    } else if (y->dtype == LN_F32) {
         e = LN_F4_CALL(widen_f32_kernel, t->dtype, small, grid_for(ctx, (pixels + 7) / 8 * ((blocks + 3) / 4) * 32), codes, sf, (float*)y->ptr, pixels, hw, (int)t->c, blocks, t->cstride, t->sf_words, t->scale);
     } else {
-        const int groups = (int)(y->cstride / 64);
-        e = LN_F4_CALL(widen_f16_kernel, t->dtype, small, grid_for(ctx, pixels * groups), codes, sf, (__half*)y->ptr, y->cstride / 2, pixels, (int)t->c, groups, t->cstride, t->sf_words, t->scale);
+        const int padded = (int)(y->cstride / 32);  // (the channels of binary16 are padded to 32)
+        e = LN_F4_CALL(widen_f16_kernel, t->dtype, small, grid_for(ctx, pixels * padded), codes, sf, (__half*)y->ptr, y->cstride / 2, pixels, (int)t->c, padded, t->cstride, t->sf_words, t->scale);
     }
     return check_launch(ctx, "ln_tensor_widen_f4", e);
 }

@@ -94,7 +94,8 @@ def inputs(rng, shape, zeros=True):
     return x.astype(np.float32)
 
 
-SHAPES = [(1, 1, 1, 1), (1, 4096, 1, 1), (3, 16, 5, 7), (2, 33, 9, 11), (5, 64, 1, 3), (1, 129, 13, 13), (2, 333, 7, 5), (130, 40, 1, 1), (1, 31, 40, 33), (2, 255, 19, 19)]
+SHAPES = [(1, 1, 1, 1), (1, 4096, 1, 1), (3, 16, 5, 7), (2, 33, 9, 11), (5, 64, 1, 3), (1, 129, 13, 13), (2, 333, 7, 5), (130, 40, 1, 1), (1, 31, 40, 33), (2, 255, 19, 19),
+          (131, 333, 1, 1), (37, 1111, 1, 1), (257, 96, 1, 1), (3, 17, 1, 1), (33, 16, 1, 1)]
 
 
 @pytest.mark.parametrize("dtype", FMT)
