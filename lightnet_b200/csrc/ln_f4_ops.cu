@@ -353,6 +353,150 @@ __global__ void conv_f4_simt_kernel(const simt_params p) {
     }
 }
 
+// ---- the product for few pixels --------------------------------------------------------------------------------------------------
+// A 1x1 stride-1 convolution of up to 16 pixels (a token, or a few): the weights are read once and nothing else costs, so what counts is how
+// many reads are in flight.  A block of 16 warps takes 32 filters and cuts their k range into chunks of 128 channels; a lane reads 16 bytes of
+// a row (filter or pixel), widens them with their block scales to binary16 (LN_F4: a code times an E4M3 scale has 6 bits and at most 2688) or
+// bfloat16 (LN_MX4: any power of two), both exact, and feeds warp-level instructions, whose k order may be any as long as both operands have
+// the same: pixels fill 8 of their columns, the tensor pipe has time.  (tcgen05 works on 128 pixels and one CTA per 64 filters then walks the
+// whole k range: 4096 -> 4096 for one token 8.5 us, this way 4.7.)  The warps' sums are added in order.
+constexpr int kFewThreads = 512, kFewFilters = 32, kFewPixels = 16;
+struct few_params {
+    const uint8_t *x, *xsf, *w, *wsf;
+    const float *wscale, *bias;
+    void* y;
+    uint8_t* ysf;
+    int64_t xs, sf_words, ys, ysf_words;
+    int pixels, F, chunks, act, exact, out_kind, hw;
+    float xscale, g, six_g;
+};
+// 32 codes of a lane -> 16 scaled pairs
+template <int FMT>
+__device__ __forceinline__ void few_operand(const uint4& q, uint32_t scale, uint32_t (&h)[16]) {
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) ln_e2m1x8_to_h2(w[i], *reinterpret_cast<uint32_t(*)[4]>(h + 4 * i));
+    if (FMT == LN_F4) {
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+            const __half2 s = __float2half2_rn(ln_e4m3_value(scale >> (8 * b) & 0xFFu));
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const __half2 v = __hmul2(*reinterpret_cast<const __half2*>(&h[8 * b + i]), s);
+                h[8 * b + i] = *reinterpret_cast<const uint32_t*>(&v);
+            }
+        }
+    } else {
+        const float s = ln_e8m0_value(scale);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[i]));
+            h[i] = __byte_perm(__float_as_uint(__fmul_rn(f.x, s)), __float_as_uint(__fmul_rn(f.y, s)), 0x7632);  // (two bits and an exponent: the low halves are zero)
+        }
+    }
+}
+template <int FMT>
+__device__ __forceinline__ void few_mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    if (FMT == LN_F4)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+template <int FMT>
+__device__ __forceinline__ void few_load(const uint8_t* codes, const uint8_t* sf, int64_t row, bool there, int64_t stride, int64_t sf_words, int chunk, int t, uint4& q, uint32_t& scale) {
+    const int64_t at = (int64_t)chunk * 64 + t * 16;
+    q = make_uint4(0, 0, 0, 0);
+    scale = 0;
+    if (!there || at >= stride) return;
+    q = __ldg(reinterpret_cast<const uint4*>(codes + row * stride + at));
+    if (FMT == LN_F4) scale = __ldg(reinterpret_cast<const uint16_t*>(sf + ln_f4_sf_at(row, chunk * 2 + (t >> 1), sf_words) + (t & 1) * 2));
+    else scale = __ldg(sf + ln_f4_sf_at(row, chunk, sf_words) + t);
+}
+template <int FMT, int NT>
+__global__ void __launch_bounds__(kFewThreads) conv_f4_few_kernel(const few_params p) {
+    ln_f4_after_predecessor();
+    __shared__ float part[kFewThreads / 32][kFewFilters][8 * NT + 1];
+    __shared__ float sums[8 * NT][kFewFilters + 1];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, f0 = (int)blockIdx.x * kFewFilters;
+    float acc[2][NT][4] = {};
+#pragma unroll 2
+    for (int chunk = warp; chunk < p.chunks; chunk += kFewThreads / 32) {
+        uint4 wq[4], xq[NT];
+        uint32_t ws[4], xsc[NT];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) few_load<FMT>(p.w, p.wsf, f0 + g + 8 * i, f0 + g + 8 * i < p.F, p.xs, p.sf_words, chunk, t, wq[i], ws[i]);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) few_load<FMT>(p.x, p.xsf, g + 8 * n, g + 8 * n < p.pixels, p.xs, p.sf_words, chunk, t, xq[n], xsc[n]);
+        uint32_t b[NT][16];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) few_operand<FMT>(xq[n], xsc[n], b[n]);
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+            uint32_t lo[16], hi[16];
+            few_operand<FMT>(wq[2 * m], ws[2 * m], lo);
+            few_operand<FMT>(wq[2 * m + 1], ws[2 * m + 1], hi);
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int s = 0; s < 8; ++s) few_mma<FMT>(acc[m][n], lo[2 * s], hi[2 * s], lo[2 * s + 1], hi[2 * s + 1], b[n][2 * s], b[n][2 * s + 1]);
+        }
+    }
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) part[warp][16 * m + g + (i >> 1) * 8][8 * n + 2 * t + (i & 1)] = acc[m][n][i];
+    __syncthreads();
+    const int i = threadIdx.x, f = f0 + (i & 31), n = i >> 5;  // (a warp: the 32 filters of a pixel)
+    if (n < 8 * NT) {
+        float sum = 0.0f;
+#pragma unroll
+        for (int k = 0; k < kFewThreads / 32; ++k) sum += part[k][i & 31][n];
+        float v = 0.0f;
+        if (f < p.F) {
+            v = __fmaf_rn(sum, __fmul_rn(p.xscale, p.wscale[f]), p.bias[f]);
+            v = p.exact ? ln_epilogue_act<true>(p.act, v) : ln_epilogue_act<false>(p.act, v);
+        }
+        if (p.out_kind == LN_OUT_Q) sums[n][i & 31] = v;
+        else if (n < p.pixels) {
+            if (p.out_kind == LN_OUT_F16) ((__half*)p.y)[n * p.ys + f] = __float2half_rn(v);  // (filters are padded to 32)
+            else if (f < p.F) {
+                const int img = n / p.hw;
+                ((float*)p.y)[((int64_t)img * p.F + f) * p.hw + n - img * p.hw] = v;
+            }
+        }
+    }
+    if (p.out_kind != LN_OUT_Q) return;
+    __syncthreads();
+    constexpr int B = FMT == LN_F4 ? 16 : 32;
+    const int pix = i / (32 / B), b = i % (32 / B);
+    if (pix >= p.pixels || pix >= 8 * NT) return;
+    float v[B];
+#pragma unroll
+    for (int j = 0; j < B; ++j) v[j] = sums[pix][b * B + j];
+    const int first = f0 + b * B;
+    p.ysf[ln_f4_sf_at(pix, first / (4 * B), p.ysf_words) + first / B % 4] = (uint8_t)store_block<FMT>(v, p.g, p.six_g, (uint8_t*)p.y + pix * p.ys + first / 2);
+}
+int few_launch(ln_ctx* ctx, const ln_f4_conv& c, int64_t pixels) {
+    const ln_tensor &x = *c.x, &y = *c.y;
+    few_params p;
+    p.x = (const uint8_t*)x.ptr; p.xsf = (const uint8_t*)x.sf; p.w = (const uint8_t*)c.w->w; p.wsf = (const uint8_t*)c.w->sf;
+    p.wscale = c.w->wscale; p.bias = c.bias; p.y = y.ptr; p.ysf = (uint8_t*)y.sf;
+    p.xs = x.cstride; p.sf_words = x.sf_words; p.ys = y.dtype == LN_F16 ? y.cstride / 2 : y.cstride; p.ysf_words = y.sf_words;
+    p.pixels = (int)pixels; p.F = (int)y.c; p.chunks = (int)((x.cstride + 63) / 64); p.act = c.act; p.exact = ctx->exact_epilogue; p.out_kind = c.out_kind; p.hw = (int)(y.h * y.w);
+    p.xscale = x.scale; p.g = y.scale; p.six_g = 6.0f * y.scale;
+    const int grid = (int)(ln_round_up(y.c, c.out_kind == LN_OUT_Q ? 64 : 32) / kFewFilters);
+    cudaError_t e;
+    if (c.dtype == LN_F4) e = pixels <= 8 ? ln_f4_launch(ctx, conv_f4_few_kernel<LN_F4, 1>, grid, kFewThreads, 0, p) : ln_f4_launch(ctx, conv_f4_few_kernel<LN_F4, 2>, grid, kFewThreads, 0, p);
+    else e = pixels <= 8 ? ln_f4_launch(ctx, conv_f4_few_kernel<LN_MX4, 1>, grid, kFewThreads, 0, p) : ln_f4_launch(ctx, conv_f4_few_kernel<LN_MX4, 2>, grid, kFewThreads, 0, p);
+    return check_launch(ctx, "ln_conv2d_bias_act_f4", e);
+}
+
 // one launch with 32-bit indexes where every index, and the step behind the last one, stays below 2^31
 #define LN_F4_CALL(KERNEL, FMT, SMALL, GRID, ...) \
     ((FMT) == LN_F4 ? ((SMALL) ? ln_f4_launch(ctx, KERNEL<LN_F4, uint32_t>, GRID, kThreads, 0, __VA_ARGS__) : ln_f4_launch(ctx, KERNEL<LN_F4, int64_t>, GRID, kThreads, 0, __VA_ARGS__)) \
@@ -535,8 +679,9 @@ int32_t ln_conv2d_bias_act_f4(ln_ctx* ctx, const ln_tensor* x, const ln_conv_wei
         c.dtype = x->dtype; c.x = x; c.w = weights; c.bias = (const float*)bias->ptr; c.y = y;
         c.k = (int)kernel_size; c.stride = (int)stride_x; c.pad = (int)padding; c.act = activation; c.out_kind = out_kind;
         if (rc == LN_OK && out_kind == LN_OUT_Q) y->scale = y_scale;
-        if (rc == LN_OK && ln_f4_umma_takes(c, stride_x, stride_y)) {
-            rc = ln_f4_umma_launch(ctx, c);
+        const bool few = kernel_size == 1 && stride_x == 1 && stride_y == 1 && padding == 0 && x->n * oh * ow <= kFewPixels;
+        if (rc == LN_OK && (few || ln_f4_umma_takes(c, stride_x, stride_y))) {
+            rc = few ? few_launch(ctx, c, x->n * oh * ow) : ln_f4_umma_launch(ctx, c);
             if (rc) { ln_tensor_release(y); return rc; }
             *out = y;
             return LN_OK;

@@ -189,6 +189,7 @@ CONV = [
     (300, 1024, 1, 1, 1000, 1, 1, 1, 0), (1, 1, 1, 1, 1, 1, 1, 1, 0), (2, 17, 5, 9, 33, 1, 1, 1, 0), (1, 512, 19, 19, 255, 1, 1, 1, 0), (3, 64, 20, 13, 96, 3, 1, 1, 1),
     (1, 256, 13, 13, 512, 3, 1, 1, 1), (2, 128, 26, 30, 72, 3, 2, 2, 1), (2, 40, 15, 17, 40, 3, 2, 2, 1), (1, 96, 38, 38, 64, 3, 1, 1, 1), (2, 192, 9, 9, 320, 3, 1, 1, 1),
     (1, 33, 8, 9, 70, 5, 1, 1, 2), (1, 70, 11, 12, 50, 3, 1, 2, 1), (2, 48, 7, 7, 24, 3, 3, 3, 0), (1, 64, 3, 3, 64, 5, 1, 1, 0), (1, 48, 2, 2, 16, 3, 2, 2, 0),
+    (8, 192, 1, 1, 40, 1, 1, 1, 0), (9, 4160, 1, 1, 100, 1, 1, 1, 0), (16, 320, 1, 1, 130, 1, 1, 1, 0), (17, 320, 1, 1, 130, 1, 1, 1, 0), (1, 96, 3, 5, 33, 1, 1, 1, 0), (2, 70, 2, 3, 65, 1, 1, 1, 0),
     (150, 64, 1, 1, 24, 1, 1, 1, 0), (131, 80, 1, 1, 40, 1, 1, 1, 0), (260, 64, 1, 1, 257, 1, 1, 1, 0), (4, 64, 1, 130, 130, 1, 2, 2, 0), (2, 80, 6, 10, 48, 2, 2, 2, 0), (1, 128, 30, 30, 128, 1, 2, 2, 0),
 ]
 
