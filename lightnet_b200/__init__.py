@@ -85,7 +85,7 @@ SYMBOLS = {
     "ln_tensor_download_f32": (C.c_int32, [_VP, _VP, _VP, C.c_int64]),
     "ln_tensor_shape": (C.c_int32, [_VP, _I64P]),
     "ln_tensor_dtype": (C.c_int32, [_VP]),
-    "ln_tensor_device_data": (C.c_int32, [_VP, _PP, _I64P, _I64P]),
+    "ln_tensor_device_data": (C.c_int32, [_VP, _VP, _VP, _VP]),
     "ln_tensor_retain": (C.c_int32, [_VP]),
     "ln_tensor_release": (C.c_int32, [_VP]),
     "ln_conv2d_f32": (C.c_int32, [_VP, _VP, _VP, _I64P] + [C.c_int64] * 10 + [_PP]),
@@ -192,6 +192,7 @@ def load_library():
 
 
 _I64x4 = C.c_int64 * 4
+_byref = C.byref
 
 
 def _shape4(shape):
@@ -246,14 +247,15 @@ class Tensor:
         dtype = _lib.ln_tensor_dtype(self.h)
         if dtype != LN_F32 and dtype != LN_F16:
             raise AttributeError("only f32 and binary16 tensors have an array interface")
-        backend, size, p, shape, s = self.backend, 4 if dtype == LN_F32 else 2, C.c_void_p(), _I64x4(), _I64x4()
-        rc = _lib.ln_tensor_device_data(self.h, p, shape, s)
+        backend, size = self.backend, 4 if dtype == LN_F32 else 2
+        view, *parts = backend._view
+        rc = _lib.ln_tensor_device_data(self.h, *parts)
         if rc:
             backend._check(rc)
-        n, c, h, w = s
+        data, *shape, n, c, h, w = view[:]
         self.__cuda_array_interface__ = d = {
-            "shape": tuple(shape), "typestr": "<f4" if size == 4 else "<f2", "data": (p.value, False), "strides": (size * n, size * c, size * h, size * w),
-            "version": 3, "stream": backend.stream}
+            "shape": tuple(shape), "typestr": "<f4" if size == 4 else "<f2", "data": (data, False), "strides": (size * n, size * c, size * h, size * w),
+            "version": 3, "stream": backend._stream}
         return d
 
 
@@ -279,6 +281,9 @@ class B200Backend:
             raise BackendError(rc, self.lib.ln_last_error(None).decode())
         self.ctx = h
         self.device = device
+        self._stream = self.lib.ln_ctx_stream(h)  # (of the context's life)
+        view = (C.c_int64 * 9)()  # what ln_tensor_device_data writes: address, shape, strides
+        self._view = view, C.byref(view), C.byref(view, 8), C.byref(view, 40)
 
     def close(self):
         if getattr(self, "ctx", None):
@@ -291,7 +296,7 @@ class B200Backend:
 
     def _out(self, fn, *args):
         h = C.c_void_p()
-        rc = fn(self.ctx, *args, C.byref(h))
+        rc = fn(self.ctx, *args, _byref(h))
         if rc:
             self._check(rc)
         return Tensor(self, h)
@@ -301,7 +306,7 @@ class B200Backend:
 
     @property
     def stream(self):
-        return self.lib.ln_ctx_stream(self.ctx)
+        return self._stream if self.ctx else None
 
     @property
     def launch_count(self):
