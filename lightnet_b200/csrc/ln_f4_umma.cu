@@ -464,37 +464,50 @@ __global__ void __launch_bounds__(kThreadsF4, 1) f4_umma_kernel(const __grid_con
         __syncwarp();
     } else if (warp < 2 + kGatherWarps) {
         // ------------------------------------------------------------------ scales of the pixels under shifted taps
-        int unit = first_unit, r = 0, s = 0, cb = 0;
-        int iy0[4], ix0[4], img[4];
+        int unit = first_unit, r = 0, s = 0, cb = 0, tap = 0;  // tap: pixels between the tap's and the first one's
+        int iy0[4], ix0[4], q0[4];                             // of the lane's rows under the first tap: place and number of the input pixel
         auto enter_tile = [&]() {
             if (unit >= p.num_units) return;
             const f4_tile t = tile_at(p, unit);
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
-                const int row = g * 32 + lane;
+                const int row = g * 32 + lane, img = t.n0 + (row >> (p.log_tw + p.log_th));
                 ix0[g] = (t.ow0 + (row & (p.TW - 1))) * p.stride - p.pad;
                 iy0[g] = (t.oh0 + ((row >> p.log_tw) & (p.TH - 1))) * p.stride - p.pad;
-                img[g] = t.n0 + (row >> (p.log_tw + p.log_th));
+                q0[g] = (img * p.H + iy0[g]) * p.W + ix0[g];
+                if (img >= p.N) iy0[g] = -(1 << 28);  // (outside under every tap)
             }
         };
         auto advance = [&]() {
             if (++cb < p.cblocks) return;
             cb = 0;
+            ++tap;
             if (++s < p.S) return;
             s = 0;
+            tap += p.W - p.S;
             if (++r < p.R) return;
-            r = 0;
+            r = tap = 0;
             unit += step;
             enter_tile();
         };
+        const size_t group_bytes = (size_t)p.sf_words * 512u;  // of the scales of 128 pixels
         auto fetch = [&](uint32_t (&v)[4][4]) {
+            const uint8_t* base = p.xsf + cb * p.words * 512;
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
-                const int y = iy0[g] + r, x = ix0[g] + s;
-                const bool inside = y >= 0 && y < p.H && x >= 0 && x < p.W && img[g] < p.N;
-                const uint8_t* src = p.xsf + (inside ? ln_f4_sf_at((img[g] * p.H + y) * p.W + x, cb * p.words, p.sf_words) : 0);
+                const bool inside = (unsigned)(iy0[g] + r) < (unsigned)p.H && (unsigned)(ix0[g] + s) < (unsigned)p.W;
+                const unsigned q = (unsigned)(q0[g] + tap);
+                const uint8_t* src = base + (size_t)(q >> 7) * group_bytes + ((q & 31u) * 16u + (q >> 5 & 3u) * 4u);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) v[g][j] = inside && j < p.words ? __ldg((const uint32_t*)(src + 512 * j)) : 0u;
+                for (int j = 0; j < 4; ++j) v[g][j] = 0u;
+                if (inside) {
+                    v[g][0] = __ldg((const uint32_t*)src);
+                    if (p.words > 1) v[g][1] = __ldg((const uint32_t*)(src + 512));
+                    if (FMT == LN_F4 && p.words > 2) {
+                        v[g][2] = __ldg((const uint32_t*)(src + 1024));
+                        v[g][3] = __ldg((const uint32_t*)(src + 1536));
+                    }
+                }
             }
         };
         if (!p.flat) {
