@@ -20,6 +20,7 @@
 // gave the same 64 us on 8192 x 4096 x 4096: a tcgen05.cp of a pair takes its thread 50 cycles and more, and twelve go with four instructions.
 // Every wait is bounded (see ln_umma.h).
 #include <cstdlib>
+#include <type_traits>
 
 #include "ln_f4.h"
 #include "ln_umma.h"
@@ -407,7 +408,6 @@ __global__ void __launch_bounds__(kThreadsF4, 1) f4_umma_kernel(const __grid_con
             // E2M1 operands (bits 7, 10: type 1), N / 8, scale type (bit 23: 1 = E8M0), M / 128, K-major; the scale ids go to bits 4 and 29
             const uint32_t idesc = (1u << 7) | (1u << 10) | ((uint32_t)(p.bn >> 3) << 17) | ((FMT == LN_MX4 ? 1u : 0u) << 23) | (1u << 27);
             const uint64_t desc_base = make_smem_desc(0u, p.bk);
-            constexpr int kWords = FMT == LN_MX4 ? 2 : 4;  // of a whole k-block
             const uint64_t sfa_desc = scale_desc(p.off_sfa), sfb_desc = scale_desc(p.off_sfb);
             int stage = 0, t = 0;
             uint32_t phase = 0, set = 0;
@@ -427,9 +427,10 @@ __global__ void __launch_bounds__(kThreadsF4, 1) f4_umma_kernel(const __grid_con
                     const uint32_t sfa = tmem_base + kScaleCols + set * kScaleSet, sfb = sfa + kScaleB;
                     const int left = p.cstride - c0, n = (left < p.bk ? left : p.bk) >> 5;  // instructions of this k-block
                     const uint64_t a_desc = desc_base + (at >> 4), b_desc = desc_base + ((at + p.off_b) >> 4);
-                    if (n == 4) {
-                        // a whole k-block of 128 bytes, unrolled with constant offsets: as loops with run-time bounds the copies and
-                        // instructions of a k-block took their thread 1100 cycles, this way 390, less than the 530 that they run for
+                    // Unrolled with constant offsets: as loops with run-time bounds the copies and instructions of a k-block of 128 bytes took
+                    // their thread 1100 cycles, this way under 200, less than the 530 that they run for.
+                    auto issue = [&](auto most, bool whole) {  // instructions of a whole k-block: 4, 2 or 1; the channels' last one may have fewer
+                        constexpr int kN = decltype(most)::value, kWords = FMT == LN_MX4 ? (kN + 1) / 2 : kN;
 #pragma unroll
                         for (int j = 0; j < kWords; ++j) {
                             tc_copy_scales(sfa + 4u * j, sfa_desc + ((at + 512u * j) >> 4));
@@ -437,20 +438,14 @@ __global__ void __launch_bounds__(kThreadsF4, 1) f4_umma_kernel(const __grid_con
                             for (int b = 0; b < WBLOCKS; ++b) tc_copy_scales(sfb + 4u * (j * WBLOCKS + b), sfb_desc + ((at + 512u * (b * kWords + j)) >> 4));
                         }
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
+                        for (int i = 0; i < kN; ++i) {
                             const uint32_t word = FMT == LN_MX4 ? i >> 1 : i, id = FMT == LN_MX4 ? (uint32_t)(i & 1) * 2u : 0u;
-                            tc_mma_scaled<FMT>(d, a_desc + 2u * i, b_desc + 2u * i, idesc | (id << 4) | (id << 29), sfa + 4u * word, sfb + 4u * word * WBLOCKS + shift, i ? 1u : (uint32_t)(kb != 0));
+                            if (whole || i < n) tc_mma_scaled<FMT>(d, a_desc + 2u * i, b_desc + 2u * i, idesc | (id << 4) | (id << 29), sfa + 4u * word, sfb + 4u * word * WBLOCKS + shift, i ? 1u : (uint32_t)(kb != 0));
                         }
-                    } else {
-                        for (int j = 0; j < p.words; ++j) {
-                            tc_copy_scales(sfa + 4u * j, sfa_desc + ((at + 512u * j) >> 4));
-                            for (int b = 0; b < WBLOCKS; ++b) tc_copy_scales(sfb + 4u * (j * WBLOCKS + b), sfb_desc + ((at + 512u * (b * p.words + j)) >> 4));
-                        }
-                        for (int i = 0; i < n; ++i) {
-                            const uint32_t word = FMT == LN_MX4 ? i >> 1 : i, id = FMT == LN_MX4 ? (uint32_t)(i & 1) * 2u : 0u;
-                            tc_mma_scaled<FMT>(d, a_desc + 2u * i, b_desc + 2u * i, idesc | (id << 4) | (id << 29), sfa + 4u * word, sfb + 4u * word * WBLOCKS + shift, (uint32_t)((kb | i) != 0));
-                        }
-                    }
+                    };
+                    if (p.bk == 128) { if (n == 4) issue(std::integral_constant<int, 4>(), true); else issue(std::integral_constant<int, 4>(), false); }
+                    else if (p.bk == 64) issue(std::integral_constant<int, 2>(), false);
+                    else issue(std::integral_constant<int, 1>(), true);
                     tc_commit(empty_bar(stage));
                     set ^= 1u;
                     c0 += p.bk;
