@@ -341,9 +341,9 @@ __global__ void conv_f4_simt_kernel(const simt_params p) {
                             sum = __fmaf_rn(u.y, v.y, sum);
                         }
                     }
-                    // (block scales first: their product is exact for LN_F4, and a sum of zero times it is never zero times infinity)
+                    // (block scales first: their product is exact for LN_F4; those of LN_MX4 need the range of 64 bits)
                     if (FMT == LN_F4) acc = __fmaf_rn(sum, __fmul_rn(ln_e4m3_value(p.xsf[xat]), ln_e4m3_value(p.wsf[at])), acc);
-                    else acc = __fmaf_rn(__fmul_rn(sum, ln_e8m0_value(p.xsf[xat])), ln_e8m0_value(p.wsf[at]), acc);
+                    else acc += __double2float_rn((double)sum * ((double)ln_e8m0_value(p.xsf[xat]) * (double)ln_e8m0_value(p.wsf[at])));
                 }
             }
         }
@@ -387,7 +387,8 @@ __device__ __forceinline__ void few_operand(const uint4& q, uint32_t scale, uint
             }
         }
     } else {
-        const float s = ln_e8m0_value(scale);
+        // (a quarter of the values: 6 * 2^126, a saturated infinity, is more than 16 bits hold; the sums are multiplied by 16)
+        const float s = 0.25f * ln_e8m0_value(scale);
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[i]));
@@ -459,7 +460,7 @@ __global__ void __launch_bounds__(kFewThreads) conv_f4_few_kernel(const few_para
         for (int k = 0; k < kFewThreads / 32; ++k) sum += part[k][i & 31][n];
         float v = 0.0f;
         if (f < p.F) {
-            v = __fmaf_rn(sum, __fmul_rn(p.xscale, p.wscale[f]), p.bias[f]);
+            v = __fmaf_rn(sum, FMT == LN_F4 ? __fmul_rn(p.xscale, p.wscale[f]) : 16.0f, p.bias[f]);
             v = p.exact ? ln_epilogue_act<true>(p.act, v) : ln_epilogue_act<false>(p.act, v);
         }
         if (p.out_kind == LN_OUT_Q) sums[n][i & 31] = v;
@@ -618,6 +619,8 @@ int32_t ln_conv_weights_f4(ln_ctx* ctx, const ln_tensor* weights_f32, int64_t fi
     if (weights_f32->dtype != LN_F32) return ln_fail(ctx, LN_ERR_ARG, "%s: f32 weights required", who);
     if (weights_f32->ctx != ctx) return ln_fail(ctx, LN_ERR_ARG, "%s: the tensor belongs to another context", who);
     if (!ln_is_f4(dtype)) return ln_fail(ctx, LN_ERR_ARG, "%s: dtype must be LN_F4 or LN_MX4", who);
+    if (channels > 0 && kernel_size > 0 && kernel_size <= 64 && channels <= (1 << 24) && channels * kernel_size * kernel_size >= (1ll << 31))
+        return ln_fail(ctx, LN_ERR_UNSUPPORTED, "%s: a filter has 2^31 weights or more", who);
     if (filters < 1 || channels < 1 || kernel_size < 1 || filters > (1 << 24) || channels > (1 << 24) || kernel_size > 64 || weights_f32->count() != filters * channels * kernel_size * kernel_size)
         return ln_fail(ctx, LN_ERR_SHAPE, "%s: weight tensor has %lld elements, expected %lld x %lld x %lld x %lld", who, (long long)weights_f32->count(), (long long)filters, (long long)channels,
                        (long long)kernel_size, (long long)kernel_size);

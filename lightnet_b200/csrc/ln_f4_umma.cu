@@ -636,10 +636,12 @@ int ln_f4_umma_launch(ln_ctx* ctx, const ln_f4_conv& c) {
     p.flat = flat ? 1 : 0;
     p.tiles_f = (p.F + p.bn - 1) / p.bn; p.tiles_w = (p.OW + p.TW - 1) / p.TW; p.tiles_h = (p.OH + p.TH - 1) / p.TH;
     const int64_t num_units = best * p.tiles_f;
-    if (num_units >= (1 << 19)) return ln_fail(ctx, LN_ERR_UNSUPPORTED, "%s: %lld tiles", who, (long long)num_units);
+    // fast_div(n, d) is exact for n < 2^24 and n d < 2^40; a magic number of 0 is a quotient of 0, for the pixels of one row of tiles
+    const int most = p.tiles_f > p.tiles_h ? p.tiles_f : p.tiles_h, row = flat ? 1 : p.tiles_w;
+    if (num_units >= (1 << 24) || num_units * (most > row ? most : row) >= (1ll << 40)) return ln_fail(ctx, LN_ERR_UNSUPPORTED, "%s: %lld tiles", who, (long long)num_units);
     p.num_units = (int)num_units;
     auto magic = [](int d) { return ((1ull << 40) + (unsigned long long)d - 1) / (unsigned long long)d; };
-    p.magic_f = magic(p.tiles_f); p.magic_w = magic(p.tiles_w); p.magic_h = magic(p.tiles_h);
+    p.magic_f = magic(p.tiles_f); p.magic_w = flat ? 0 : magic(p.tiles_w); p.magic_h = magic(p.tiles_h);
     p.off_b = 128u * p.bk;
     p.off_sfa = p.off_b + (uint32_t)p.bn * p.bk;
     p.off_sfb = p.off_sfa + (uint32_t)p.words * 512u;

@@ -283,6 +283,60 @@ def test_nan_and_infinity_in_a_product(be, dtype):
         assert np.isfinite(y[:, :, ~nan & ~near]).all()
 
 
+@pytest.mark.parametrize("tile", ["64", "128", "256"])
+@pytest.mark.parametrize("dtype", FMT)
+def test_each_tile_of_filters(be, monkeypatch, dtype, tile):
+    """Whatever a size would choose: outputs of all kinds, several tiles per SM, filters that end inside a tile."""
+    monkeypatch.setenv("LN_F4_BN", tile)
+    for case in ((1, 512, 19, 19, 255, 1, 1, 1, 0), (131, 80, 1, 1, 40, 1, 1, 1, 0), (300, 1024, 1, 1, 1000, 1, 1, 1, 0), (2, 192, 9, 9, 320, 3, 1, 1, 1), (2, 128, 26, 30, 72, 3, 2, 2, 1),
+                 (3, 70, 120, 119, 136, 1, 1, 1, 0), (2, 40, 75, 77, 300, 3, 1, 1, 1)):
+        y, ref, bound = run_conv(be, case, dtype, "mish", ln.LN_OUT_F32)
+        wide = be.download_f32(y)
+        assert np.max(np.abs(wide - ref) / bound) <= 1, case
+        y, ref, bound = run_conv(be, case, dtype, "mish", ln.LN_OUT_F16)
+        assert np.array_equal(be.download_f16(y), wide.astype(np.float16).astype(np.float32)), case
+        ys = 1.0 if dtype == ln.LN_MX4 else 0.25
+        q, _, _ = run_conv(be, case, dtype, "mish", ln.LN_OUT_Q, y_scale=ys)
+        assert np.array_equal(be.download_f32(be.widen_f4(q)), narrow(wide, dtype, ys)[2].astype(np.float32)), case
+
+
+@pytest.mark.parametrize("case", [(2, 256, 1, 1, 48, 1, 1, 1, 0), (40, 256, 1, 1, 48, 1, 1, 1, 0), (1, 96, 9, 10, 48, 3, 1, 1, 1), (1, 96, 9, 10, 48, 3, 1, 2, 1)])
+def test_the_range_of_power_of_two_scales(be, case):
+    """LN_MX4 holds values of the whole range of binary32: blocks of very large and very small ones against weights of the other end."""
+    n, c, h, w, f, k, sx, sy, pad = case
+    rng = np.random.default_rng(sum(case))
+    bias = np.zeros(f, np.float32)
+    for px, pw in ((127, -40), (120, -120), (-122, 100), (-127, 126)):
+        x = np.ldexp(rng.uniform(0.5, 1, (n, c, h, w)) * rng.choice([-1, 1], (n, c, h, w)), px - rng.integers(0, 4, (n, c, h, w))).astype(np.float32)
+        wt = np.ldexp(rng.uniform(0.5, 1, (f, c, k, k)) * rng.choice([-1, 1], (f, c, k, k)), pw).astype(np.float32)
+        q, packed = be.narrow_f4(be.upload_f32(x.shape, x), 1.0, ln.LN_MX4), be.conv_weights_f4(be.upload_f32(wt.shape, wt), f, c, k, ln.LN_MX4)
+        oh, ow = (h + 2 * pad - k) // sy + 1, (w + 2 * pad - k) // sx + 1
+        got = be.download_f32(be.conv2d_bias_act_f4(q, packed, be.upload_f32((1, f, 1, 1), bias), (n, f, oh, ow), c, h, w, f, k, sx, sy, 1, pad, 1, "linear", 1.0, ln.LN_OUT_F32))
+        xv, wv = narrow(x, ln.LN_MX4, 1.0)[2], narrow(wt, ln.LN_MX4, np.ones(f))[2]
+        ref, size = conv64(xv, wv, k, sx, sy, pad), conv64(np.abs(xv), np.abs(wv), k, sx, sy, pad)
+        assert np.max(np.abs(got - ref) / (1.1 * (c * k * k / 64 + 8) * 2.0 ** -23 * size)) <= 1, (px, pw)
+
+
+def test_more_tiles_than_any_network(be):
+    """2^26 pixels and more: indexes of tiles, codes and scales at that size."""
+    h, w, s = 8192, 8200, 64
+    rng = np.random.default_rng(8)
+    for dtype in FMT:
+        x = rng.integers(-6, 7, (1, 1, h, w)).astype(np.float32)
+        g = 1.0
+        q = be.narrow_f4(be.upload_f32(x.shape, x), g, dtype)
+        one, three = np.full((1, 1, 1, 1), 1.5, np.float32), rng.integers(-4, 5, (1, 1, 3, 3)).astype(np.float32)
+        gw = 1.0 if dtype == ln.LN_MX4 else f32(np.abs(three).max((1, 2, 3)).astype(np.float64) / 2688)
+        value = narrow(x[:, :, -s:], dtype, g)[2]
+        assert np.array_equal(be.download_f32(be.widen_f4(q))[:, :, -s:], value)
+        b = be.zeros_f32((1, 1, 1, 1))
+        y = be.download_f32(be.conv2d_bias_act_f4(q, be.conv_weights_f4(be.upload_f32(one.shape, one), 1, 1, 1, dtype), b, x.shape, 1, h, w, 1, 1, 1, 1, 1, 0, 1, "linear", 1.0, ln.LN_OUT_F32))
+        assert np.allclose(y[:, :, -s:], value * 1.5, rtol=2.0 ** -21, atol=0)
+        y = be.download_f32(be.conv2d_bias_act_f4(q, be.conv_weights_f4(be.upload_f32(three.shape, three), 1, 1, 3, dtype), b, x.shape, 1, h, w, 1, 3, 1, 1, 1, 1, 1, "linear", 1.0, ln.LN_OUT_F32))
+        ref = conv64(value, narrow(three, dtype, gw)[2], 3, 1, 1, 1)[:, :, 1:]
+        assert np.max(np.abs(y[:, :, 1 - s:] - ref)) <= 1.1 * 9 * 2.0 ** -23 * 9 * 6 * 4.0
+
+
 def test_operators_together(be):
     """binary16 map -> 4 bits -> 1x1 -> 4 bits -> 3x3 -> binary16, twice on the same handles and again after other work: the same bits."""
     n, c, h, w, f = 2, 128, 20, 20, 64
@@ -328,6 +382,82 @@ def test_images_do_not_depend_on_the_batch(be):
             assert np.allclose(product(x[lo:hi]), whole[lo:hi], rtol=0, atol=2.0 ** -20 * np.abs(whole).max())
 
 
+def test_captured_and_replayed(be):
+    """The operators on the backend's stream inside a captured graph: replays see what the input holds then."""
+    torch = pytest.importorskip("torch")
+    n, c, h, w, f = 2, 96, 14, 14, 72
+    rng = np.random.default_rng(31)
+    stream = torch.cuda.ExternalStream(be.stream)
+    for dtype in FMT:
+        g = 1.0 if dtype == ln.LN_MX4 else float(np.float32(5 / 2688))
+        x = [rng.normal(0, 1, (n, c, h, w)).astype(np.float32) for _ in range(3)]
+        w1, w2 = rng.normal(0, 0.1, (f, c, 1, 1)).astype(np.float32), rng.normal(0, 0.05, (f, f, 3, 3)).astype(np.float32)
+        t = be.upload_f32(x[0].shape, x[0])
+        p1, p2, b = be.conv_weights_f4(be.upload_f32(w1.shape, w1), f, c, 1, dtype), be.conv_weights_f4(be.upload_f32(w2.shape, w2), f, f, 3, dtype), be.zeros_f32((1, f, 1, 1))
+
+        def chain():
+            q = be.narrow_f4(t, g, dtype)
+            y = be.conv2d_bias_act_f4(q, p1, b, (n, f, h, w), c, h, w, f, 1, 1, 1, 1, 0, 1, "leaky", g, ln.LN_OUT_Q)
+            z = be.conv2d_bias_act_f4(y, p2, b, (n, f, h, w), f, h, w, f, 3, 1, 1, 1, 1, 1, "mish", g, ln.LN_OUT_Q)
+            return q, y, z, be.widen_f4(z)
+
+        want = []
+        for v in x:
+            t_view = torch.as_tensor(t, device="cuda")
+            be.sync()
+            t_view.copy_(torch.from_numpy(v))
+            torch.cuda.synchronize()
+            want.append(be.download_f32(chain()[3]))
+        be.sync()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            kept = chain()  # (its memory comes from what the chains above gave back)
+        for i in (1, 2, 0):
+            t_view.copy_(torch.from_numpy(x[i]))
+            torch.cuda.synchronize()
+            with torch.cuda.stream(stream):
+                graph.replay()
+                graph.replay()
+            assert np.array_equal(be.download_f32(kept[3]), want[i])
+        be.sync()
+        del graph
+
+
+def test_two_backends_at_once():
+    """Two threads, a context each: the same bits as one after the other."""
+    import threading
+    rng = np.random.default_rng(41)
+    n, c, h, w, f = 3, 128, 26, 26, 160
+    x = [rng.normal(0, 1, (n, c, h, w)).astype(np.float32) for _ in range(2)]
+    wt = rng.normal(0, 0.05, (f, c, 3, 3)).astype(np.float32)
+    bes = [ln.B200Backend(0) for _ in range(2)]
+    try:
+        def work(i, rounds):
+            be, out = bes[i], []
+            packed, b = be.conv_weights_f4(be.upload_f32(wt.shape, wt), f, c, 3, FMT[i]), be.zeros_f32((1, f, 1, 1))
+            for _ in range(rounds):
+                q = be.narrow_f4(be.upload_f32(x[i].shape, x[i]), 1.0, FMT[i])
+                out.append(be.download_f32(be.conv2d_bias_act_f4(q, packed, b, (n, f, h, w), c, h, w, f, 3, 1, 1, 1, 1, 1, "swish", 1.0, ln.LN_OUT_F32)))
+            return out
+
+        alone = [work(i, 1)[0] for i in range(2)]
+        got = [None, None]
+
+        def run(i):
+            got[i] = work(i, 20)
+
+        threads = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+        for i in range(2):
+            assert got[i] is not None and all(np.array_equal(y, alone[i]) for y in got[i])
+    finally:
+        for b in bes:
+            b.close()
+
+
 def test_array_interface_shares_the_memory(be):
     torch = pytest.importorskip("torch")
     x = np.random.default_rng(1).normal(0, 1, (2, 37, 3, 5)).astype(np.float32)
@@ -371,6 +501,7 @@ def test_refusals(be):
     wt = be.upload_f32((8, 32, 3, 3), np.ones((8, 32, 3, 3), np.float32))
     refused("shape", be.conv_weights_f4, wt, 8, 32, 1)
     refused("shape", be.conv_weights_f4, wt, 0, 32, 3)
+    refused("unsupported", be.conv_weights_f4, wt, 1, 1 << 24, 64)
     refused("argument", be.conv_weights_f4, wt, 8, 32, 3, ln.LN_F8)
     refused("argument", be.conv_weights_f4, q, 8, 32, 3)
     w, wm = be.conv_weights_f4(wt, 8, 32, 3), be.conv_weights_f4(wt, 8, 32, 3, ln.LN_MX4)
