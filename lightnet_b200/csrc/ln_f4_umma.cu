@@ -15,11 +15,14 @@
 // of four that take the units of 32 columns of the tiles in turn.  TMEM: 416 columns of accumulators, 2 x 48 of scales.  Three tiles of
 // 128 filters or six of 64 fit; two of 256 overlap by 96 columns (0..255 and 160..415), so their epilogue reads the four units that hold
 // the overlap first, and the next tile starts when those have been read.
+// The last round of tiles, where it would leave SMs idle, is cut into units of fewer filters; each is the last one of its CTA, so nothing
+// waits for its accumulator to be free.
 // What bounds it: large k ranges the way from L2 to shared memory (54 KB per k-block of 256 filters at 64 bytes a cycle are 844 cycles, the
 // instructions take 528; measured 830), short ones the epilogue.  CTA pairs (cta_group::2, half of the filters' codes per CTA) were built and
 // gave the same 64 us on 8192 x 4096 x 4096: a tcgen05.cp of a pair takes its thread 50 cycles and more, and twelve go with four instructions.
 // Every wait is bounded (see ln_umma.h).
 #include <cstdlib>
+#include <cstring>
 #include <type_traits>
 
 #include "ln_f4.h"
@@ -39,7 +42,7 @@ constexpr int kMaxSmemF4 = 227 * 1024;
 constexpr size_t kLeastSmemF4 = 118 * 1024;
 
 struct f4_params {
-    CUtensorMap tmA[4], tmB, tmXS, tmWS;  // codes of pixels and filters; their scales as rows of 512 bytes
+    CUtensorMap tmA[4], tmB[2], tmXS, tmWS;  // codes of pixels and filters (whole tiles, narrow ones); their scales as rows of 512 bytes
     const uint8_t* xsf;
     const float *wscale, *bias;
     void* y;
@@ -51,6 +54,7 @@ struct f4_params {
     int bk, bn, cblocks, words;
     int R, S, stride, pad, H, W, N, OH, OW, F, hw;
     int TW, TH, TN, log_tw, log_th, tiles_f, tiles_w, tiles_h, num_units;  // units: pixel tiles x filter tiles
+    int whole, log_split, narrow;  // the tiles behind the first `whole` are cut into 2^log_split units of `narrow` filters
     unsigned long long magic_f, magic_w, magic_h;
     int stages, nbuf, acc_step, subs, act, exact, flat;
     uint32_t off_b, off_sfa, off_sfb, stage_bytes;
@@ -139,15 +143,23 @@ __device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[32]) { tme
 __device__ __forceinline__ void store_32(uint8_t* dst, const uint32_t (&v)[8]) {  // a whole sector
     asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
 }
-// the place of a tile: output box origin and first filter
-struct f4_tile {
-    int ow0, oh0, n0, f0;
+// what a unit is: pixels and filters, and the output box's origin
+struct f4_unit {
+    int pixel_tile, f0;
 };
-__device__ __forceinline__ f4_tile tile_at(const f4_params& p, int unit) {
-    const int q1 = fast_div(unit, p.magic_f), tf = unit - q1 * p.tiles_f;
+__device__ __forceinline__ f4_unit unit_at(const f4_params& p, int unit) {
+    const int v = unit - p.whole, tile = v < 0 ? unit : p.whole + (v >> p.log_split);
+    const int pixel_tile = fast_div(tile, p.magic_f), f0 = (tile - pixel_tile * p.tiles_f) * p.bn;
+    return {pixel_tile, v < 0 ? f0 : f0 + (v & ((1 << p.log_split) - 1)) * p.narrow};
+}
+struct f4_box {
+    int ow0, oh0, n0;
+};
+__device__ __forceinline__ f4_box box_at(const f4_params& p, int unit) {
+    const int q1 = unit_at(p, unit).pixel_tile;
     const int q2 = fast_div(q1, p.magic_w), tw = q1 - q2 * p.tiles_w;
     const int tn = fast_div(q2, p.magic_h), th = q2 - tn * p.tiles_h;
-    return {tw * p.TW, th * p.TH, tn * p.TN, tf * p.bn};
+    return {tw * p.TW, th * p.TH, tn * p.TN};
 }
 
 // what the epilogue shares with the other roles: shared addresses of its table and barriers
@@ -171,19 +183,21 @@ __device__ __forceinline__ void f4_epilogue(const f4_params& p, const f4_epilogu
     // epilogue (measured 2400).
     constexpr bool scaled = FMT == LN_F4;
     float wscale = 0.0f, bias = 0.0f;
-    int unit = first_unit, order = group, buf = 0, pixel_tile = 0, f0 = 0;  // of the next unit
+    int unit = first_unit, order = group, buf = 0, pixel_tile = 0, col = 0, f0 = 0;  // of the next unit
     uint32_t phase = 0;
     auto settle = [&]() {  // units beyond the tile's: the next tiles
-        while (order >= p.subs) {
-            order -= p.subs;
+        while (unit < p.num_units && order >= (unit < p.whole ? p.subs : p.narrow / CH)) {
+            order -= p.subs;  // (nothing follows a narrow unit)
             unit += step;
             if (++buf == p.nbuf) { buf = 0; phase ^= 1u; }
         }
     };
     auto prefetch = [&]() {
         if (unit >= p.num_units) return;
-        pixel_tile = fast_div(unit, p.magic_f);
-        f0 = (unit - pixel_tile * p.tiles_f) * p.bn + (overlap && buf == 0 ? order ^ 4 : order) * CH;  // (what overlaps the other accumulator first)
+        const f4_unit u = unit_at(p, unit);
+        pixel_tile = u.pixel_tile;
+        col = (overlap && buf == 0 && unit < p.whole ? order ^ 4 : order) * CH;  // (what overlaps the other accumulator first)
+        f0 = u.f0 + col;
         const int f = f0 + lane;
         wscale = bias = 0.0f;
         if (f >= p.F) return;
@@ -195,7 +209,7 @@ __device__ __forceinline__ void f4_epilogue(const f4_params& p, const f4_epilogu
     bool ok = true;
     while (unit < p.num_units) {
         const int this_f0 = f0, this_buf = buf;
-        const uint32_t this_phase = phase, taddr = e.tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(this_buf * p.acc_step + (overlap && buf == 0 ? order ^ 4 : order) * CH);
+        const uint32_t this_phase = phase, taddr = e.tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(this_buf * p.acc_step + col);
         const bool first = order < 4;
         int pix = pixel_tile * 128 + row;  // (of a valid row below 2^30)
         bool valid = pix < p.OW;
@@ -356,7 +370,7 @@ __global__ void __launch_bounds__(kThreadsF4, 1) f4_umma_kernel(const __grid_con
             uint32_t phase = 0;
             bool ok = true;
             for (int unit = first_unit; ok && unit < p.num_units; unit += step) {
-                const f4_tile t = tile_at(p, unit);
+                const f4_box t = box_at(p, unit);
                 int sf_row = (t.ow0 >> 7) * kblocks * p.words;  // (flat)
                 for (int r = 0; ok && r < p.R; ++r)
                     for (int s = 0; ok && s < p.S; ++s) {
@@ -382,18 +396,19 @@ __global__ void __launch_bounds__(kThreadsF4, 1) f4_umma_kernel(const __grid_con
     } else if (warp == 6) {
         // ------------------------------------------------------------------ loads of the weights
         if (elect_one()) {
-            const uint32_t bytes = (uint32_t)p.bn * p.bk + WBLOCKS * (uint32_t)p.words * 512u;
             int stage = 0;
             uint32_t phase = 0;
             bool ok = true;
             for (int unit = first_unit; ok && unit < p.num_units; unit += step) {
-                const int f0 = (unit - fast_div(unit, p.magic_f) * p.tiles_f) * p.bn;
+                const int f0 = unit_at(p, unit).f0;
+                const CUtensorMap* codes = &p.tmB[unit < p.whole ? 0 : 1];
+                const uint32_t bytes = (uint32_t)(unit < p.whole ? p.bn : p.narrow) * p.bk + WBLOCKS * (uint32_t)p.words * 512u;
                 int col = 0, c0 = 0;  // first byte of the tap, of the k-block inside it
                 for (int kb = 0; kb < kblocks; ++kb) {
                     if (!(ok = mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag, p.status, LN_STATUS_PRODUCER_TIMEOUT))) break;
                     const uint32_t at = smem_base + (uint32_t)stage * p.stage_bytes, bar = full_bar(stage);
                     mbar_arrive_expect_tx(bar, bytes);
-                    tma_load_2d(at + p.off_b, &p.tmB, col + c0, f0, bar);
+                    tma_load_2d(at + p.off_b, codes, col + c0, f0, bar);
                     tma_load_3d(at + p.off_sfb, &p.tmWS, 0, kb * p.words, f0 >> 7, bar);
                     c0 += p.bk;
                     if (c0 >= p.cstride) { c0 = 0; col += p.cstride; }
@@ -406,7 +421,7 @@ __global__ void __launch_bounds__(kThreadsF4, 1) f4_umma_kernel(const __grid_con
         // ------------------------------------------------------------------ instructions
         if (elect_one()) {
             // E2M1 operands (bits 7, 10: type 1), N / 8, scale type (bit 23: 1 = E8M0), M / 128, K-major; the scale ids go to bits 4 and 29
-            const uint32_t idesc = (1u << 7) | (1u << 10) | ((uint32_t)(p.bn >> 3) << 17) | ((FMT == LN_MX4 ? 1u : 0u) << 23) | (1u << 27);
+            const uint32_t idesc_base = (1u << 7) | (1u << 10) | ((FMT == LN_MX4 ? 1u : 0u) << 23) | (1u << 27);
             const uint64_t desc_base = make_smem_desc(0u, p.bk);
             const uint64_t sfa_desc = scale_desc(p.off_sfa), sfb_desc = scale_desc(p.off_sfb);
             int stage = 0, t = 0;
@@ -418,8 +433,8 @@ __global__ void __launch_bounds__(kThreadsF4, 1) f4_umma_kernel(const __grid_con
                 if (overlap && t > 0 && !(ok = mbar_wait(early_bar(buf ^ 1), (uint32_t)(((t - 1) >> 1) & 1), abort_flag, p.status, LN_STATUS_MMA_TIMEOUT))) break;
                 tc_fence_after();
                 const uint32_t d = tmem_base + (uint32_t)(buf * p.acc_step);
-                const int tf = unit - fast_div(unit, p.magic_f) * p.tiles_f;
-                const uint32_t shift = (uint32_t)((tf * p.bn & 127) >> 5);  // first column of the tile's filters inside their group of 128
+                const uint32_t idesc = idesc_base | ((uint32_t)((unit < p.whole ? p.bn : p.narrow) >> 3) << 17);
+                const uint32_t shift = (uint32_t)((unit_at(p, unit).f0 & 127) >> 5);  // first column of the tile's filters inside their group of 128
                 int c0 = 0;
                 for (int kb = 0; kb < kblocks; ++kb) {
                     if (!(ok = mbar_wait(full_bar(stage), phase, abort_flag, p.status, LN_STATUS_MMA_TIMEOUT))) break;
@@ -463,7 +478,7 @@ __global__ void __launch_bounds__(kThreadsF4, 1) f4_umma_kernel(const __grid_con
         int iy0[4], ix0[4], q0[4];                             // of the lane's rows under the first tap: place and number of the input pixel
         auto enter_tile = [&]() {
             if (unit >= p.num_units) return;
-            const f4_tile t = tile_at(p, unit);
+            const f4_box t = box_at(p, unit);
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
                 const int row = g * 32 + lane, img = t.n0 + (row >> (p.log_tw + p.log_th));
@@ -615,19 +630,30 @@ int ln_f4_umma_launch(ln_ctx* ctx, const ln_f4_conv& c) {
     // A launch takes about start + (k-blocks of a tile + (rounds - 1) x the longer of k-blocks and epilogue), rounds = tiles per SM, in ns
     // as measured over 27 shapes of both types with binary16 output (leaky), 3 to 76 us, each with every tile; the choice was the best one or
     // within 4 % of it on all of them.  Where most SMs have nothing to do, a k-block of 256 filters comes faster.
-    const int64_t kblocks = (int64_t)c.k * c.k * kb.cblocks;
+    // The tiles of the last, partly filled round may be cut into units of fewer filters, where those fit into one round.
+    const int64_t kblocks = (int64_t)c.k * c.k * kb.cblocks, sms = ctx->sm_count;
     const int cand[3] = {256, 128, 64}, start[3] = {5400, 3650, 3300}, out[3] = {3300, 1750, 900}, flat_k[3] = {490, 360, 320}, tap_k[3] = {640, 520, 420};
     int64_t least = -1;
     const bool rows = c.out_kind == LN_OUT_F32 && flat && p.hw == 1 && p.F % 8 != 0;  // (their way through shared memory leaves no four stages of the widest tile)
-    for (int i = rows ? 1 : 0; i < 3; ++i) {
-        const int64_t units = best * ((p.F + cand[i] - 1) / cand[i]), rounds = (units + ctx->sm_count - 1) / ctx->sm_count;
-        const int64_t chain = kblocks * (!flat ? tap_k[i] : (i == 0 && 2 * units <= ctx->sm_count ? 330 : flat_k[i]));
-        const int64_t cost = start[i] + chain + (rounds - 1) * (chain > out[i] ? chain : out[i]);
-        if (least < 0 || cost < least) { least = cost; p.bn = cand[i]; }
+    int force = 0, force_narrow = 0;
+    if (const char* e = getenv("LN_F4_BN")) {  // (A/B measurements: another filter tile, "256/64": with the last round in units of 64)
+        force = atoi(e);
+        if (const char* slash = strchr(e, '/')) force_narrow = atoi(slash + 1);
+        if ((force != 256 || rows) && force != 128 && force != 64) force = 0;
     }
-    if (const char* e = getenv("LN_F4_BN")) {  // (A/B measurements: another filter tile)
-        for (int bn : cand)
-            if (atoi(e) == bn && !(rows && bn == 256)) p.bn = bn;
+    for (int i = rows ? 1 : 0; i < 3; ++i) {
+        if (force && cand[i] != force) continue;
+        const int64_t tiles = best * ((p.F + cand[i] - 1) / cand[i]), rounds = (tiles + sms - 1) / sms, rest = tiles % sms;
+        const int64_t chain = kblocks * (!flat ? tap_k[i] : (i == 0 && 2 * tiles <= sms ? 330 : flat_k[i])), round = chain > out[i] ? chain : out[i];
+        for (int j = i; j < 3; ++j) {
+            if (j > i && (rounds == 1 || rest == 0 || rest * (cand[i] / cand[j]) > sms)) continue;
+            const int64_t tail = kblocks * (flat ? flat_k[j] : tap_k[j]);
+            int64_t cost = start[j] + chain + (rounds - 1) * round;
+            if (j > i) cost += (tail > out[i] ? tail : out[i]) - round;
+            if (force && force_narrow == cand[j]) cost = 0;
+            if (force && !force_narrow && j > i) continue;
+            if (least < 0 || cost < least) { least = cost; p.bn = cand[i]; p.narrow = cand[j]; }
+        }
     }
     const int wblocks = p.bn > 128 ? 2 : 1;
     p.nbuf = p.bn == 256 ? 2 : (int)kScaleCols / p.bn;
@@ -635,11 +661,14 @@ int ln_f4_umma_launch(ln_ctx* ctx, const ln_f4_conv& c) {
     p.subs = p.bn / CH;
     p.flat = flat ? 1 : 0;
     p.tiles_f = (p.F + p.bn - 1) / p.bn; p.tiles_w = (p.OW + p.TW - 1) / p.TW; p.tiles_h = (p.OH + p.TH - 1) / p.TH;
-    const int64_t num_units = best * p.tiles_f;
+    const int64_t tiles = best * p.tiles_f;
+    p.log_split = log2_of(p.bn / p.narrow);
+    const int64_t cut = p.log_split ? tiles % sms : 0, num_units = tiles - cut + (cut << p.log_split);
     // fast_div(n, d) is exact for n < 2^24 and n d < 2^40; a magic number of 0 is a quotient of 0, for the pixels of one row of tiles
     const int most = p.tiles_f > p.tiles_h ? p.tiles_f : p.tiles_h, row = flat ? 1 : p.tiles_w;
     if (num_units >= (1 << 24) || num_units * (most > row ? most : row) >= (1ll << 40)) return ln_fail(ctx, LN_ERR_UNSUPPORTED, "%s: %lld tiles", who, (long long)num_units);
     p.num_units = (int)num_units;
+    p.whole = (int)(tiles - cut);
     auto magic = [](int d) { return ((1ull << 40) + (unsigned long long)d - 1) / (unsigned long long)d; };
     p.magic_f = magic(p.tiles_f); p.magic_w = flat ? 0 : magic(p.tiles_w); p.magic_h = magic(p.tiles_h);
     p.off_b = 128u * p.bk;
@@ -676,9 +705,12 @@ int ln_f4_umma_launch(ln_ctx* ctx, const ln_f4_conv& c) {
     {
         const cuuint64_t dims[2] = {(cuuint64_t)((int64_t)c.k * c.k * x.cstride), (cuuint64_t)p.F};
         const cuuint64_t strides[1] = {(cuuint64_t)((int64_t)c.k * c.k * x.cstride)};
-        const cuuint32_t box[2] = {(cuuint32_t)p.bk, (cuuint32_t)p.bn};
-        const CUresult r = ctx->encode_tiled(&p.tmB, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, c.w->w, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swz, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+        CUresult r = CUDA_SUCCESS;
+        for (int m = 0; m < (p.log_split ? 2 : 1) && r == CUDA_SUCCESS; ++m) {
+            const cuuint32_t box[2] = {(cuuint32_t)p.bk, (cuuint32_t)(m ? p.narrow : p.bn)};
+            r = ctx->encode_tiled(&p.tmB[m], CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, c.w->w, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swz, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
                                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+        }
         if (r != CUDA_SUCCESS) return ln_fail(ctx, LN_ERR_CUDA, "%s: cuTensorMapEncodeTiled(weights) failed with %d", who, (int)r);
     }
     {
