@@ -157,21 +157,31 @@ struct ln_f4_conv {  // one convolution: operands, geometry, output
     ln_tensor* y = nullptr;
     int k = 1, stride = 1, pad = 0, act = 0, out_kind = LN_OUT_F32;
 };
-// launches a 4-bit kernel (all begin with ln_f4_after_predecessor) on the ctx stream
+// launches a 4-bit kernel (all begin with ln_f4_after_predecessor) on the ctx stream, in clusters of `cluster` CTAs
 template <typename... P, typename... A>
-inline cudaError_t ln_f4_launch(ln_ctx* ctx, void (*kernel)(P...), int grid, int threads, size_t smem, const A&... args) {
+inline cudaError_t ln_f4_launch_clusters(ln_ctx* ctx, void (*kernel)(P...), int grid, int threads, size_t smem, int cluster, const A&... args) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)grid);
     cfg.blockDim = dim3((unsigned)threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = ctx->stream;
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
+    if (cluster > 1) {
+        attr[1].id = cudaLaunchAttributeClusterDimension;
+        attr[1].val.clusterDim.x = (unsigned)cluster;
+        attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+        cfg.numAttrs = 2;
+    }
     ctx->launches++;
     return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+}
+template <typename... P, typename... A>
+inline cudaError_t ln_f4_launch(ln_ctx* ctx, void (*kernel)(P...), int grid, int threads, size_t smem, const A&... args) {
+    return ln_f4_launch_clusters(ctx, kernel, grid, threads, smem, 1, args...);
 }
 bool ln_f4_umma_takes(const ln_f4_conv& c, int64_t stride_x, int64_t stride_y);
 int ln_f4_umma_launch(ln_ctx* ctx, const ln_f4_conv& c);

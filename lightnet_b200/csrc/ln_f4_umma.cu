@@ -15,7 +15,8 @@
 // of four that take the units of 32 columns of the tiles in turn.  TMEM: 416 columns of accumulators, 2 x 48 of scales.  Three tiles of
 // 128 filters or six of 64 fit; two of 256 overlap by 96 columns (0..255 and 160..415), so their epilogue reads the four units that hold
 // the overlap first, and the next tile starts when those have been read.
-// The last round of tiles, where it would leave SMs idle, is cut into units of fewer filters; each is the last one of its CTA, so nothing
+// Where all tiles leave SMs idle, long k ranges are split over clusters: each CTA takes a part, then one unit of the tile's sums, which
+// the others write into its shared memory.  The last round of tiles, where it would leave SMs idle, is cut into units of fewer filters; each is the last one of its CTA, so nothing
 // waits for its accumulator to be free.
 // What bounds it: large k ranges the way from L2 to shared memory (54 KB per k-block of 256 filters at 64 bytes a cycle are 844 cycles, the
 // instructions take 528; measured 830), short ones the epilogue.  CTA pairs (cta_group::2, half of the filters' codes per CTA) were built and
@@ -54,6 +55,7 @@ struct f4_params {
     int bk, bn, cblocks, words;
     int R, S, stride, pad, H, W, N, OH, OW, F, hw;
     int TW, TH, TN, log_tw, log_th, tiles_f, tiles_w, tiles_h, num_units;  // units: pixel tiles x filter tiles
+    int log_parts;  // CTAs of a cluster that share a tile's k range, as many as the tile has units of 32 columns
     int whole, log_split, narrow;  // the tiles behind the first `whole` are cut into 2^log_split units of `narrow` filters
     unsigned long long magic_f, magic_w, magic_h;
     int stages, nbuf, acc_step, subs, act, exact, flat;
@@ -64,6 +66,15 @@ __device__ __forceinline__ bool elect_one() {
     uint32_t p;
     asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(p));
     return p != 0;
+}
+__device__ __forceinline__ void cluster_sync() {  // (of whole warps)
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t peer_smem(uint32_t addr, int rank) {
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
 }
 // a wait of the whole warp: one answer for all lanes
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status, int code) {
@@ -164,12 +175,38 @@ __device__ __forceinline__ f4_box box_at(const f4_params& p, int unit) {
 
 // what the epilogue shares with the other roles: shared addresses of its table and barriers
 struct f4_epilogue_at {
-    uint32_t tmem, tab, rows, tfull, tempty, early;  // rows: 32 rows of 17 words
+    uint32_t tmem, tab, rows, tfull, tempty, early, ring;  // rows: 32 rows of 17 words
     volatile int* abort_flag;
+    int unit, step, rank;  // first unit; units from one to the next; place in the cluster
 };
-template <int FMT, int OUT, int WBLOCKS, int ACT, bool EXACT>
+constexpr uint32_t kPartBytes = 128 * CH * 4;  // of a unit's partial sums: [quarter of 32 rows][4 columns][row][column]
+// A split k range: every CTA of the cluster has partial sums of the whole tile.  It finishes one unit, and writes the others into the shared
+// memory of the CTAs that do those; their stages are free then.
+__device__ __forceinline__ void f4_exchange(const f4_params& p, const f4_epilogue_at& e) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quad = warp & 3;
+    const bool ok = warp_wait(e.tfull, 0, e.abort_flag, p.status, LN_STATUS_EPILOGUE_TIMEOUT);
+    __syncwarp();
+    cluster_sync();  // (all instructions of all CTAs are done)
+    tc_fence_after();
+    if (ok)
+        for (int j = (warp - kFirstEpilogueWarp) >> 2; j < p.subs; j += 4) {
+            if (j == e.rank) continue;
+            const uint32_t dst = peer_smem(e.ring + (uint32_t)(e.rank < j ? e.rank : e.rank - 1) * kPartBytes + 4096u * quad + 16u * lane, j);
+#pragma unroll 1
+            for (int c0 = 0; c0 < CH; c0 += 16) {
+                uint32_t acc[16];
+                tmem_ld(e.tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(j * CH + c0), acc);
+#pragma unroll
+                for (int i = 0; i < 16; i += 4)
+                    asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + 128u * (c0 + i)), "r"(acc[i]), "r"(acc[i + 1]), "r"(acc[i + 2]), "r"(acc[i + 3]) : "memory");
+            }
+        }
+    __syncwarp();
+    cluster_sync();
+}
+template <int FMT, int OUT, int WBLOCKS, bool PARTS, int ACT, bool EXACT>
 __device__ __forceinline__ void f4_epilogue(const f4_params& p, const f4_epilogue_at& e) {
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, first_unit = (int)blockIdx.x, step = (int)gridDim.x;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, step = e.step;
     constexpr bool overlap = WBLOCKS == 2;
     // Group g takes the units with number % 4 == g.  (nbuf * subs >= 4: a group that waits for a tile's accumulator has finished a unit
     // of the tile nbuf before it or a later one, so the parity is unambiguous.)
@@ -183,7 +220,7 @@ __device__ __forceinline__ void f4_epilogue(const f4_params& p, const f4_epilogu
     // epilogue (measured 2400).
     constexpr bool scaled = FMT == LN_F4;
     float wscale = 0.0f, bias = 0.0f;
-    int unit = first_unit, order = group, buf = 0, pixel_tile = 0, col = 0, f0 = 0;  // of the next unit
+    int unit = e.unit, order = PARTS ? (group ? p.subs : e.rank) : group, buf = 0, pixel_tile = 0, col = 0, f0 = 0;  // of the next unit
     uint32_t phase = 0;
     auto settle = [&]() {  // units beyond the tile's: the next tiles
         while (unit < p.num_units && order >= (unit < p.whole ? p.subs : p.narrow / CH)) {
@@ -227,7 +264,7 @@ __device__ __forceinline__ void f4_epilogue(const f4_params& p, const f4_epilogu
         } else
             asm volatile("st.shared.f32 [%0], %1;" ::"r"(tab + 4u * lane), "f"(bias) : "memory");
         __syncwarp();
-        order += 4;
+        order += PARTS ? p.subs : 4;
         settle();
         prefetch();
         if (!(ok = warp_wait(e.tfull + 8u * this_buf, this_phase, e.abort_flag, p.status, LN_STATUS_EPILOGUE_TIMEOUT))) break;
@@ -239,6 +276,17 @@ __device__ __forceinline__ void f4_epilogue(const f4_params& p, const f4_epilogu
             uint32_t acc[W];
             __syncwarp();  // (rows behind the last pixel store nothing)
             tmem_ld(taddr + c0, acc);
+            for (int part = 1; PARTS && part < 1 << p.log_parts; ++part) {  // (this CTA's own sum first, the others in their order)
+#pragma unroll
+                for (int i = 0; i < W; i += 4) {
+                    float4 t;
+                    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(t.x), "=f"(t.y), "=f"(t.z), "=f"(t.w) : "r"(e.ring + (uint32_t)(part - 1) * kPartBytes + 4096u * quad + 16u * lane + 128u * (c0 + i)));
+                    acc[i] = __float_as_uint(__fadd_rn(__uint_as_float(acc[i]), t.x));
+                    acc[i + 1] = __float_as_uint(__fadd_rn(__uint_as_float(acc[i + 1]), t.y));
+                    acc[i + 2] = __float_as_uint(__fadd_rn(__uint_as_float(acc[i + 2]), t.z));
+                    acc[i + 3] = __float_as_uint(__fadd_rn(__uint_as_float(acc[i + 3]), t.w));
+                }
+            }
             if (c0 + W == CH) {
                 tc_fence_before();
                 __syncwarp();
@@ -320,8 +368,8 @@ __device__ __forceinline__ void f4_epilogue(const f4_params& p, const f4_epilogu
     }
 }
 
-// WBLOCKS: groups of 128 filters that a tile's scales are in
-template <int FMT, int OUT, int WBLOCKS>
+// WBLOCKS: groups of 128 filters that a tile's scales are in; PARTS: clusters whose CTAs split the k range of one tile
+template <int FMT, int OUT, int WBLOCKS, bool PARTS>
 __global__ void __launch_bounds__(kThreadsF4, 1) f4_umma_kernel(const __grid_constant__ f4_params p) {
     extern __shared__ uint8_t smem_raw[];
     const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -359,7 +407,10 @@ __global__ void __launch_bounds__(kThreadsF4, 1) f4_umma_kernel(const __grid_con
     tc_fence_after();
     ln_f4_after_predecessor();
     const uint32_t tmem_base = *tmem_slot;
-    const int kblocks = p.R * p.S * p.cblocks, first_unit = (int)blockIdx.x, step = (int)gridDim.x;
+    const int kblocks = p.R * p.S * p.cblocks, log_parts = PARTS ? p.log_parts : 0, rank = (int)blockIdx.x & ((1 << log_parts) - 1);
+    const int first_unit = (int)blockIdx.x >> log_parts, step = (int)gridDim.x >> log_parts;
+    const int k0 = (kblocks * rank) >> log_parts, k1 = (kblocks * (rank + 1)) >> log_parts;  // of this CTA
+    const int tap0 = PARTS ? k0 / p.cblocks : 0, cb0 = k0 - tap0 * p.cblocks, r0 = PARTS ? tap0 / p.S : 0, s0 = tap0 - r0 * p.S;
     constexpr bool overlap = WBLOCKS == 2;
 
     if (warp == 0) {
@@ -371,25 +422,28 @@ __global__ void __launch_bounds__(kThreadsF4, 1) f4_umma_kernel(const __grid_con
             bool ok = true;
             for (int unit = first_unit; ok && unit < p.num_units; unit += step) {
                 const f4_box t = box_at(p, unit);
-                int sf_row = (t.ow0 >> 7) * kblocks * p.words;  // (flat)
-                for (int r = 0; ok && r < p.R; ++r)
-                    for (int s = 0; ok && s < p.S; ++s) {
-                        int ty = r - p.pad, tx = s - p.pad, map = 0;
-                        if (p.stride == 2) {
-                            const int py = ty & 1, px = tx & 1;  // parity class of the tap
-                            ty = (ty - py) >> 1;
-                            tx = (tx - px) >> 1;
-                            map = py * 2 + px;
-                        }
-                        for (int c0 = 0; c0 < p.cstride; c0 += p.bk, sf_row += p.words) {
-                            if (!(ok = mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag, p.status, LN_STATUS_PRODUCER_TIMEOUT))) break;
-                            const uint32_t at = smem_base + (uint32_t)stage * p.stage_bytes, bar = full_bar(stage);
-                            mbar_arrive_expect_tx(bar, bytes);
-                            tma_load_4d(at, &p.tmA[map], c0, t.ow0 + tx, t.oh0 + ty, t.n0, bar);
-                            if (p.flat) tma_load_2d(at + p.off_sfa, &p.tmXS, 0, sf_row, bar);
-                            if (++stage == p.stages) { stage = 0; phase ^= 1u; }
-                        }
+                int sf_row = ((t.ow0 >> 7) * kblocks + k0) * p.words;  // (flat)
+                int r = r0, s = s0, c0 = cb0 * p.bk;
+                for (int kb = k0; kb < k1;) {  // a tap's k-blocks
+                    int ty = r - p.pad, tx = s - p.pad, map = 0;
+                    if (p.stride == 2) {
+                        const int py = ty & 1, px = tx & 1;  // parity class of the tap
+                        ty = (ty - py) >> 1;
+                        tx = (tx - px) >> 1;
+                        map = py * 2 + px;
                     }
+                    for (; c0 < p.cstride && kb < k1; c0 += p.bk, ++kb, sf_row += p.words) {
+                        if (!(ok = mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag, p.status, LN_STATUS_PRODUCER_TIMEOUT))) break;
+                        const uint32_t at = smem_base + (uint32_t)stage * p.stage_bytes, bar = full_bar(stage);
+                        mbar_arrive_expect_tx(bar, bytes);
+                        tma_load_4d(at, &p.tmA[map], c0, t.ow0 + tx, t.oh0 + ty, t.n0, bar);
+                        if (p.flat) tma_load_2d(at + p.off_sfa, &p.tmXS, 0, sf_row, bar);
+                        if (++stage == p.stages) { stage = 0; phase ^= 1u; }
+                    }
+                    if (!ok) break;
+                    c0 = 0;
+                    if (++s == p.S) { s = 0; ++r; }
+                }
             }
         }
         __syncwarp();
@@ -403,8 +457,8 @@ __global__ void __launch_bounds__(kThreadsF4, 1) f4_umma_kernel(const __grid_con
                 const int f0 = unit_at(p, unit).f0;
                 const CUtensorMap* codes = &p.tmB[unit < p.whole ? 0 : 1];
                 const uint32_t bytes = (uint32_t)(unit < p.whole ? p.bn : p.narrow) * p.bk + WBLOCKS * (uint32_t)p.words * 512u;
-                int col = 0, c0 = 0;  // first byte of the tap, of the k-block inside it
-                for (int kb = 0; kb < kblocks; ++kb) {
+                int col = tap0 * p.cstride, c0 = cb0 * p.bk;  // first byte of the tap, of the k-block inside it
+                for (int kb = k0; kb < k1; ++kb) {
                     if (!(ok = mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag, p.status, LN_STATUS_PRODUCER_TIMEOUT))) break;
                     const uint32_t at = smem_base + (uint32_t)stage * p.stage_bytes, bar = full_bar(stage);
                     mbar_arrive_expect_tx(bar, bytes);
@@ -435,8 +489,8 @@ __global__ void __launch_bounds__(kThreadsF4, 1) f4_umma_kernel(const __grid_con
                 const uint32_t d = tmem_base + (uint32_t)(buf * p.acc_step);
                 const uint32_t idesc = idesc_base | ((uint32_t)((unit < p.whole ? p.bn : p.narrow) >> 3) << 17);
                 const uint32_t shift = (uint32_t)((unit_at(p, unit).f0 & 127) >> 5);  // first column of the tile's filters inside their group of 128
-                int c0 = 0;
-                for (int kb = 0; kb < kblocks; ++kb) {
+                int c0 = cb0 * p.bk;
+                for (int kb = k0; kb < k1; ++kb) {
                     if (!(ok = mbar_wait(full_bar(stage), phase, abort_flag, p.status, LN_STATUS_MMA_TIMEOUT))) break;
                     const uint32_t at = smem_base + (uint32_t)stage * p.stage_bytes;
                     const uint32_t sfa = tmem_base + kScaleCols + set * kScaleSet, sfb = sfa + kScaleB;
@@ -455,7 +509,7 @@ __global__ void __launch_bounds__(kThreadsF4, 1) f4_umma_kernel(const __grid_con
 #pragma unroll
                         for (int i = 0; i < kN; ++i) {
                             const uint32_t word = FMT == LN_MX4 ? i >> 1 : i, id = FMT == LN_MX4 ? (uint32_t)(i & 1) * 2u : 0u;
-                            if (whole || i < n) tc_mma_scaled<FMT>(d, a_desc + 2u * i, b_desc + 2u * i, idesc | (id << 4) | (id << 29), sfa + 4u * word, sfb + 4u * word * WBLOCKS + shift, i ? 1u : (uint32_t)(kb != 0));
+                            if (whole || i < n) tc_mma_scaled<FMT>(d, a_desc + 2u * i, b_desc + 2u * i, idesc | (id << 4) | (id << 29), sfa + 4u * word, sfb + 4u * word * WBLOCKS + shift, i ? 1u : (uint32_t)(kb != k0));
                         }
                     };
                     if (p.bk == 128) { if (n == 4) issue(std::integral_constant<int, 4>(), true); else issue(std::integral_constant<int, 4>(), false); }
@@ -474,7 +528,7 @@ __global__ void __launch_bounds__(kThreadsF4, 1) f4_umma_kernel(const __grid_con
         __syncwarp();
     } else if (warp < 2 + kGatherWarps) {
         // ------------------------------------------------------------------ scales of the pixels under shifted taps
-        int unit = first_unit, r = 0, s = 0, cb = 0, tap = 0;  // tap: pixels between the tap's and the first one's
+        int unit = first_unit, r = r0, s = s0, cb = cb0, tap = r0 * p.W + s0;  // tap: pixels between the tap's and the first one's
         int iy0[4], ix0[4], q0[4];                             // of the lane's rows under the first tap: place and number of the input pixel
         auto enter_tile = [&]() {
             if (unit >= p.num_units) return;
@@ -526,9 +580,11 @@ __global__ void __launch_bounds__(kThreadsF4, 1) f4_umma_kernel(const __grid_con
             int stage = warp - 2;  // (fewer than stages)
             uint32_t phase = 0;
             uint32_t v[4][4];
+            int left = k1 - k0 - stage;  // k-blocks from this one on, where they end inside a unit
             bool ok = true;
-            if (unit < p.num_units) fetch(v);
-            while (ok && unit < p.num_units) {
+            auto more = [&]() { return unit < p.num_units && (!PARTS || left > 0); };
+            if (more()) fetch(v);
+            while (ok && more()) {
                 if (!(ok = warp_wait(empty_bar(stage), phase ^ 1u, abort_flag, p.status, LN_STATUS_PRODUCER_TIMEOUT))) break;
                 const uint32_t dst = smem_base + (uint32_t)stage * p.stage_bytes + p.off_sfa + 16u * lane;
 #pragma unroll
@@ -542,26 +598,33 @@ __global__ void __launch_bounds__(kThreadsF4, 1) f4_umma_kernel(const __grid_con
                 if (stage >= p.stages) { stage -= p.stages; phase ^= 1u; }
                 // (behind the fence, which would wait for the reads; the other warps' k-blocks cover their latency)
                 for (int i = 0; i < kGatherWarps; ++i) advance();
-                if (unit < p.num_units) fetch(v);
+                left -= kGatherWarps;
+                if (more()) fetch(v);
             }
         }
+        __syncwarp();
     } else if (warp >= kFirstEpilogueWarp) {
         // ------------------------------------------------------------------ epilogue
         // (one loop per activation: a choice inside it put the code of a unit in pieces far apart, and its warps waited for instructions)
-        const f4_epilogue_at at = {tmem_base, tab_base + (uint32_t)(warp - kFirstEpilogueWarp) * 256u, tab_base + kTabBytesF4 + (uint32_t)(warp - kFirstEpilogueWarp) * kRowBytesF4, tfull_bar(0), tempty_bar(0), early_bar(0), abort_flag};
+        const f4_epilogue_at at = {tmem_base, tab_base + (uint32_t)(warp - kFirstEpilogueWarp) * 256u, tab_base + kTabBytesF4 + (uint32_t)(warp - kFirstEpilogueWarp) * kRowBytesF4, tfull_bar(0), tempty_bar(0), early_bar(0), smem_base, abort_flag, first_unit, step, rank};
+        if (PARTS) f4_exchange(p, at);
         switch (p.act + (p.exact ? 8 : 0)) {
-            case LN_ACT_LEAKY: case LN_ACT_LEAKY + 8: f4_epilogue<FMT, OUT, WBLOCKS, LN_ACT_LEAKY, true>(p, at); break;
-            case LN_ACT_RELU: case LN_ACT_RELU + 8: f4_epilogue<FMT, OUT, WBLOCKS, LN_ACT_RELU, true>(p, at); break;
-            case LN_ACT_MISH: f4_epilogue<FMT, OUT, WBLOCKS, LN_ACT_MISH, false>(p, at); break;
-            case LN_ACT_SWISH: f4_epilogue<FMT, OUT, WBLOCKS, LN_ACT_SWISH, false>(p, at); break;
-            case LN_ACT_LOGISTIC: f4_epilogue<FMT, OUT, WBLOCKS, LN_ACT_LOGISTIC, false>(p, at); break;
-            case LN_ACT_MISH + 8: f4_epilogue<FMT, OUT, WBLOCKS, LN_ACT_MISH, true>(p, at); break;
-            case LN_ACT_SWISH + 8: f4_epilogue<FMT, OUT, WBLOCKS, LN_ACT_SWISH, true>(p, at); break;
-            case LN_ACT_LOGISTIC + 8: f4_epilogue<FMT, OUT, WBLOCKS, LN_ACT_LOGISTIC, true>(p, at); break;
-            default: f4_epilogue<FMT, OUT, WBLOCKS, LN_ACT_LINEAR, true>(p, at); break;
+            case LN_ACT_LEAKY: case LN_ACT_LEAKY + 8: f4_epilogue<FMT, OUT, WBLOCKS, PARTS, LN_ACT_LEAKY, true>(p, at); break;
+            case LN_ACT_RELU: case LN_ACT_RELU + 8: f4_epilogue<FMT, OUT, WBLOCKS, PARTS, LN_ACT_RELU, true>(p, at); break;
+            case LN_ACT_MISH: f4_epilogue<FMT, OUT, WBLOCKS, PARTS, LN_ACT_MISH, false>(p, at); break;
+            case LN_ACT_SWISH: f4_epilogue<FMT, OUT, WBLOCKS, PARTS, LN_ACT_SWISH, false>(p, at); break;
+            case LN_ACT_LOGISTIC: f4_epilogue<FMT, OUT, WBLOCKS, PARTS, LN_ACT_LOGISTIC, false>(p, at); break;
+            case LN_ACT_MISH + 8: f4_epilogue<FMT, OUT, WBLOCKS, PARTS, LN_ACT_MISH, true>(p, at); break;
+            case LN_ACT_SWISH + 8: f4_epilogue<FMT, OUT, WBLOCKS, PARTS, LN_ACT_SWISH, true>(p, at); break;
+            case LN_ACT_LOGISTIC + 8: f4_epilogue<FMT, OUT, WBLOCKS, PARTS, LN_ACT_LOGISTIC, true>(p, at); break;
+            default: f4_epilogue<FMT, OUT, WBLOCKS, PARTS, LN_ACT_LINEAR, true>(p, at); break;
         }
     }
 
+    if (PARTS && warp < kFirstEpilogueWarp) {  // (the two barriers of the exchange: every warp of the cluster comes to both, whatever its waits ended with)
+        cluster_sync();
+        cluster_sync();
+    }
     tc_fence_before();
     __syncthreads();
     if (*abort_flag && warp == 0 && lane == 0) {
@@ -583,13 +646,14 @@ int log2_of(int v) {
 
 template <int FMT, int OUT>
 cudaError_t launch(ln_ctx* ctx, const f4_params& p, int grid, size_t smem) {
-    void (*k)(const f4_params) = p.bn > 128 ? f4_umma_kernel<FMT, OUT, 2> : f4_umma_kernel<FMT, OUT, 1>;
+    void (*k)(const f4_params) = p.bn > 128 ? f4_umma_kernel<FMT, OUT, 2, false>
+                                            : (p.log_parts ? f4_umma_kernel<FMT, OUT, 1, true> : f4_umma_kernel<FMT, OUT, 1, false>);
     if (!ctx->configured_kernels.count((const void*)k)) {
         const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmemF4);
         if (e != cudaSuccess) return e;
         ctx->configured_kernels.insert((const void*)k);
     }
-    return ln_f4_launch(ctx, k, grid, kThreadsF4, smem, p);
+    return ln_f4_launch_clusters(ctx, k, grid, kThreadsF4, smem, 1 << p.log_parts, p);
 }
 
 }  // namespace
@@ -630,30 +694,34 @@ int ln_f4_umma_launch(ln_ctx* ctx, const ln_f4_conv& c) {
     // A launch takes about start + (k-blocks of a tile + (rounds - 1) x the longer of k-blocks and epilogue), rounds = tiles per SM, in ns
     // as measured over 27 shapes of both types with binary16 output (leaky), 3 to 76 us, each with every tile; the choice was the best one or
     // within 4 % of it on all of them.  Where most SMs have nothing to do, a k-block of 256 filters comes faster.
-    // The tiles of the last, partly filled round may be cut into units of fewer filters, where those fit into one round.
+    // The tiles of the last, partly filled round may be cut into units of fewer filters, where those fit into one round.  Where all tiles
+    // leave SMs idle, the k range may be split over a cluster, which costs 3.1 us more (launch, two barriers, exchange; 4.3 where most SMs take part): worth it from about
+    // 20 k-blocks on (128 x 11008 -> 4096, LN_F4: 16.8 us, split over four 11.4; 3x3 C1024->K512 at 13x13: 14.9 and 10.2).
     const int64_t kblocks = (int64_t)c.k * c.k * kb.cblocks, sms = ctx->sm_count;
     const int cand[3] = {256, 128, 64}, start[3] = {5400, 3650, 3300}, out[3] = {3300, 1750, 900}, flat_k[3] = {490, 360, 320}, tap_k[3] = {640, 520, 420};
-    int64_t least = -1;
     const bool rows = c.out_kind == LN_OUT_F32 && flat && p.hw == 1 && p.F % 8 != 0;  // (their way through shared memory leaves no four stages of the widest tile)
-    int force = 0, force_narrow = 0;
-    if (const char* e = getenv("LN_F4_BN")) {  // (A/B measurements: another filter tile, "256/64": with the last round in units of 64)
-        force = atoi(e);
+    int force = 0, force_narrow = 0, force_parts = 1;
+    if (const char* e = getenv("LN_F4_BN")) {  // (A/B measurements: another filter tile where it can be; "256/64": with the last round in units of 64; "128*4": its k range over 4 CTAs)
+        force = force_narrow = atoi(e);
         if (const char* slash = strchr(e, '/')) force_narrow = atoi(slash + 1);
-        if ((force != 256 || rows) && force != 128 && force != 64) force = 0;
+        if (const char* star = strchr(e, '*')) force_parts = atoi(star + 1);
     }
+    int64_t least = -1;
+    int parts = 1;
+    auto consider = [&](int bn, int narrow, int split, int64_t cost) {
+        if (force && (bn != force || narrow != force_narrow || split != force_parts)) cost += 1ll << 50;
+        if (least < 0 || cost < least) { least = cost; p.bn = bn; p.narrow = narrow; parts = split; }
+    };
     for (int i = rows ? 1 : 0; i < 3; ++i) {
-        if (force && cand[i] != force) continue;
         const int64_t tiles = best * ((p.F + cand[i] - 1) / cand[i]), rounds = (tiles + sms - 1) / sms, rest = tiles % sms;
         const int64_t chain = kblocks * (!flat ? tap_k[i] : (i == 0 && 2 * tiles <= sms ? 330 : flat_k[i])), round = chain > out[i] ? chain : out[i];
-        for (int j = i; j < 3; ++j) {
-            if (j > i && (rounds == 1 || rest == 0 || rest * (cand[i] / cand[j]) > sms)) continue;
+        consider(cand[i], cand[i], 1, start[i] + chain + (rounds - 1) * round);
+        for (int j = i + 1; j < 3; ++j) {
             const int64_t tail = kblocks * (flat ? flat_k[j] : tap_k[j]);
-            int64_t cost = start[j] + chain + (rounds - 1) * round;
-            if (j > i) cost += (tail > out[i] ? tail : out[i]) - round;
-            if (force && force_narrow == cand[j]) cost = 0;
-            if (force && !force_narrow && j > i) continue;
-            if (least < 0 || cost < least) { least = cost; p.bn = cand[i]; p.narrow = cand[j]; }
+            if (rounds > 1 && rest && rest * (cand[i] / cand[j]) <= sms) consider(cand[i], cand[j], 1, start[j] + chain + (rounds - 2) * round + (tail > out[i] ? tail : out[i]));
         }
+        const int split = cand[i] / CH;
+        if (i && tiles * split <= sms && kblocks >= split) consider(cand[i], cand[i], split, start[i] + chain / split + (4 * tiles * split > 3 * sms ? 4300 : 3100));
     }
     const int wblocks = p.bn > 128 ? 2 : 1;
     p.nbuf = p.bn == 256 ? 2 : (int)kScaleCols / p.bn;
@@ -678,9 +746,13 @@ int ln_f4_umma_launch(ln_ctx* ctx, const ln_f4_conv& c) {
     const size_t rest = 1024 + kBarBytesF4 + kTabBytesF4 + (rows ? 16 * kRowBytesF4 : 0);
     p.stages = (int)((kMaxSmemF4 - rest) / p.stage_bytes);
     if (p.stages > kMaxStagesF4) p.stages = kMaxStagesF4;
+    p.log_parts = log2_of(parts);
     size_t smem = rest + (size_t)p.stages * p.stage_bytes;
     // One CTA per SM: it takes all of TMEM and would wait while another one has it, so none asks for less than half of an SM's shared memory.
     if (smem < kLeastSmemF4) smem = kLeastSmemF4;
+    // The CTAs of a cluster wait for each other: with one of another such kernel beside each, two clusters could hold the TMEM that the other
+    // one waits for.  With all of the shared memory asked for none fits.
+    if (parts > 1) smem = kMaxSmemF4;
     p.xsf = (const uint8_t*)x.sf; p.wscale = c.w->wscale; p.bias = c.bias;
     p.y = y.ptr; p.ys = y.cstride; p.ysf = (uint8_t*)y.sf; p.ysf_words = y.sf_words;
     p.xscale = x.scale; p.g = y.scale; p.six_g = 6.0f * y.scale;
@@ -727,7 +799,7 @@ int ln_f4_umma_launch(ln_ctx* ctx, const ln_f4_conv& c) {
         }
         if (r != CUDA_SUCCESS) return ln_fail(ctx, LN_ERR_CUDA, "%s: cuTensorMapEncodeTiled(scales) failed with %d", who, (int)r);
     }
-    const int grid = p.num_units < ctx->sm_count ? p.num_units : ctx->sm_count;
+    const int grid = parts > 1 ? p.num_units * parts : (p.num_units < ctx->sm_count ? p.num_units : ctx->sm_count);
     cudaError_t e;
 #define LN_F4_LAUNCH(FMT) \
     (c.out_kind == LN_OUT_F32 ? launch<FMT, LN_OUT_F32>(ctx, p, grid, smem) : c.out_kind == LN_OUT_F16 ? launch<FMT, LN_OUT_F16>(ctx, p, grid, smem) : launch<FMT, LN_OUT_Q>(ctx, p, grid, smem))
