@@ -17,8 +17,11 @@ __device__ __forceinline__ void ln_store_32(void* dst, const uint32_t (&v)[8]) {
 // 16 bytes that are read once
 __device__ __forceinline__ uint4 ln_ldg_stream(const __half* p) { return __ldcs(reinterpret_cast<const uint4*>(p)); }
 
-int grid_for(ln_ctx* ctx, int64_t n) {
-    const int64_t b = (n + kThreads - 1) / kThreads, cap = (int64_t)ctx->sm_count * 16;
+// Up to 64 blocks per SM: with 16, few enough for loops of two or three rounds, the last round left SMs idle (64 x 128 x 76 x 76, LN_F4, to
+// binary16 21.4 us, now 19.9, to f32 43.5, now 38.9).  The rows of narrow_rows_kernel go through shared memory and want 16 (33.8 us against
+// 35.9 for 8192 x 4096).
+int grid_for(ln_ctx* ctx, int64_t n, int per_sm = 64) {
+    const int64_t b = (n + kThreads - 1) / kThreads, cap = (int64_t)ctx->sm_count * per_sm;
     return (int)(b < 1 ? 1 : (b > cap ? cap : b));
 }
 int check_launch(ln_ctx* ctx, const char* what, cudaError_t e) {
@@ -60,7 +63,7 @@ __device__ __forceinline__ uint32_t store_block(const float* x, float g, float s
     return scale;
 }
 template <int FMT, typename I>
-__global__ void __launch_bounds__(kThreads) narrow_f16_kernel(const __half* __restrict__ x, int64_t xs, uint8_t* __restrict__ codes, uint8_t* __restrict__ sf, int64_t pixels, int C, int groups,
+__global__ void __launch_bounds__(kThreads, 5) narrow_f16_kernel(const __half* __restrict__ x, int64_t xs, uint8_t* __restrict__ codes, uint8_t* __restrict__ sf, int64_t pixels, int C, int groups,
                                                               int64_t cstride, int64_t sf_words, float g, float six_g) {
     ln_f4_after_predecessor();
     constexpr int B = FMT == LN_F4 ? 16 : 32;
@@ -511,7 +514,7 @@ int narrow_into(ln_ctx* ctx, const ln_tensor* t, ln_tensor* q) {
     cudaError_t e;
     const int blocks = (int)(q->cstride * 2 / ln_f4_block(q->dtype));
     if (t->dtype == LN_F32 && hw == 1) {
-        const int grid = grid_for(ctx, pixels * blocks);
+        const int grid = grid_for(ctx, pixels * blocks, 16);
         e = q->dtype == LN_F4 ? ln_f4_launch(ctx, narrow_rows_kernel<LN_F4>, grid, kThreads, 0, (const float*)t->ptr, codes, sf, pixels, (int)t->c, blocks, q->cstride, q->sf_words, g, six_g)
                               : ln_f4_launch(ctx, narrow_rows_kernel<LN_MX4>, grid, kThreads, 0, (const float*)t->ptr, codes, sf, pixels, (int)t->c, blocks, q->cstride, q->sf_words, g, six_g);
     } else if (t->dtype == LN_F32) {
