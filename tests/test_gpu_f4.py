@@ -369,7 +369,7 @@ def test_operators_together(be):
 
 
 def test_images_do_not_depend_on_the_batch(be):
-    """An image has the same bits alone and in a batch, whatever kernel a size leads to."""
+    """An image has the same values alone and in a batch, to the rounding of the sums, whatever kernel a size leads to."""
     rng = np.random.default_rng(21)
     for dtype, (c, h, w, f, k) in ((ln.LN_F4, (96, 9, 11, 80, 3)), (ln.LN_MX4, (256, 13, 13, 64, 1)), (ln.LN_F4, (2048, 1, 1, 300, 1))):
         x = rng.normal(0, 1, (40, c, h, w)).astype(np.float32)
