@@ -556,6 +556,7 @@ int32_t ln_tensor_narrow_f4(ln_ctx* ctx, const ln_tensor* t, float scale, int32_
     if (t->dtype != LN_F32 && t->dtype != LN_F16) return ln_fail(ctx, LN_ERR_ARG, "%s: f32 or binary16 tensor required", who);
     if (t->ctx != ctx) return ln_fail(ctx, LN_ERR_ARG, "%s: the tensor belongs to another context", who);
     if (!ln_is_f4(dtype)) return ln_fail(ctx, LN_ERR_ARG, "%s: dtype must be LN_F4 or LN_MX4", who);
+    if (t->c > (1 << 30)) return ln_fail(ctx, LN_ERR_UNSUPPORTED, "%s: more than 2^30 channels", who);
     if (!usable_scale(dtype, scale)) return ln_fail(ctx, LN_ERR_ARG, "%s: scale %g is not %s", who, scale, dtype == LN_MX4 ? "1 (LN_MX4 has no tensor scale)" : "in [2^-100, 2^100]");
     return guarded(ctx, who, [&]() -> int32_t {
         cudaSetDevice(ctx->device);

@@ -333,6 +333,9 @@ def test_more_tiles_than_any_network(be):
         gw = 1.0 if dtype == ln.LN_MX4 else f32(np.abs(three).max((1, 2, 3)).astype(np.float64) / 2688)
         value = narrow(x[:, :, -s:], dtype, g)[2]
         assert np.array_equal(be.download_f32(be.widen_f4(q))[:, :, -s:], value)
+        again = be.narrow_f4(be.widen_f4(q, ln.LN_F16), g, dtype)
+        assert np.array_equal(be.download_f32(be.widen_f4(again))[:, :, -s:], value)
+        del again
         b = be.zeros_f32((1, 1, 1, 1))
         y = be.download_f32(be.conv2d_bias_act_f4(q, be.conv_weights_f4(be.upload_f32(one.shape, one), 1, 1, 1, dtype), b, x.shape, 1, h, w, 1, 1, 1, 1, 1, 0, 1, "linear", 1.0, ln.LN_OUT_F32))
         assert np.allclose(y[:, :, -s:], value * 1.5, rtol=2.0 ** -21, atol=0)
@@ -538,6 +541,7 @@ def test_refusals(be):
     finally:
         other.close()
     refused("argument", ln.GpuExecutableNetwork, be, "[net]\nwidth=32\nheight=32\nchannels=3\n[convolutional]\nfilters=8\nsize=1\nstride=1\nactivation=linear\n", 1, ln.LN_F4)
+    refused("unsupported", be.narrow_f4, be.zeros_f32((1, (1 << 30) + 1, 1, 1)), 1.0)
     # a failed allocation is an error of the call, and the next one works
     be.debug_fail_alloc(1)
     refused("cuda", be.narrow_f4, t, 0.01)
