@@ -76,6 +76,12 @@ __device__ __forceinline__ uint32_t peer_smem(uint32_t addr, int rank) {
     asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
     return r;
 }
+// whether a phase is complete, now
+__device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    return ok != 0;
+}
 // a wait of the whole warp: one answer for all lanes
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status, int code) {
     return __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity, abort_flag, status, code));
@@ -480,7 +486,7 @@ __global__ void __launch_bounds__(kThreadsF4, 1) f4_umma_kernel(const __grid_con
             const uint64_t sfa_desc = scale_desc(p.off_sfa), sfb_desc = scale_desc(p.off_sfb);
             int stage = 0, t = 0;
             uint32_t phase = 0, set = 0;
-            bool ok = true;
+            bool ok = true, ready = false;  // ready: the next k-block was there when this one was issued
             for (int unit = first_unit; ok && unit < p.num_units; unit += step, ++t) {
                 const int buf = t % p.nbuf;
                 if (!(ok = mbar_wait(tempty_bar(buf), (uint32_t)((t / p.nbuf) & 1) ^ 1u, abort_flag, p.status, LN_STATUS_MMA_TIMEOUT))) break;
@@ -491,7 +497,9 @@ __global__ void __launch_bounds__(kThreadsF4, 1) f4_umma_kernel(const __grid_con
                 const uint32_t shift = (uint32_t)((unit_at(p, unit).f0 & 127) >> 5);  // first column of the tile's filters inside their group of 128
                 int c0 = cb0 * p.bk;
                 for (int kb = k0; kb < k1; ++kb) {
-                    if (!(ok = mbar_wait(full_bar(stage), phase, abort_flag, p.status, LN_STATUS_MMA_TIMEOUT))) break;
+                    if (!ready && !(ok = mbar_wait(full_bar(stage), phase, abort_flag, p.status, LN_STATUS_MMA_TIMEOUT))) break;
+                    const int next = stage + 1 == p.stages ? 0 : stage + 1;
+                    const uint32_t next_phase = next ? phase : phase ^ 1u;
                     const uint32_t at = smem_base + (uint32_t)stage * p.stage_bytes;
                     const uint32_t sfa = tmem_base + kScaleCols + set * kScaleSet, sfb = sfa + kScaleB;
                     const int left = p.cstride - c0, n = (left < p.bk ? left : p.bk) >> 5;  // instructions of this k-block
@@ -510,6 +518,8 @@ __global__ void __launch_bounds__(kThreadsF4, 1) f4_umma_kernel(const __grid_con
                         for (int i = 0; i < kN; ++i) {
                             const uint32_t word = FMT == LN_MX4 ? i >> 1 : i, id = FMT == LN_MX4 ? (uint32_t)(i & 1) * 2u : 0u;
                             if (whole || i < n) tc_mma_scaled<FMT>(d, a_desc + 2u * i, b_desc + 2u * i, idesc | (id << 4) | (id << 29), sfa + 4u * word, sfb + 4u * word * WBLOCKS + shift, i ? 1u : (uint32_t)(kb != k0));
+                            // (asked for while instructions are still being issued: a wait takes its thread 150 cycles even where there is nothing to wait for)
+                            if (i == (kN - 1) / 2) ready = mbar_test(full_bar(next), next_phase);
                         }
                     };
                     if (p.bk == 128) { if (n == 4) issue(std::integral_constant<int, 4>(), true); else issue(std::integral_constant<int, 4>(), false); }
@@ -519,7 +529,8 @@ __global__ void __launch_bounds__(kThreadsF4, 1) f4_umma_kernel(const __grid_con
                     set ^= 1u;
                     c0 += p.bk;
                     if (c0 >= p.cstride) c0 = 0;
-                    if (++stage == p.stages) { stage = 0; phase ^= 1u; }
+                    stage = next;
+                    phase = next_phase;
                 }
                 if (!ok) break;
                 tc_commit(tfull_bar(buf));
