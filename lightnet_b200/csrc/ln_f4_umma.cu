@@ -19,7 +19,8 @@
 // the others write into its shared memory.  The last round of tiles, where it would leave SMs idle, is cut into units of fewer filters; each is the last one of its CTA, so nothing
 // waits for its accumulator to be free.
 // What bounds it: large k ranges the way from L2 to shared memory (54 KB per k-block of 256 filters at 64 bytes a cycle are 844 cycles, the
-// instructions take 528; measured 830), short ones the epilogue.  CTA pairs (cta_group::2, half of the filters' codes per CTA) were built and
+// instructions take 528, measured 830 to 900; 28 KB of 64 filters 437, measured 550) and, in runs of seconds, power (1500 MHz); short ones the
+// epilogue.  K-blocks of half the size (8192 x 4096 x 4096 in 80 us instead of 63) pay the fixed cost of a k-block twice.  CTA pairs (cta_group::2, half of the filters' codes per CTA) were built and
 // gave the same 64 us on 8192 x 4096 x 4096: a tcgen05.cp of a pair takes its thread 50 cycles and more, and twelve go with four instructions.
 // Every wait is bounded (see ln_umma.h).
 #include <cstdlib>
