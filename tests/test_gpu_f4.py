@@ -293,7 +293,7 @@ def test_each_tile_of_filters(be, monkeypatch, dtype, tile):
     monkeypatch.setenv("LN_F4_BN", tile)
     for case in ((1, 512, 19, 19, 255, 1, 1, 1, 0), (131, 80, 1, 1, 40, 1, 1, 1, 0), (300, 1024, 1, 1, 1000, 1, 1, 1, 0), (2, 192, 9, 9, 320, 3, 1, 1, 1), (2, 128, 26, 30, 72, 3, 2, 2, 1),
                  (3, 70, 120, 119, 136, 1, 1, 1, 0), (2, 40, 75, 77, 300, 3, 1, 1, 1),
-                 (1, 64, 150, 150, 200, 1, 1, 1, 0), (1, 200, 140, 141, 72, 3, 1, 1, 1), (1, 512, 13, 13, 300, 3, 1, 1, 1), (20, 4096, 1, 1, 264, 1, 1, 1, 0), (1, 96, 12, 13, 136, 5, 2, 2, 2)):
+                 (1, 64, 150, 150, 200, 1, 1, 1, 0), (1, 200, 140, 141, 72, 3, 1, 1, 1), (1, 512, 13, 13, 300, 3, 1, 1, 1), (20, 4096, 1, 1, 264, 1, 1, 1, 0), (40, 2048, 1, 1, 257, 1, 1, 1, 0), (1, 96, 12, 13, 136, 5, 2, 2, 2)):
         y, ref, bound = run_conv(be, case, dtype, "mish", ln.LN_OUT_F32)
         wide = be.download_f32(y)
         assert np.max(np.abs(wide - ref) / bound) <= 1, case
