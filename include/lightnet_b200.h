@@ -90,9 +90,14 @@ int32_t ln_tensor_download_f32(ln_ctx* ctx, const ln_tensor* t, float* host, int
 int32_t ln_tensor_shape(const ln_tensor* t, int64_t shape[4]);
 int32_t ln_tensor_dtype(const ln_tensor* t);
 /* Device address of an f32 or binary16 tensor's first value, its shape and the distance in values between neighbours along each axis, for a
-   program that hands the tensor to another library on the same GPU.  The handle keeps the memory; work on another stream has to be
-   ordered behind the ctx stream (ln_ctx_stream) by the caller, and in front of it again before the handle is released. */
+   program that hands the tensor to another library on the same GPU.  The handle keeps the memory; work on another stream is ordered by
+   ln_tensor_share. */
 int32_t ln_tensor_device_data(const ln_tensor* t, void** data, int64_t shape[4], int64_t strides[4]);
+/* Lets work on another stream of the ctx's device read a tensor (NULL: the legacy default stream): what `stream` is given from here on waits for
+   what the ctx stream holds now, and once the last handle is gone the memory is used again only behind what `stream` holds then.  The stream
+   has to exist until that release.  A tensor may be shared with several streams.  Nothing waits on the host.  LN_ERR_UNSUPPORTED, and nothing is ordered, where one
+   of the two streams is being captured into a graph that the other is not part of. */
+int32_t ln_tensor_share(ln_ctx* ctx, ln_tensor* t, void* stream);
 int32_t ln_tensor_retain(ln_tensor* t);
 int32_t ln_tensor_release(ln_tensor* t);
 

@@ -86,6 +86,7 @@ SYMBOLS = {
     "ln_tensor_shape": (C.c_int32, [_VP, _I64P]),
     "ln_tensor_dtype": (C.c_int32, [_VP]),
     "ln_tensor_device_data": (C.c_int32, [_VP, _VP, _VP, _VP]),
+    "ln_tensor_share": (C.c_int32, [_VP, _VP, _VP]),
     "ln_tensor_retain": (C.c_int32, [_VP]),
     "ln_tensor_release": (C.c_int32, [_VP]),
     "ln_conv2d_f32": (C.c_int32, [_VP, _VP, _VP, _I64P] + [C.c_int64] * 10 + [_PP]),
@@ -239,24 +240,31 @@ class Tensor:
     def scale(self):
         return float(_lib.ln_tensor_scale(self.h))
 
-    def __getattr__(self, name):
-        """`__cuda_array_interface__`: f32 and binary16 tensors for other libraries on the same GPU (`torch.as_tensor(t, device="cuda")`
-        shares the memory and keeps the handle); order their work behind the backend's stream.  Made when it is first asked for."""
-        if name != "__cuda_array_interface__":
-            raise AttributeError(name)
-        dtype = _lib.ln_tensor_dtype(self.h)
+    def share(self, stream=0):
+        """Lets `stream` (a CUDA stream handle; 0: the default stream) read the tensor's memory: its next work waits for what made the tensor, and the
+        memory is used again only behind what the stream holds when the last reference goes.  The stream has to exist until then."""
+        self.backend._check(_lib.ln_tensor_share(self.backend.ctx, self.h, stream))
+
+    @property
+    def __cuda_array_interface__(self):
+        """f32 and binary16 tensors for other libraries on the same GPU: `torch.as_tensor(t, device="cuda")` shares the memory and keeps the handle.
+        Asking for it shares the tensor with the default stream (not while the backend's stream is being captured); one that is used on another
+        stream is shared with that by `share`."""
+        backend, dtype = self.backend, _lib.ln_tensor_dtype(self.h)
         if dtype != LN_F32 and dtype != LN_F16:
             raise AttributeError("only f32 and binary16 tensors have an array interface")
-        backend, size = self.backend, 4 if dtype == LN_F32 else 2
+        size = 4 if dtype == LN_F32 else 2
         view, *parts = backend._view
         rc = _lib.ln_tensor_device_data(self.h, *parts)
         if rc:
             backend._check(rc)
         data, *shape, n, c, h, w = view[:]
-        self.__cuda_array_interface__ = d = {
-            "shape": tuple(shape), "typestr": "<f4" if size == 4 else "<f2", "data": (data, False), "strides": (size * n, size * c, size * h, size * w),
-            "version": 3, "stream": backend._stream}
-        return d
+        if backend.ctx:
+            rc = _lib.ln_tensor_share(backend.ctx, self.h, None)
+            if rc and STATUS.get(rc) != "unsupported":
+                backend._check(rc)
+        return {"shape": tuple(shape), "typestr": "<f4" if size == 4 else "<f2", "data": (data, False), "strides": (size * n, size * c, size * h, size * w),
+                "version": 3, "stream": backend.stream}
 
 
 class ConvWeights:

@@ -35,6 +35,14 @@ struct ln_ctx {
     std::vector<std::pair<void*, size_t>>* held_blocks = nullptr;
     size_t pool_bytes = 0;                     // bytes held from the device: live + cached
     size_t cached_bytes = 0;
+    // blocks that another stream may still read and that could not be ordered behind it when they were released (a capture was going on)
+    struct late_block {
+        void* p;
+        size_t bytes;
+        std::vector<cudaStream_t> readers;
+    };
+    std::vector<late_block> late_blocks;
+    cudaEvent_t ev_order = nullptr;            // of ln_order_streams, made when it is first needed
     int64_t fail_alloc = 0;                    // test aid: that many allocations from now one fails (ln_debug_fail_alloc)
     int* h_status = nullptr;  // status word in page-locked memory, written by kernels whose bounded waits give up
     ln_encode_tiled_fn encode_tiled = nullptr;
@@ -63,6 +71,7 @@ struct ln_tensor {
     float scale = 1.0f;                  // 8-bit tensors: value = code * scale; LN_F4: value = code * block scale * scale
     void* sf = nullptr;                  // 4-bit tensors: block scales (behind the codes in the same block, order in ln_f4.h)
     int64_t sf_words = 0;                // and their 4-byte words per pixel
+    std::vector<cudaStream_t> readers;   // streams that the memory was shared with (of the owner of the block, not of views)
     int64_t count() const { return n * c * h * w; }
 };
 
@@ -101,6 +110,7 @@ int ln_image_preprocess_into(ln_ctx* ctx, const uint8_t* pixels_host, const int6
                              int32_t count, int32_t mode, int32_t dst_w, int32_t dst_h, float* dst);
 void* ln_pool_alloc(ln_ctx* ctx, size_t bytes);
 void ln_pool_free(ln_ctx* ctx, void* p, size_t bytes);
+int ln_order_streams(ln_ctx* ctx, cudaStream_t first, cudaStream_t then, const char* who);  // what `then` is given next waits for what `first` holds now
 ln_tensor* ln_tensor_new(ln_ctx* ctx, int dtype, int64_t n, int64_t c, int64_t h, int64_t w);  // allocates storage
 ln_tensor* ln_tensor_view_q(ln_tensor* parent, int64_t channel_offset, int64_t channels);      // channel slice of an NHWC tensor
 ln_tensor* ln_tensor_view_batch(ln_tensor* parent, int64_t start, int64_t count);               // image range of an f32 NCHW tensor

@@ -1,6 +1,8 @@
 // Context, device-memory pool and tensor handles of liblightnet_b200.
+#include <algorithm>
 #include <cstdlib>
 #include <cstring>
+#include <exception>
 
 #include "ln_common.h"
 #include "ln_f4.h"
@@ -30,7 +32,65 @@ static void pool_drop_cached(ln_ctx* ctx, std::multimap<size_t, void*>::iterator
     ctx->free_blocks.erase(it);
 }
 
+namespace {
+struct device_guard {  // the ctx's device for a while: these calls also come from a host language's clean-up, in the middle of other work
+    int before = -1;
+    explicit device_guard(const ln_ctx* ctx) {
+        if (cudaGetDevice(&before) != cudaSuccess) before = -1;
+        if (before != ctx->device) cudaSetDevice(ctx->device);
+        else before = -1;
+    }
+    ~device_guard() {
+        if (before >= 0) cudaSetDevice(before);
+    }
+};
+}  // namespace
+
+// Streams of the ctx's device; NULL is its legacy default stream.  LN_ERR_UNSUPPORTED where one of the two is being captured and the other is not
+// part of the same graph: an event between them would break the capture, so nothing is ordered.
+int ln_order_streams(ln_ctx* ctx, cudaStream_t first, cudaStream_t then, const char* who) {
+    if (first == then) return LN_OK;
+    device_guard guard(ctx);
+    cudaStreamCaptureStatus a = cudaStreamCaptureStatusNone, b = cudaStreamCaptureStatusNone;
+    unsigned long long graph_a = 0, graph_b = 0;
+    cudaError_t e = cudaStreamGetCaptureInfo(first, &a, &graph_a);
+    if (e == cudaSuccess) e = cudaStreamGetCaptureInfo(then, &b, &graph_b);
+    if (e == cudaErrorStreamCaptureImplicit || (e == cudaSuccess && (a != b || (a != cudaStreamCaptureStatusNone && (a != cudaStreamCaptureStatusActive || graph_a != graph_b))))) {
+        (void)cudaGetLastError();
+        return ln_fail(ctx, LN_ERR_UNSUPPORTED, "%s: one of the two streams is being captured into a graph that the other is not part of", who);
+    }
+    if (e == cudaSuccess && !ctx->ev_order) e = cudaEventCreateWithFlags(&ctx->ev_order, cudaEventDisableTiming);
+    if (e == cudaSuccess) e = cudaEventRecord(ctx->ev_order, first);
+    if (e == cudaSuccess) e = cudaStreamWaitEvent(then, ctx->ev_order, 0);
+    if (e == cudaSuccess) return LN_OK;
+    (void)cudaGetLastError();
+    return ln_fail(ctx, LN_ERR_CUDA, "%s: %s", who, cudaGetErrorString(e));
+}
+
+// Gives a block back that other streams may still read: what the ctx stream writes there next waits for what they hold now.  Where a capture
+// keeps that from being said now, the block waits for the next allocation outside of one.
+static void pool_free_behind(ln_ctx* ctx, void* p, size_t bytes, std::vector<cudaStream_t>&& readers) {
+    const std::string err = ctx->err;  // (a release has no status: the last error stays that of the last call that has one)
+    while (!readers.empty()) {
+        const int rc = ln_order_streams(ctx, readers.back(), ctx->stream, "release");
+        if (rc == LN_ERR_UNSUPPORTED) break;
+        if (rc != LN_OK) {  // (a stream that no longer exists)
+            device_guard guard(ctx);
+            cudaDeviceSynchronize();
+        }
+        readers.pop_back();
+    }
+    ctx->err = err;
+    if (readers.empty()) ln_pool_free(ctx, p, bytes);
+    else ctx->late_blocks.push_back({p, bytes, std::move(readers)});
+}
+
 void* ln_pool_alloc(ln_ctx* ctx, size_t bytes) {
+    if (!ctx->late_blocks.empty()) {
+        std::vector<ln_ctx::late_block> late;
+        late.swap(ctx->late_blocks);
+        for (auto& b : late) pool_free_behind(ctx, b.p, b.bytes, std::move(b.readers));
+    }
     bytes = (size_t)ln_round_up((int64_t)(bytes ? bytes : 1), 512);
     if (ctx->fail_alloc > 0 && --ctx->fail_alloc == 0) {
         ln_fail(ctx, LN_ERR_CUDA, "cudaMalloc(%zu bytes): refused by ln_debug_fail_alloc", bytes);
@@ -124,6 +184,7 @@ ln_tensor* ln_tensor_view_q(ln_tensor* parent, int64_t channel_offset, int64_t c
     t->bytes = 0;
     t->parent = parent;
     parent->refcount++;
+    t->readers.clear();
     t->c = channels;
     t->ptr = (char*)parent->ptr + channel_offset;
     return t;
@@ -137,6 +198,7 @@ ln_tensor* ln_tensor_view_batch(ln_tensor* parent, int64_t start, int64_t count)
     t->bytes = 0;
     t->parent = parent;
     parent->refcount++;
+    t->readers.clear();
     t->n = count;
     t->ptr = (char*)parent->ptr + (size_t)start * parent->c * parent->h * parent->w * 4;
     return t;
@@ -195,6 +257,8 @@ int32_t ln_ctx_destroy(ln_ctx* ctx) {
     cudaSetDevice(ctx->device);
     cudaStreamSynchronize(ctx->stream);
     for (auto& kv : ctx->free_blocks) cudaFree(kv.second);
+    for (auto& b : ctx->late_blocks) cudaFree(b.p);
+    if (ctx->ev_order) cudaEventDestroy(ctx->ev_order);
     if (ctx->h_status) cudaFreeHost(ctx->h_status);
     if (ctx->h_stage) cudaFreeHost(ctx->h_stage);
     cudaStreamDestroy(ctx->stream);
@@ -318,6 +382,22 @@ int32_t ln_tensor_device_data(const ln_tensor* t, void** data, int64_t shape[4],
     return LN_OK;
 }
 
+int32_t ln_tensor_share(ln_ctx* ctx, ln_tensor* t, void* stream) {
+    const char* who = "ln_tensor_share";
+    if (!ctx || !t) return ln_fail(ctx, LN_ERR_ARG, "%s: NULL argument", who);
+    if (t->ctx != ctx) return ln_fail(ctx, LN_ERR_ARG, "%s: the tensor belongs to another context", who);
+    if ((cudaStream_t)stream == ctx->stream) return LN_OK;
+    while (t->parent) t = t->parent;
+    try {
+        t->readers.reserve(t->readers.size() + 1);
+    } catch (const std::exception&) {
+        return ln_fail(ctx, LN_ERR_CUDA, "%s: host memory exhausted", who);
+    }
+    const int rc = ln_order_streams(ctx, ctx->stream, (cudaStream_t)stream, who);
+    if (rc == LN_OK && std::find(t->readers.begin(), t->readers.end(), (cudaStream_t)stream) == t->readers.end()) t->readers.push_back((cudaStream_t)stream);
+    return rc;
+}
+
 float ln_tensor_scale(const ln_tensor* t) { return t ? t->scale : 0.0f; }
 
 int32_t ln_tensor_retain(ln_tensor* t) {
@@ -329,7 +409,8 @@ int32_t ln_tensor_retain(ln_tensor* t) {
 int32_t ln_tensor_release(ln_tensor* t) {
     if (!t) return LN_OK;
     if (--t->refcount > 0) return LN_OK;
-    if (t->base) ln_pool_free(t->ctx, t->base, t->bytes);
+    if (t->base && !t->readers.empty()) pool_free_behind(t->ctx, t->base, t->bytes, std::move(t->readers));
+    else if (t->base) ln_pool_free(t->ctx, t->base, t->bytes);
     ln_tensor* parent = t->parent;
     delete t;
     if (parent) ln_tensor_release(parent);
