@@ -98,6 +98,12 @@ int32_t ln_tensor_device_data(const ln_tensor* t, void** data, int64_t shape[4],
    has to exist until that release.  A tensor may be shared with several streams.  Nothing waits on the host.  LN_ERR_UNSUPPORTED, and nothing is ordered, where one
    of the two streams is being captured into a graph that the other is not part of. */
 int32_t ln_tensor_share(ln_ctx* ctx, ln_tensor* t, void* stream);
+/* A tensor from f32 or binary16 values (dtype LN_F32 or LN_F16) in memory of the ctx's device: a copy into this library's layout.  strides: the
+   distance in values between neighbours along each axis, of any sign, 0 for an axis that is broadcast.  The copy waits for what `stream`
+   (NULL: the legacy default stream) holds now, and what `stream` is given next waits for the copy; nothing waits on the host.  Values that do not all
+   lie in memory of the ctx's device are refused.  LN_ERR_UNSUPPORTED as for ln_tensor_share. */
+int32_t ln_tensor_from_device(ln_ctx* ctx, const void* data, int32_t dtype, const int64_t shape[4], const int64_t strides[4], void* stream,
+                              ln_tensor** out);
 int32_t ln_tensor_retain(ln_tensor* t);
 int32_t ln_tensor_release(ln_tensor* t);
 

@@ -87,6 +87,7 @@ SYMBOLS = {
     "ln_tensor_dtype": (C.c_int32, [_VP]),
     "ln_tensor_device_data": (C.c_int32, [_VP, _VP, _VP, _VP]),
     "ln_tensor_share": (C.c_int32, [_VP, _VP, _VP]),
+    "ln_tensor_from_device": (C.c_int32, [_VP, _VP, C.c_int32, _I64P, _I64P, _VP, _PP]),
     "ln_tensor_retain": (C.c_int32, [_VP]),
     "ln_tensor_release": (C.c_int32, [_VP]),
     "ln_conv2d_f32": (C.c_int32, [_VP, _VP, _VP, _I64P] + [C.c_int64] * 10 + [_PP]),
@@ -194,6 +195,7 @@ def load_library():
 
 _I64x4 = C.c_int64 * 4
 _byref = C.byref
+_DEVICE_DTYPES = {"<f4": LN_F32, "<f2": LN_F16}
 
 
 def _shape4(shape):
@@ -374,6 +376,25 @@ class B200Backend:
             raise BackendError(1, "host data has %d values for shape %s" % (host.size, tuple(shape)))
         return self._out(self.lib.ln_tensor_upload_f32, _shape4(shape), _ptr(host))
 
+    def from_device(self, array, stream=None):
+        """A tensor from an f32 or binary16 array on the GPU with four dimensions and any strides (anything with `__cuda_array_interface__`, a torch tensor for
+        one): a copy that is ordered behind `stream`, a CUDA stream handle, and in front of that stream's next work.  None: the stream that
+        the array's interface names, or the default stream."""
+        i = array.__cuda_array_interface__
+        dtype = _DEVICE_DTYPES.get(i["typestr"])
+        if dtype is None or i.get("mask") is not None:
+            raise ValueError("f32 or binary16 values without a mask are wanted")
+        shape, strides = i["shape"], i.get("strides")
+        s = _shape4(shape)
+        size = 4 if dtype == LN_F32 else 2
+        if strides is None:
+            strides = (shape[1] * shape[2] * shape[3], shape[2] * shape[3], shape[3], 1)
+        elif any(v % size for v in strides):
+            raise ValueError("strides are whole values")
+        else:
+            strides = [v // size for v in strides]
+        return self._out(self.lib.ln_tensor_from_device, i["data"][0], dtype, s, _I64x4(*strides), i.get("stream") if stream is None else stream)
+
     def zeros_f32(self, shape):
         return self._out(self.lib.ln_tensor_zeros_f32, _shape4(shape))
 
@@ -549,7 +570,10 @@ class B200Backend:
 
     # ---- microscaled 4-bit tensors ----------------------------------------------------------------
     def narrow_f4(self, t, scale=1.0, dtype=LN_F4):
-        """An f32 or binary16 tensor in 4 bits (LN_F4: blocks of 16 with the tensor scale `scale`; LN_MX4: blocks of 32, scale 1)."""
+        """An f32 or binary16 tensor in 4 bits (LN_F4: blocks of 16 with the tensor scale `scale`; LN_MX4: blocks of 32, scale 1).  An array on the
+        GPU is taken by `from_device` first."""
+        if not isinstance(t, Tensor):
+            t = self.from_device(t)
         return self._out(self.lib.ln_tensor_narrow_f4, t.h, float(scale), dtype)
 
     def widen_f4(self, t, dtype=LN_F32):

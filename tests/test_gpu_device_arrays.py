@@ -115,3 +115,129 @@ def test_share_refuses(be):
         other.close()
     with pytest.raises(AttributeError):
         be.narrow_f4(t, 0.5).__cuda_array_interface__
+
+
+LAYOUTS = {
+    "rows": lambda x: x,
+    "channels last": lambda x: x.to(memory_format=torch.channels_last),
+    "every other": lambda x: torch.stack([x, x + 1], -1)[..., 0],
+    "turned": lambda x: x.permute(2, 3, 0, 1).contiguous().permute(2, 3, 0, 1),
+    "columns": lambda x: x.transpose(2, 3).contiguous().transpose(2, 3),
+    "odd start": lambda x: torch.cat([x.flatten()[:1], x.flatten()])[1:].reshape(x.shape),
+}
+
+
+@pytest.mark.parametrize("layout", sorted(LAYOUTS))
+@pytest.mark.parametrize("kind", [torch.float32, torch.float16])
+@pytest.mark.parametrize("shape", [(1, 1, 1, 1), (1, 4096, 1, 1), (3, 40, 7, 9), (130, 33, 1, 1), (2, 65, 13, 1), (1, 129, 1, 66), (5, 1, 64, 65), (2, 257, 19, 23)])
+def test_a_tensor_from_device_memory(be, shape, kind, layout):
+    x = torch.randn(shape, generator=torch.Generator("cuda").manual_seed(sum(shape)), device="cuda").to(kind)
+    v = LAYOUTS[layout](x)
+    assert torch.equal(v, x)
+    t = be.from_device(v)
+    assert t.shape == shape and t.dtype == (ln.LN_F32 if kind == torch.float32 else ln.LN_F16)
+    got = be.download_f32(t) if kind == torch.float32 else be.download_f16(t)
+    assert np.array_equal(got, x.float().cpu().numpy())
+
+
+def test_broadcast_and_backward_strides(be):
+    x = torch.arange(2 * 3 * 4 * 5, dtype=torch.float32, device="cuda").reshape(2, 3, 4, 5)
+    wide = x[:, :1].expand(2, 70, 4, 5)
+    assert np.array_equal(be.download_f32(be.from_device(wide)), wide.cpu().numpy())
+    half = wide.half()[:, :1].expand(2, 70, 4, 5)
+    assert np.array_equal(be.download_f16(be.from_device(half)), wide.cpu().numpy())
+    back = be._out(be.lib.ln_tensor_from_device, x.data_ptr() + 4 * (x.numel() - 1), ln.LN_F32, ln._shape4(x.shape), ln._shape4([-s for s in x.stride()]), None)
+    assert np.array_equal(be.download_f32(back), x.flip(0, 1, 2, 3).cpu().numpy())
+
+
+def test_padding_channels_are_zero(be):
+    """A binary16 convolution over memory that held NaN: the same as over an uploaded tensor."""
+    n, c, h, w, f = 2, 40, 9, 10, 24
+    rng = np.random.default_rng(7)
+    x, wt = rng.normal(0, 1, (n, c, h, w)).astype(np.float16), rng.normal(0, 0.1, (f, c, 3, 3)).astype(np.float32)
+    packed, b = be.conv_weights_f16(be.upload_f32(wt.shape, wt), f, c * 9), be.zeros_f32((1, f, 1, 1))
+
+    def conv(t):
+        return be.download_f16(be.conv2d_bias_act_f16(t, packed, b, (n, f, h, w), c, h, w, f, 3, 1, 1, 1, 1, 1, "leaky"))
+
+    t = be.upload_f16(x.shape, x.astype(np.float32))
+    want, where = conv(t), address(t)
+    del t
+    nan = be.upload_f16((n, 64, h, w), np.full((n, 64, h, w), np.nan, np.float32))
+    assert address(nan) == where
+    del nan
+    t = be.from_device(torch.from_numpy(x).cuda())
+    assert address(t) == where and np.array_equal(conv(t), want)
+
+
+@pytest.mark.parametrize("side", [False, True])
+@pytest.mark.parametrize("kind", [torch.float32, torch.float16])
+def test_the_copy_lies_between_its_neighbours_on_the_stream(be, kind, side):
+    x = torch.zeros(SHAPE, dtype=kind, device="cuda")
+    new = torch.from_numpy(values(8)).cuda().to(kind)
+    torch.cuda.synchronize()
+    stream = torch.cuda.Stream() if side else torch.cuda.current_stream()
+    with torch.cuda.stream(stream):
+        torch.cuda._sleep(SPIN)
+        x.copy_(new)
+        with torch.cuda.stream(torch.cuda.ExternalStream(be.stream)):
+            torch.cuda._sleep(3 * SPIN)
+        t = be.from_device(x, stream.cuda_stream if side else None)
+        x.fill_(7)
+    got = be.download_f32(t) if kind == torch.float32 else be.download_f16(t)
+    assert np.array_equal(got, new.float().cpu().numpy())
+    torch.cuda.synchronize()
+    assert bool((x == 7).all())
+
+
+@pytest.mark.parametrize("dtype", [ln.LN_F4, ln.LN_MX4])
+@pytest.mark.parametrize("kind", [torch.float32, torch.float16])
+def test_narrow_takes_an_array_on_the_gpu(be, kind, dtype):
+    x = torch.from_numpy(np.random.default_rng(9).normal(0, 1, SHAPE).astype(np.float16)).cuda().to(kind)
+    scale = 1.0 if dtype == ln.LN_MX4 else 0.002
+    host = x.float().cpu().numpy()
+    want = be.download_f4(be.narrow_f4(be.upload_f32(SHAPE, host) if kind == torch.float32 else be.upload_f16(SHAPE, host), scale, dtype))
+    got = be.download_f4(be.narrow_f4(x, scale, dtype))
+    assert all(np.array_equal(a, b) for a, b in zip(got, want))
+
+
+def test_from_device_refuses(be):
+    x = torch.zeros(SHAPE, device="cuda")
+    one = ln._shape4((1, 1, 1, 1))
+
+    def take(data=x.data_ptr(), dtype=ln.LN_F32, shape=SHAPE, strides=x.stride()):
+        return be._out(be.lib.ln_tensor_from_device, data, dtype, ln._shape4(shape), ln._shape4(strides), None)
+
+    def refused(kind, **what):
+        with pytest.raises(ln.BackendError) as e:
+            take(**what)
+        assert e.value.kind == kind, str(e.value)
+
+    take()
+    host = np.zeros(SHAPE, np.float32)
+    refused("argument", data=0)
+    refused("argument", data=host.ctypes.data)
+    refused("argument", data=torch.zeros(SHAPE).pin_memory().data_ptr())
+    refused("argument", data=x.data_ptr() + 2)
+    refused("argument", dtype=ln.LN_Q8)
+    refused("argument", dtype=ln.LN_F4)
+    refused("argument", strides=(1 << 36, 1, 1, 1))
+    refused("argument", strides=(-(1 << 36), 1, 1, 1))
+    refused("argument", strides=(1 << 62, 1 << 62, 1 << 62, 1 << 62))
+    refused("shape", shape=(3, 0, 33, 35))
+    refused("shape", shape=(3, -1, 33, 35))
+    refused("shape", shape=(1 << 40, 1, 1, 1), strides=(0, 0, 0, 0))
+    refused("unsupported", shape=(1 << 20, 1 << 20, 1, 1), strides=(0, 0, 0, 0))
+    assert be.lib.ln_tensor_from_device(None, x.data_ptr(), ln.LN_F32, one, one, None, None) == 5
+    with pytest.raises(ValueError):
+        be.from_device(x.double())
+    with pytest.raises(ValueError):
+        be.from_device(x[0])
+    be.debug_fail_alloc(1)
+    refused("cuda")
+    take()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=torch.cuda.ExternalStream(be.stream)):
+        refused("unsupported")
+    del graph
+    take()
