@@ -274,11 +274,6 @@ class _Session:
         return cls.ln, cls.backend
 
 
-def _upload(be, x):
-    host = x.detach().float().cpu().numpy()
-    return be.upload_f16(host.shape, host) if x.dtype == torch.float16 else be.upload_f32(host.shape, host)
-
-
 def _dtype(ln, kind):
     return {"f4": ln.LN_F4, "mx4": ln.LN_MX4, "f32": ln.LN_F32, "f16": ln.LN_F16}[kind]
 
@@ -290,13 +285,13 @@ def _prepare_own(s):
 
     def packed(w, b):
         f, c, k, _ = w.shape
-        return be.conv_weights_f4(_upload(be, w), f, c, k, dtype), _upload(be, b.reshape(1, f, 1, 1))
+        return be.conv_weights_f4(be.from_device(w), f, c, k, dtype), be.from_device(b.reshape(1, f, 1, 1))
 
     own_state = {"case": case, "ln": ln, "be": be, "dtype": dtype, "x_scale": s["x_scale"], "y_scale": s.get("y_scale", 1.0)}
     if case["kind"] in ("narrow", "chain"):
-        own_state["x"] = _upload(be, s["x"])
+        own_state["x"] = s["x"]  # (the array that the plain form takes: the framework's layout of it is made within the call)
     else:
-        own_state["x"] = be.narrow_f4(_upload(be, s["x"]), s["x_scale"], dtype)
+        own_state["x"] = be.narrow_f4(s["x"], s["x_scale"], dtype)
     if case["kind"] == "product":
         own_state["w"] = packed(s["w"], s["b"])
     if case["kind"] == "chain":
