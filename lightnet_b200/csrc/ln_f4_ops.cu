@@ -94,7 +94,7 @@ __global__ void __launch_bounds__(kThreads, 5) narrow_f16_kernel(const __half* _
 #pragma unroll
         for (int b = 0; b < 32 / B; ++b) s |= ln_f4_quantise<FMT>(v + b * B, g, six_g, w + b * B / 8) << (8 * b);
         *reinterpret_cast<uint4*>(codes + (int64_t)pix * cstride + c0 / 2) = make_uint4(w[0], w[1], w[2], w[3]);
-        const uint32_t other = __shfl_down_sync(__activemask(), s, 1);
+        const uint32_t other = __shfl_xor_sync(3u << (threadIdx.x & 30), s, 1);  // (the pair's own mask: blocks take different ways through the quantisation)
         if ((c0 & 32) == 0) {
             uint8_t* dst = sf + ln_f4_sf_at(pix, c0 / (4 * B), sf_words) + c0 / B % 4;
             if (FMT == LN_F4) *reinterpret_cast<uint32_t*>(dst) = s | other << 16;
