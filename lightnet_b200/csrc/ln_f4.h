@@ -120,21 +120,26 @@ __device__ __forceinline__ uint32_t ln_f4_quantise(const float* x, float g, floa
     const uint32_t scale = ln_f4_scale_of<FMT>(amax, six_g);
     float t[B];
     if (FMT == LN_F4) {
-        const float d = ln_f4_factor<FMT>(scale, g);
-        if (scale == 126u) {  // the scale may have saturated: quotients of any size
+        // x / d by one correction of x * (1 / d), three operations instead of a division: the codes are those of the rounded quotient for every
+        // d >= 2^-101 (for all 2^23 significands of d and the x next to each border between codes); below that the correction's remainder loses
+        // bits, so smaller ones are taken 2^64 times as large.  Codes end at 6, so quotients end at 8 where the scale is the largest and they may be of any size
+        // (|x / d| is at most 9 otherwise, at the smallest scale).
+        float d = ln_f4_factor<FMT>(scale, g);
+        if (scale == 126u || __float_as_uint(d) - 1u < 0x0F800000u - 1u) {  // 0 < d < 2^-96
+            const float up = d < 0x1p-96f ? 0x1p64f : 1.0f, most = 8.0f * (d *= up);
 #pragma unroll
-            for (int i = 0; i < B; ++i) t[i] = __fdiv_rn(x[i], d);
+            for (int i = 0; i < B; ++i) t[i] = fminf(fmaxf(__fmul_rn(x[i], up), -most), most);
         } else {
-            // |x / d| < 8 here (or everything is NaN): x / d by one correction of x * (1 / d), three operations instead of a division.
-            // The result is the rounded quotient but where that is within 2^-22 steps of the middle of two numbers.
-            const float r = scale ? __frcp_rn(d) : 0.0f;
 #pragma unroll
-            for (int i = 0; i < B; i += 2) {
-                float q0, q1, e0, e1;
-                fmul2(q0, q1, x[i], x[i + 1], r, r);
-                ffma2(e0, e1, -q0, -q1, d, d, x[i], x[i + 1]);
-                ffma2(t[i], t[i + 1], e0, e1, r, r, q0, q1);
-            }
+            for (int i = 0; i < B; ++i) t[i] = x[i];
+        }
+        const float r = scale ? __frcp_rn(d) : 0.0f;
+#pragma unroll
+        for (int i = 0; i < B; i += 2) {
+            float q0, q1, e0, e1;
+            fmul2(q0, q1, t[i], t[i + 1], r, r);
+            ffma2(e0, e1, -q0, -q1, d, d, t[i], t[i + 1]);
+            ffma2(t[i], t[i + 1], e0, e1, r, r, q0, q1);
         }
     } else {
         const float inv = __uint_as_float((254u - (scale > 253u ? 253u : scale)) << 23);  // 2^-e, exact
