@@ -97,6 +97,22 @@ __device__ __forceinline__ void ln_e2m1x8_to_h2(uint32_t codes, uint32_t (&h)[4]
         : "r"(codes));
 }
 
+// Activations behind a product.  The 8-bit types clamp what goes into exp (their codes cannot show it); these types hold values of the whole range,
+// where v / (1 + e^60) is no longer small.  Below the clamp, swish and mish are v e^v and the logistic e^v to 1e-26 of their value: e^v is the
+// square of e^(v / 2), which is 0 after the clamp of ln_det_expf too.
+template <bool EXACT>
+__host__ __device__ constexpr float ln_f4_far(int act) {  // from here down; -inf for activations that need no exp
+    return act == LN_ACT_MISH || act == LN_ACT_SWISH || act == LN_ACT_LOGISTIC ? (EXACT ? -87.0f : -60.0f) : -__builtin_huge_valf();
+}
+__device__ __forceinline__ float ln_f4_act_far(int act, float v) {
+    const float h = ln_det_expf(0.5f * v);
+    return act == LN_ACT_LOGISTIC ? __fmul_rn(h, h) : __fmul_rn(__fmul_rn(fmaxf(v, -1000.0f), h), h);  // (-inf times 0 is no number)
+}
+template <bool EXACT>
+__device__ __forceinline__ float ln_f4_act(int act, float v) {
+    return v < ln_f4_far<EXACT>(act) ? ln_f4_act_far(act, v) : ln_epilogue_act<EXACT>(act, v);
+}
+
 // Block scale: its stored byte and the binary32 factor d of the codes (g is not used for LN_MX4).
 template <int FMT>
 __device__ __forceinline__ uint32_t ln_f4_scale_of(float amax, float six_g) {

@@ -350,7 +350,7 @@ __global__ void conv_f4_simt_kernel(const simt_params p) {
                 }
             }
         }
-        const float v = ln_epilogue_act<EXACT>(p.act, __fmaf_rn(acc, __fmul_rn(p.xscale, p.wscale[f]), p.bias[f]));
+        const float v = ln_f4_act<EXACT>(p.act, __fmaf_rn(acc, __fmul_rn(p.xscale, p.wscale[f]), p.bias[f]));
         if (p.out_f16) ((__half*)p.y)[pix * p.ys + f] = __float2half_rn(v);
         else ((float*)p.y)[((n * p.F + f) * p.OH + oy) * p.OW + ox] = v;
     }
@@ -464,7 +464,7 @@ __global__ void __launch_bounds__(kFewThreads) conv_f4_few_kernel(const few_para
         float v = 0.0f;
         if (f < p.F) {
             v = __fmaf_rn(sum, FMT == LN_F4 ? __fmul_rn(p.xscale, p.wscale[f]) : 16.0f, p.bias[f]);
-            v = p.exact ? ln_epilogue_act<true>(p.act, v) : ln_epilogue_act<false>(p.act, v);
+            v = p.exact ? ln_f4_act<true>(p.act, v) : ln_f4_act<false>(p.act, v);
         }
         if (p.out_kind == LN_OUT_Q) sums[n][i & 31] = v;
         else if (n < p.pixels) {

@@ -59,3 +59,66 @@ def test_quotients_next_to_a_border_at_the_smallest_scales(be):
             x[0, at, 0, 0] = v * np.where(at % 2, 1, -1)
             scales = same_as_defined(be, x, g, ln.LN_F4, "f32")
             assert (scales == s).all()
+
+
+# shapes [n, c, h, w], kernel and strides that lead to each kernel of the product: up to 16 pixels, tensor cores (flat and under taps, with the k range
+# split over a cluster), every other geometry
+KERNELS = {"few": (3, 64, 1, 1, 1, 1, 1), "flat": (150, 64, 1, 1, 1, 1, 1), "taps": (1, 64, 9, 10, 3, 1, 1), "split": (20, 8192, 1, 1, 1, 1, 1), "any": (1, 64, 6, 7, 3, 1, 2)}
+FAR = [-1e30, -3e38, -1e10, -1000.0, -180.0, -175.0, -174.0, -130.0, -104.0, -103.0, -100.0, -95.0, -90.0, -88.0, -87.5, -87.0, -86.5, -80.0, -61.0, -60.0, -59.5, -30.0,
+       -1.0, -0.0, 0.5, 3.0, 25.0, 100.0, 1e10, 1e30, 3e38, -np.inf, np.inf]
+
+
+def act64(v, act):
+    with np.errstate(all="ignore"):
+        if act == "linear":
+            return v
+        if act == "leaky":
+            return np.maximum(v, f32(0.1) * v)
+        if act == "relu":
+            return np.maximum(v, 0)
+        if act == "logistic":
+            return 1 / (1 + np.exp(-v))
+        limit = np.where(np.isposinf(v), np.inf, -0.0)
+        got = v / (1 + np.exp(-v)) if act == "swish" else v * np.tanh(np.logaddexp(v, 0))
+        return np.where(np.isinf(v), limit, got)
+
+
+def product_of(be, kernel, dtype, act, bias, x=None, out=ln.LN_OUT_F32, wt=None):
+    """A product with given biases: of zeros where there is no x, so that what goes into the activation is the bias itself."""
+    n, c, h, w, k, sx, sy = KERNELS[kernel]
+    f, pad = len(bias), k // 2
+    oh, ow = (h + 2 * pad - k) // sy + 1, (w + 2 * pad - k) // sx + 1
+    x = np.zeros((n, c, h, w), np.float32) if x is None else x
+    wt = np.full((f, c, k, k), 0.01, np.float32) if wt is None else wt
+    q, packed = be.narrow_f4(be.upload_f32(x.shape, x), 1.0, dtype), be.conv_weights_f4(be.upload_f32(wt.shape, wt), f, c, k, dtype)
+    b = be.upload_f32((1, f, 1, 1), np.asarray(bias, np.float32))
+    return be.conv2d_bias_act_f4(q, packed, b, (n, f, oh, ow), c, h, w, f, k, sx, sy, 1, pad, 1, act, 1.0, out)
+
+
+@pytest.mark.parametrize("exact", [False, True])
+@pytest.mark.parametrize("act", sorted(ln.ACTIVATIONS))
+@pytest.mark.parametrize("kernel", sorted(KERNELS))
+def test_activations_of_the_whole_range(be, kernel, act, exact):
+    """Against 64 bits, relative to the value.  The fast exponentials take their argument times log2(e) in binary32: off by up to |v| half steps of 1.45,
+    to -60 (for mish to -87); a few operations more; what is below 2^-126 is off by half a step of 2^-149 times v and up to e^20 more for the ratio of mish."""
+    be.set_exact_epilogue(exact)
+    try:
+        v = np.asarray(FAR, np.float32).astype(np.float64)
+        want = act64(v, act)
+        for dtype in FMT:
+            got = be.download_f32(product_of(be, kernel, dtype, act, FAR)).astype(np.float64)
+            half = be.download_f16(product_of(be, kernel, dtype, act, FAR, out=ln.LN_OUT_F16)).astype(np.float64)
+            for i, (a, r) in enumerate(zip(v, want)):
+                with np.errstate(over="ignore"):
+                    r16 = float(np.float16(r))
+                if not np.isfinite(np.float32(r)):
+                    assert np.array_equal(got[:, i], np.full_like(got[:, i], r)) and np.array_equal(half[:, i], np.full_like(half[:, i], r)), a
+                    continue
+                off = (min(abs(a), 87.0) + 16) * 2.0 ** -23 * abs(r) + 2.0 ** -149 * min(max(abs(a), 2), 200)
+                assert np.max(np.abs(got[:, i] - r)) <= off, (dtype, a, r, got[0, i].ravel()[0])
+                if np.isinf(r16):
+                    assert np.array_equal(half[:, i], np.full_like(half[:, i], r16)), a
+                else:
+                    assert np.max(np.abs(half[:, i] - r)) <= off + 2.0 ** -11 * abs(r) + 2.0 ** -25, (dtype, a)
+    finally:
+        be.set_exact_epilogue(False)
