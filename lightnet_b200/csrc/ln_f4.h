@@ -110,7 +110,9 @@ __device__ __forceinline__ float ln_f4_act_far(int act, float v) {
 }
 template <bool EXACT>
 __device__ __forceinline__ float ln_f4_act(int act, float v) {
-    return v < ln_f4_far<EXACT>(act) ? ln_f4_act_far(act, v) : ln_epilogue_act<EXACT>(act, v);
+    if (act == LN_ACT_RELU) return ln_max_nan(v, 0.0f);
+    const float a = v < ln_f4_far<EXACT>(act) ? ln_f4_act_far(act, v) : ln_epilogue_act<EXACT>(act, v);
+    return v == v ? a : v;  // (a NaN stays one: the clamps of the 8-bit types drop it)
 }
 
 // Block scale: its stored byte and the binary32 factor d of the codes (g is not used for LN_MX4).

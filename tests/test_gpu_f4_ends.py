@@ -122,3 +122,38 @@ def test_activations_of_the_whole_range(be, kernel, act, exact):
                     assert np.max(np.abs(half[:, i] - r)) <= off + 2.0 ** -11 * abs(r) + 2.0 ** -25, (dtype, a)
     finally:
         be.set_exact_epilogue(False)
+
+
+@pytest.mark.parametrize("exact", [False, True])
+@pytest.mark.parametrize("act", sorted(ln.ACTIVATIONS))
+@pytest.mark.parametrize("kernel", sorted(KERNELS))
+def test_nan_behind_every_activation(be, kernel, act, exact):
+    """A NaN bias makes its filter's outputs NaN, a NaN in a pixel those of the pixels that its block reaches, and no others; a block handed on in 4 bits is NaN."""
+    n, c, h, w, k, sx, sy = KERNELS[kernel]
+    f, pad = 70, k // 2
+    rng = np.random.default_rng(5)
+    bias = rng.normal(0, 1, f).astype(np.float32)
+    bias[3] = np.nan
+    x = np.abs(rng.normal(0, 1, (n, c, h, w))).astype(np.float32)
+    x[n // 2, 5, h // 2, w // 2] = np.nan
+    hit = np.zeros((n, h + 2 * pad, w + 2 * pad), bool)
+    hit[n // 2, h // 2 + pad, w // 2 + pad] = True
+    oh, ow = (h + 2 * pad - k) // sy + 1, (w + 2 * pad - k) // sx + 1
+    nan = np.zeros((n, f, oh, ow), bool)
+    for r in range(k):
+        for s in range(k):
+            nan |= hit[:, None, r:r + sy * (oh - 1) + 1:sy, s:s + sx * (ow - 1) + 1:sx]
+    nan[:, 3] = True
+    be.set_exact_epilogue(exact)
+    try:
+        for dtype in FMT:
+            for out, read in ((ln.LN_OUT_F32, be.download_f32), (ln.LN_OUT_F16, be.download_f16)):
+                got = read(product_of(be, kernel, dtype, act, bias, x, out))
+                assert np.array_equal(np.isnan(got), nan), (dtype, out)
+            scales = be.download_f4(product_of(be, kernel, dtype, act, bias, x, ln.LN_OUT_Q))[1]
+            size, none = BLOCK[dtype], 0x7F if dtype == ln.LN_F4 else 0xFF
+            padded = np.zeros((n, -(-f // size) * size, oh, ow), bool)
+            padded[:, :f] = nan
+            assert np.array_equal(scales == none, padded.reshape(n, -1, size, oh, ow).any(2)), dtype
+    finally:
+        be.set_exact_epilogue(False)
