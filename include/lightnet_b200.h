@@ -249,7 +249,8 @@ int32_t ln_tensor_widen_f4(ln_ctx* ctx, const ln_tensor* t, int32_t dtype, ln_te
 /* Codes in NCHW order, one per byte (bit 3 = sign), and block scales [batch, ceil(channels / block), height, width] as they are
    stored (E4M3, or e + 127 with 255 = NaN).  Counts are checked against the tensor's. */
 int32_t ln_tensor_download_f4(ln_ctx* ctx, const ln_tensor* t, uint8_t* host_codes, int64_t code_count, uint8_t* host_scales, int64_t scale_count);
-/* f32 [filters, channels * k * k] weights -> 4 bits; LN_F4: g = max|w| / (6 * 448) per filter.  Released with ln_conv_weights_release. */
+/* f32 [filters, channels * k * k] weights -> 4 bits; LN_F4: g = max|w| / (6 * 448) per filter.  A NaN among a filter's weights makes all of them,
+   and so every output of that filter, NaN.  Released with ln_conv_weights_release. */
 int32_t ln_conv_weights_f4(ln_ctx* ctx, const ln_tensor* weights_f32, int64_t filters, int64_t channels, int64_t kernel_size,
                            int32_t dtype, ln_conv_weights** out);
 /* acc = sum of the products of codes and block scales (binary32 sums), v = fma(acc, x.scale * w.scale[f], bias[f]), a = act(v).

@@ -284,10 +284,12 @@ __global__ void pack_weights_f4_kernel(const float* __restrict__ w, int C, int k
     __syncthreads();
     amax = 0.0f;
     for (int i = 0; i < (int)(blockDim.x >> 5); ++i) amax = ln_max_nan(amax, part[i]);
-    // g stays in the range of tensor scales: 1 for a filter of zeros or with a NaN (whose block is NaN), the end of the range behind it
+    // g stays in the range of tensor scales: 1 for a filter of zeros, the end of the range behind it.  A filter with a NaN is NaN as a whole, scale and
+    // blocks: whether taps outside the image multiply it by zero or are left out then makes no difference.
+    const bool nan = amax != amax;
     float g = 1.0f;
     if (FMT == LN_F4 && amax > 0.0f) g = fminf(fmaxf(__fdiv_rn(amax, 6.0f * 448.0f), 0x1p-100f), 0x1p100f);
-    if (threadIdx.x == 0) wscale[f] = g;
+    if (threadIdx.x == 0) wscale[f] = nan ? amax : g;
     const int blocks = (int)(cstride * 2 / B);
     for (int i = threadIdx.x; i < k2 * blocks; i += blockDim.x) {
         const int tap = i / blocks, b = i - tap * blocks;
@@ -295,7 +297,8 @@ __global__ void pack_weights_f4_kernel(const float* __restrict__ w, int C, int k
 #pragma unroll
         for (int j = 0; j < B; ++j) v[j] = b * B + j < C ? src[(int64_t)(b * B + j) * k2 + tap] : 0.0f;
         const int64_t at = ln_f4_sf_at(f, (int64_t)tap * sf_words + (b >> 2), k2 * sf_words) + (b & 3);
-        sf[at] = (uint8_t)store_block<FMT>(v, g, 6.0f * g, codes + ((int64_t)f * k2 + tap) * cstride + b * (B / 2));
+        const uint32_t scale = store_block<FMT>(v, g, 6.0f * g, codes + ((int64_t)f * k2 + tap) * cstride + b * (B / 2));
+        sf[at] = (uint8_t)(!nan ? scale : (FMT == LN_F4 ? 0x7Fu : 0xFFu));
     }
 }
 

@@ -157,3 +157,28 @@ def test_nan_behind_every_activation(be, kernel, act, exact):
             assert np.array_equal(scales == none, padded.reshape(n, -1, size, oh, ow).any(2)), dtype
     finally:
         be.set_exact_epilogue(False)
+
+
+@pytest.mark.parametrize("kernel", sorted(KERNELS))
+def test_nan_and_infinity_among_the_weights(be, kernel):
+    """A filter with a NaN has no other outputs than NaN, also where the tap that holds it lies outside the image, over an image of zeros, and in every
+    kernel; an infinite weight saturates and makes none; the other filters do not change."""
+    n, c, h, w, k, sx, sy = KERNELS[kernel]
+    f = 40
+    rng = np.random.default_rng(9)
+    wt = rng.normal(0, 0.1, (f, c, k, k)).astype(np.float32)
+    x = rng.normal(0, 1, (n, c, h, w)).astype(np.float32)
+    bad = wt.copy()
+    bad[7, 3, 0, 0] = np.nan
+    bad[33, c - 1, k - 1, k - 1] = np.nan
+    bad[12, 40, 0, 0] = np.inf
+    rest = [i for i in range(f) if i not in (7, 33, 12)]
+    for dtype in FMT:
+        want = be.download_f32(product_of(be, kernel, dtype, "linear", np.ones(f), x, wt=wt))
+        for data in (x, np.zeros_like(x)):
+            got = be.download_f32(product_of(be, kernel, dtype, "linear", np.ones(f), data, wt=bad))
+            assert np.isnan(got[:, [7, 33]]).all()
+            assert not np.isnan(got[:, rest + [12]]).any()
+        assert (got[:, rest + [12]] == 1).all()
+        got = be.download_f32(product_of(be, kernel, dtype, "linear", np.ones(f), x, wt=bad))
+        assert np.array_equal(got[:, rest], want[:, rest])
