@@ -307,22 +307,25 @@ struct simt_params {
     const uint8_t *x, *xsf, *w, *wsf;
     const float *wscale, *bias;
     void* y;
-    int64_t xs, xsf_words, ys, total;
-    int C, H, W, F, k, sx, sy, pad, OH, OW, blocks, act, out_f16;
-    float xscale;
+    uint8_t* ysf;
+    int64_t xs, xsf_words, ys, ysf_words, total;
+    int H, W, F, fpad, k, sx, sy, pad, OH, OW, blocks, act, out_kind;  // fpad: filters as they are counted, F, or for a 4-bit output its padded channels
+    float xscale, g, six_g;
 };
-// One thread per output value, filters fastest.  Takes every geometry.
+// One thread per output value, filters fastest.  Takes every geometry.  A 4-bit output's channels are padded to 64, so that a warp is 32 filters of
+// one pixel; the first lane of each block collects its values (a tensor between this kernel and a narrow would be memory that a
+// caller who captures the call cannot keep for the replays).
 template <int FMT, bool EXACT>
 __global__ void conv_f4_simt_kernel(const simt_params p) {
     ln_f4_after_predecessor();
     constexpr int B = FMT == LN_F4 ? 16 : 32;
     for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < p.total; i += (int64_t)gridDim.x * blockDim.x) {
-        const int f = (int)(i % p.F);
-        const int64_t pix = i / p.F;
+        const int f = (int)(i % p.fpad);
+        const int64_t pix = i / p.fpad;
         const int ox = (int)(pix % p.OW), oy = (int)(pix / p.OW % p.OH);
         const int64_t n = pix / p.OW / p.OH;
         float acc = 0.0f;
-        for (int r = 0; r < p.k; ++r) {
+        for (int r = 0; r < p.k && f < p.F; ++r) {
             const int yy = oy * p.sy - p.pad + r;
             if (yy < 0 || yy >= p.H) continue;
             for (int s = 0; s < p.k; ++s) {
@@ -353,8 +356,14 @@ __global__ void conv_f4_simt_kernel(const simt_params p) {
                 }
             }
         }
-        const float v = ln_f4_act<EXACT>(p.act, __fmaf_rn(acc, __fmul_rn(p.xscale, p.wscale[f]), p.bias[f]));
-        if (p.out_f16) ((__half*)p.y)[pix * p.ys + f] = __float2half_rn(v);
+        const float v = f < p.F ? ln_f4_act<EXACT>(p.act, __fmaf_rn(acc, __fmul_rn(p.xscale, p.wscale[f]), p.bias[f])) : 0.0f;
+        if (p.out_kind == LN_OUT_Q) {
+            const int lane = threadIdx.x & 31;
+            float b[B];
+#pragma unroll
+            for (int j = 0; j < B; ++j) b[j] = __shfl_sync(0xFFFFFFFFu, v, (lane & ~(B - 1)) + j);
+            if (lane % B == 0) p.ysf[ln_f4_sf_at(pix, f / (4 * B), p.ysf_words) + f / B % 4] = (uint8_t)store_block<FMT>(b, p.g, p.six_g, (uint8_t*)p.y + pix * p.ys + f / 2);
+        } else if (p.out_kind == LN_OUT_F16) ((__half*)p.y)[pix * p.ys + f] = __float2half_rn(v);
         else ((float*)p.y)[((n * p.F + f) * p.OH + oy) * p.OW + ox] = v;
     }
 }
@@ -683,7 +692,7 @@ int32_t ln_conv2d_bias_act_f4(ln_ctx* ctx, const ln_tensor* x, const ln_conv_wei
     if (rc) return rc;
     return guarded(ctx, who, [&]() -> int32_t {
         cudaSetDevice(ctx->device);
-        ln_tensor *y = nullptr, *wide = nullptr;
+        ln_tensor* y = nullptr;
         int rc = new_tensor(ctx, out_kind == LN_OUT_Q ? x->dtype : (out_kind == LN_OUT_F16 ? LN_F16 : LN_F32), x->n, filters, oh, ow, &y);
         ln_f4_conv c;
         c.dtype = x->dtype; c.x = x; c.w = weights; c.bias = (const float*)bias->ptr; c.y = y;
@@ -696,20 +705,19 @@ int32_t ln_conv2d_bias_act_f4(ln_ctx* ctx, const ln_tensor* x, const ln_conv_wei
             *out = y;
             return LN_OK;
         }
-        if (rc == LN_OK && out_kind == LN_OUT_Q) rc = new_tensor(ctx, LN_F32, x->n, filters, oh, ow, &wide);
         if (rc == LN_OK && y->dtype == LN_F16 && y->cstride != 2 * filters) {
             const cudaError_t e = cudaMemsetAsync(y->ptr, 0, y->bytes, ctx->stream);
             if (e != cudaSuccess) rc = ln_fail(ctx, LN_ERR_CUDA, "%s: %s", who, cudaGetErrorString(e));
         }
         if (rc == LN_OK) {
-            const ln_tensor* dst = wide ? wide : y;
             simt_params p;
             p.x = (const uint8_t*)x->ptr; p.xsf = (const uint8_t*)x->sf; p.w = (const uint8_t*)weights->w; p.wsf = (const uint8_t*)weights->sf;
-            p.wscale = weights->wscale; p.bias = (const float*)bias->ptr; p.y = dst->ptr;
-            p.xs = x->cstride; p.xsf_words = x->sf_words; p.ys = dst->cstride / 2; p.total = x->n * oh * ow * filters;
-            p.C = (int)channels; p.H = (int)input_height; p.W = (int)input_width; p.F = (int)filters; p.k = (int)kernel_size; p.sx = (int)stride_x; p.sy = (int)stride_y; p.pad = (int)padding;
+            p.wscale = weights->wscale; p.bias = (const float*)bias->ptr; p.y = y->ptr; p.ysf = (uint8_t*)y->sf;
+            p.xs = x->cstride; p.xsf_words = x->sf_words; p.ys = out_kind == LN_OUT_F16 ? y->cstride / 2 : y->cstride; p.ysf_words = y->sf_words;
+            p.fpad = out_kind == LN_OUT_Q ? (int)ln_round_up(filters, 64) : (int)filters; p.total = x->n * oh * ow * p.fpad;
+            p.H = (int)input_height; p.W = (int)input_width; p.F = (int)filters; p.k = (int)kernel_size; p.sx = (int)stride_x; p.sy = (int)stride_y; p.pad = (int)padding;
             p.OH = (int)oh; p.OW = (int)ow; p.blocks = (int)(x->cstride * 2 / ln_f4_block(x->dtype));
-            p.act = activation; p.out_f16 = dst->dtype == LN_F16; p.xscale = x->scale;
+            p.act = activation; p.out_kind = out_kind; p.xscale = x->scale; p.g = y->scale; p.six_g = 6.0f * y->scale;
             const int grid = grid_for(ctx, p.total);
             cudaError_t e;
             if (x->dtype == LN_F4) {
@@ -720,9 +728,7 @@ int32_t ln_conv2d_bias_act_f4(ln_ctx* ctx, const ln_tensor* x, const ln_conv_wei
                 else e = ln_f4_launch(ctx, conv_f4_simt_kernel<LN_MX4, false>, grid, kThreads, 0, p);
             }
             rc = check_launch(ctx, who, e);
-            if (rc == LN_OK && wide) rc = narrow_into(ctx, wide, y);
         }
-        if (wide) ln_tensor_release(wide);
         if (rc) { if (y) ln_tensor_release(y); return rc; }
         *out = y;
         return LN_OK;

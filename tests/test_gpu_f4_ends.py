@@ -182,3 +182,38 @@ def test_nan_and_infinity_among_the_weights(be, kernel):
         assert (got[:, rest + [12]] == 1).all()
         got = be.download_f32(product_of(be, kernel, dtype, "linear", np.ones(f), x, wt=bad))
         assert np.array_equal(got[:, rest], want[:, rest])
+
+
+@pytest.mark.parametrize("kernel", sorted(KERNELS))
+def test_a_replay_writes_no_memory_but_its_tensors(kernel):
+    """A captured product that hands 4 bits on: with its tensors kept, a replay leaves what later calls put elsewhere."""
+    torch = pytest.importorskip("torch")
+    be = ln.B200Backend(0)
+    n, c, h, w, k, sx, sy = KERNELS[kernel]
+    f, pad = 70, k // 2
+    oh, ow = (h + 2 * pad - k) // sy + 1, (w + 2 * pad - k) // sx + 1
+    rng = np.random.default_rng(3)
+    try:
+        for dtype in FMT:
+            wt = rng.normal(0, 0.1, (f, c, k, k)).astype(np.float32)
+            x, packed, b = be.upload_f32((n, c, h, w), rng.normal(0, 1, (n, c, h, w))), be.conv_weights_f4(be.upload_f32(wt.shape, wt), f, c, k, dtype), be.zeros_f32((1, f, 1, 1))
+
+            def call():
+                q = be.narrow_f4(x, 1.0, dtype)
+                return q, be.conv2d_bias_act_f4(q, packed, b, (n, f, oh, ow), c, h, w, f, k, sx, sy, 1, pad, 1, "mish", 1.0, ln.LN_OUT_Q)
+
+            want = be.download_f4(call()[1])
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=torch.cuda.ExternalStream(be.stream)):
+                kept = call()
+            others, value = [], np.full((n, f, oh, ow), 7.0, np.float32)
+            for size in (value, value[:, : f // 4], value[:, : f // 8]):
+                others += [be.upload_f32(size.shape, size) for _ in range(4)]
+            with torch.cuda.stream(torch.cuda.ExternalStream(be.stream)):
+                graph.replay()
+            be.sync()
+            assert all((be.download_f32(t) == 7).all() for t in others)
+            assert all(np.array_equal(a, r) for a, r in zip(be.download_f4(kept[1]), want))
+            del graph, kept
+    finally:
+        be.close()
