@@ -199,6 +199,7 @@ _DEVICE_DTYPES = {"<f4": LN_F32, "<f2": LN_F16}
 
 
 def _shape4(shape):
+    shape = tuple(shape)
     if len(shape) != 4:
         raise ValueError("shapes are [batch, channels, height, width]")
     try:

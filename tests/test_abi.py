@@ -62,3 +62,14 @@ def test_product_does_not_touch_the_oracle():
                 if f.endswith((".py", ".cu", ".h", ".cpp", ".cuh")):
                     text = open(os.path.join(dirpath, f)).read()
                     assert "oracle" not in text.lower(), os.path.join(dirpath, f)
+
+
+def test_shapes_are_any_iterable_of_four_numbers():
+    """Tuples, lists, arrays, generators, maps; numbers of other types count as int() takes them."""
+    import numpy as np
+
+    for shape in ((2, 3, 4, 5), [2, 3, 4, 5], np.array([2, 3, 4, 5]), np.array([2.0, 3.0, 4.0, 5.0]), (v for v in (2, 3, 4, 5)), map(int, "2345"), (np.int32(2), 3.0, "4", 5)):
+        assert list(ln._shape4(shape)) == [2, 3, 4, 5]
+    for shape in ((), (1, 2, 3), (v for v in range(5)), np.zeros((4, 1))[:3]):
+        with pytest.raises(ValueError):
+            ln._shape4(shape)
