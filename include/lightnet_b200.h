@@ -458,6 +458,9 @@ int32_t ln_debug_mma_peak_shape(ln_ctx* ctx, int32_t dtype, int32_t n, int32_t p
 int32_t ln_ctx_debug_cycles(ln_ctx* ctx, int64_t cycles[32]);
 /* The n-th request for device memory that the ctx makes from now on fails, once, as if the device had none left (0 = none does). */
 int32_t ln_debug_fail_alloc(ln_ctx* ctx, int64_t n);
+/* The last 4-bit product on the tensor cores: filters of a tile, of the units that the last round of tiles was cut into (0: not cut), CTAs that share a
+   tile's k range.  Zeros where the product ran in another kernel. */
+int32_t ln_debug_f4_plan(const ln_ctx* ctx, int32_t plan[3]);
 /* Forwards of the network so far whose layers were one launch of a captured graph (8-bit and binary16; the others ran kernel by kernel). */
 int64_t ln_debug_net_replays(const ln_net* net);
 

@@ -168,6 +168,7 @@ SYMBOLS = {
     "ln_conv2d_bias_act_f4": (C.c_int32, [_VP, _VP, _VP, _VP, _I64P] + [C.c_int64] * 10 + [C.c_int32, C.c_float, C.c_int32, _PP]),
     "ln_debug_score_key_error": (C.c_int32, [_VP, C.c_float, C.c_float, C.c_float, C.c_float, C.c_int32, C.c_int32, C.POINTER(C.c_uint32)]),
     "ln_ctx_debug_cycles": (C.c_int32, [_VP, _I64P]),
+    "ln_debug_f4_plan": (C.c_int32, [_VP, C.POINTER(C.c_int32)]),
     "ln_debug_net_replays": (C.c_int64, [_VP]),
     "ln_debug_fail_alloc": (C.c_int32, [_VP, C.c_int64]),
     "ln_modern_yolo_forward_f32": (C.c_int32, [_VP, _VP, C.c_int64, _VP]),
@@ -598,6 +599,12 @@ class B200Backend:
         return self._out(self.lib.ln_conv2d_bias_act_f4, x.h, weights.h, bias.h, _shape4(output_shape), channels, input_height,
                          input_width, filters, kernel_size, stride_x, stride_y, dilation, padding, groups, _act(activation),
                          float(y_scale), out_kind)
+
+    def debug_f4_plan(self):
+        """(filters of a tile, of the last round's units or 0, CTAs per tile) of the last 4-bit product on the tensor cores; zeros for another kernel."""
+        plan = (C.c_int32 * 3)()
+        self._check(self.lib.ln_debug_f4_plan(self.ctx, plan))
+        return tuple(plan)
 
     # ---- [yolo] decode + NMS ---------------------------------------------------------------------
     @staticmethod

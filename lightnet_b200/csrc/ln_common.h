@@ -43,6 +43,7 @@ struct ln_ctx {
     };
     std::vector<late_block> late_blocks;
     cudaEvent_t ev_order = nullptr;            // of ln_order_streams, made when it is first needed
+    int32_t f4_plan[3] = {0, 0, 0};            // of the last 4-bit product (ln_debug_f4_plan)
     int64_t fail_alloc = 0;                    // test aid: that many allocations from now one fails (ln_debug_fail_alloc)
     int* h_status = nullptr;  // status word in page-locked memory, written by kernels whose bounded waits give up
     ln_encode_tiled_fn encode_tiled = nullptr;

@@ -690,6 +690,7 @@ int32_t ln_conv2d_bias_act_f4(ln_ctx* ctx, const ln_tensor* x, const ln_conv_wei
     if (input_height > (1 << 24) || input_width > (1 << 24)) return ln_fail(ctx, LN_ERR_UNSUPPORTED, "%s: more than 2^24 rows or columns", who);
     int rc = ln_status(ctx, who);  // of an earlier call
     if (rc) return rc;
+    ctx->f4_plan[0] = ctx->f4_plan[1] = ctx->f4_plan[2] = 0;
     return guarded(ctx, who, [&]() -> int32_t {
         cudaSetDevice(ctx->device);
         ln_tensor* y = nullptr;

@@ -848,5 +848,8 @@ int ln_f4_umma_launch(ln_ctx* ctx, const ln_f4_conv& c) {
         (void)cudaGetLastError();
         return ln_fail(ctx, LN_ERR_CUDA, "%s: launch failed: %s", who, cudaGetErrorString(e));
     }
+    ctx->f4_plan[0] = p.bn;
+    ctx->f4_plan[1] = cut ? p.narrow : 0;
+    ctx->f4_plan[2] = parts;
     return LN_OK;
 }

@@ -293,6 +293,13 @@ int32_t ln_debug_fail_alloc(ln_ctx* ctx, int64_t n) {
     return LN_OK;
 }
 
+// Debug aid: what the last 4-bit product ran as.
+int32_t ln_debug_f4_plan(const ln_ctx* ctx, int32_t plan[3]) {
+    if (!ctx || !plan) return LN_ERR_ARG;
+    memcpy(plan, ctx->f4_plan, sizeof ctx->f4_plan);
+    return LN_OK;
+}
+
 int32_t ln_ctx_set_exact_epilogue(ln_ctx* ctx, int32_t on) {
     if (!ctx) return LN_ERR_ARG;
     ctx->exact_epilogue = on != 0;

@@ -217,3 +217,36 @@ def test_a_replay_writes_no_memory_but_its_tensors(kernel):
             del graph, kept
     finally:
         be.close()
+
+
+@pytest.mark.parametrize("tile", ["64", "128", "256", "128/64", "256/128", "256/64", "64*2", "128*4"])
+def test_a_forced_tile_runs_where_it_can(be, monkeypatch, tile):
+    """Sizes that each form of the tensor-core kernel takes: a cut last round wants more tiles than the 148 SMs and a last round whose units fit into one (76 x 2
+    or 51 x 3 tiles: 4 and 5 behind the first round), a split wants few tiles and a long k range.  What ran is asked for: the form in two cases at least, and the
+    outputs of the choice by size in all."""
+    filters, narrow, parts = int(tile.split("/")[0].split("*")[0]), int(tile.split("/")[1]) if "/" in tile else 0, int(tile.split("*")[1]) if "*" in tile else 1
+    rng, taken, rows = np.random.default_rng(2), 0, 76 if filters == 256 else 51
+    cases = [(1, 70, 150, 147, 264, 3), (19000, 200, 1, 1, 258, 1), (1, 70, rows, 128, 264, 3), (rows * 128, 200, 1, 1, 264, 1)]
+    for n, c, h, w, f, k in [(1, 320, 31, 33, 264, 3), (40, 2112, 1, 1, 257, 1)] if parts > 1 else cases:
+        x, wt = rng.normal(0, 1, (n, c, h, w)).astype(np.float32), rng.normal(0, 0.05, (f, c, k, k)).astype(np.float32)
+        for dtype in FMT:
+            q, packed, b = be.narrow_f4(be.upload_f32(x.shape, x), 1.0, dtype), be.conv_weights_f4(be.upload_f32(wt.shape, wt), f, c, k, dtype), be.zeros_f32((1, f, 1, 1))
+
+            def call():
+                return be.download_f32(be.conv2d_bias_act_f4(q, packed, b, (n, f, h, w), c, h, w, f, k, 1, 1, 1, k // 2, 1, "linear", 1.0, ln.LN_OUT_F32))
+
+            monkeypatch.setenv("LN_F4_BN", tile)
+            got, ran = call(), be.debug_f4_plan()
+            monkeypatch.delenv("LN_F4_BN")
+            want = call()
+            taken += ran == (filters, narrow, parts)
+            assert np.max(np.abs(got - want)) <= 2.0 ** -20 * np.abs(want).max()
+    assert taken >= 2 * len(FMT), taken
+
+
+def test_which_kernel_a_size_runs_in(be):
+    for kernel, tiles in (("few", False), ("any", False), ("flat", True), ("taps", True), ("split", True)):
+        product_of(be, kernel, ln.LN_F4, "linear", np.zeros(70))
+        filters, _, parts = be.debug_f4_plan()
+        assert (filters > 0) == tiles and (parts > 1) == (kernel == "split"), kernel
+    assert be.lib.ln_debug_f4_plan(None, None) == 5
