@@ -236,7 +236,7 @@ int32_t ln_channel_affine_act_f16(ln_ctx* ctx, const ln_tensor* x, const ln_tens
    Elements are E2M1: 0, 0.5, 1, 1.5, 2, 3, 4, 6 and a sign.  A block is consecutive channels of one pixel (of one tap of one filter
    for weights) that share a scale:
      LN_F4   16 channels, block scale s in E4M3, and one f32 scale g per tensor (ln_tensor_scale; per filter for weights):
-             s = e4m3(amax / (6 g)), d = s * g, code = e2m1(x / d), value = code * d.  s = 0 gives codes 0.
+             s = e4m3(amax / (6 g)), d = s * g, code = e2m1(x / d), value = code * d.  s = 0 gives zeros of the values' signs.
              g = amax / (6 * 448) of a calibration run uses the whole range of s.
      LN_MX4  32 channels, block scale d = 2^e, e = max(floor(log2(amax)) - 2, -127), code = e2m1(x / d), value = code * d (the
              ranges of the OCP microscaling format).  There is no other scale: `scale` arguments have to be 1.

@@ -250,3 +250,22 @@ def test_which_kernel_a_size_runs_in(be):
         filters, _, parts = be.debug_f4_plan()
         assert (filters > 0) == tiles and (parts > 1) == (kernel == "split"), kernel
     assert be.lib.ln_debug_f4_plan(None, None) == 5
+
+
+@pytest.mark.parametrize("source", ["f32", "f16"])
+def test_the_smallest_block_scales(be, source):
+    """amax / (6 g) around 2^-10, where the scale becomes 0, and in the middle between two of the smallest scales, where |x / d| is up to 9: one block for each,
+    with values of both signs down to nothing beside the largest."""
+    at = [0.0, 2.0 ** -12, 0.999 * 2.0 ** -10, 2.0 ** -10, 1.001 * 2.0 ** -10] + [m * 2.0 ** -9 for m in (0.75, 1, 1.49, 1.5, 1.51, 2, 2.49, 2.5, 2.51, 3.5, 6.5, 7.4, 7.5, 7.6, 8.5)]
+    x = np.zeros((2, 16 * len(at), 3, 1), np.float32)
+    part = np.array([1, -1, 0.97, -0.9, 0.8, -0.7, 0.6, 0.5, -0.4, 0.3, 0.2, -0.1, 0.05, -0.01, 0.0, -0.0])
+    for i, q in enumerate(at):
+        x[:, 16 * i:16 * i + 16] = (6 * q * part).reshape(1, 16, 1, 1)
+    if source == "f16":
+        x = (x * 64).astype(np.float16).astype(np.float32)
+    scales = same_as_defined(be, x, 64.0 if source == "f16" else 1.0, ln.LN_F4, source)
+    assert (scales[:, :3] == 0).all() and (scales[:, 4] == 1).all() and scales.max() == 8
+    q = be.narrow_f4(be.upload_f32(x.shape, x), 64.0 if source == "f16" else 1.0)
+    codes = be.download_f4(q)[0]
+    assert set(np.unique(codes[:, :48])) <= {0, 8}  # zeros of either sign
+    assert not np.isnan(be.download_f32(be.widen_f4(q))).any()
