@@ -51,6 +51,9 @@ __device__ __forceinline__ void ln_f4_after_predecessor() {
     asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
+__device__ __forceinline__ void ln_store_32(void* dst, const uint32_t (&v)[8]) {  // a whole sector
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
+}
 // max that hands a NaN on
 __device__ __forceinline__ float ln_max_nan(float a, float b) {
     float r;

@@ -11,9 +11,6 @@ namespace {
 
 constexpr int kThreads = 256;
 
-__device__ __forceinline__ void ln_store_32(void* dst, const uint32_t (&v)[8]) {  // a whole sector
-    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
-}
 // 16 bytes that are read once
 __device__ __forceinline__ uint4 ln_ldg_stream(const __half* p) { return __ldcs(reinterpret_cast<const uint4*>(p)); }
 

@@ -185,9 +185,6 @@ __device__ __forceinline__ void act_all(float (&v)[W]) {
 }
 __device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[16]) { tmem_ld_32x16(taddr, r); tmem_ld_wait(); }
 __device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[32]) { tmem_ld_32x32(taddr, r); tmem_ld_wait(); }
-__device__ __forceinline__ void store_32(uint8_t* dst, const uint32_t (&v)[8]) {  // a whole sector
-    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
-}
 // what a unit is: pixels and filters, and the output box's origin
 struct f4_unit {
     int pixel_tile, f0;
@@ -357,7 +354,7 @@ __device__ __forceinline__ void f4_epilogue(const f4_params& p, const f4_epilogu
 #pragma unroll
                         for (int i = 0; i < W; i += 8) {
                             const uint32_t (&h)[8] = *reinterpret_cast<const uint32_t(*)[8]>(v + i);
-                            if (valid && f + i < p.F) store_32((uint8_t*)(dst + i), h);
+                            if (valid && f + i < p.F) ln_store_32(dst + i, h);
                         }
                         continue;
                     }
@@ -388,7 +385,7 @@ __device__ __forceinline__ void f4_epilogue(const f4_params& p, const f4_epilogu
                     const __half2 q = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
                     h[i] = *reinterpret_cast<const uint32_t*>(&q);
                 }
-                if (valid) store_32((uint8_t*)p.y + (long long)pix * p.ys + 2 * f, h);
+                if (valid) ln_store_32((uint8_t*)p.y + (long long)pix * p.ys + 2 * f, h);
             } else {
                 uint32_t q[W / 8];
                 const uint32_t sf = ln_f4_quantise<FMT>(v, p.g, p.six_g, q);
