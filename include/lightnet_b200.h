@@ -259,7 +259,8 @@ int32_t ln_conv_weights_f4(ln_ctx* ctx, const ln_tensor* weights_f32, int64_t fi
    call gives the same bits, an image alone and in a batch the same values to rounding.)
    LN_OUT_F32 stores a in NCHW, LN_OUT_F16 in binary16 NHWC, LN_OUT_Q narrows a to the input's 4-bit type again with y_scale.
    A 1x1 convolution of [tokens, channels, 1, 1] is the matrix product of tokens and weights.  groups and dilation must be 1.
-   The call does not wait for the GPU: should the kernel give up a wait, ln_sync, a download or the next 4-bit call returns LN_ERR_TIMEOUT. */
+   The call does not wait for the GPU: should the kernel give up a wait, ln_sync, a download or the next 4-bit
+   product returns LN_ERR_TIMEOUT, once. */
 int32_t ln_conv2d_bias_act_f4(ln_ctx* ctx, const ln_tensor* x, const ln_conv_weights* weights, const ln_tensor* bias,
                               const int64_t output_shape[4], int64_t channels, int64_t input_height, int64_t input_width,
                               int64_t filters, int64_t kernel_size, int64_t stride_x, int64_t stride_y, int64_t dilation,
@@ -458,6 +459,8 @@ int32_t ln_debug_mma_peak_shape(ln_ctx* ctx, int32_t dtype, int32_t n, int32_t p
 int32_t ln_ctx_debug_cycles(ln_ctx* ctx, int64_t cycles[32]);
 /* The n-th request for device memory that the ctx makes from now on fails, once, as if the device had none left (0 = none does). */
 int32_t ln_debug_fail_alloc(ln_ctx* ctx, int64_t n);
+/* Test aid: the status word as a kernel leaves it that gave a wait up (1: TMA producer, 2: MMA issuer, 3: epilogue). */
+int32_t ln_debug_set_status(ln_ctx* ctx, int32_t status);
 /* The last 4-bit product on the tensor cores: filters of a tile, of the units that the last round of tiles was cut into (0: not cut), CTAs that share a
    tile's k range.  Zeros where the product ran in another kernel. */
 int32_t ln_debug_f4_plan(const ln_ctx* ctx, int32_t plan[3]);

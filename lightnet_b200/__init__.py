@@ -168,6 +168,7 @@ SYMBOLS = {
     "ln_conv2d_bias_act_f4": (C.c_int32, [_VP, _VP, _VP, _VP, _I64P] + [C.c_int64] * 10 + [C.c_int32, C.c_float, C.c_int32, _PP]),
     "ln_debug_score_key_error": (C.c_int32, [_VP, C.c_float, C.c_float, C.c_float, C.c_float, C.c_int32, C.c_int32, C.POINTER(C.c_uint32)]),
     "ln_ctx_debug_cycles": (C.c_int32, [_VP, _I64P]),
+    "ln_debug_set_status": (C.c_int32, [_VP, C.c_int32]),
     "ln_debug_f4_plan": (C.c_int32, [_VP, C.POINTER(C.c_int32)]),
     "ln_debug_net_replays": (C.c_int64, [_VP]),
     "ln_debug_fail_alloc": (C.c_int32, [_VP, C.c_int64]),

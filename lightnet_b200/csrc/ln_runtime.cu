@@ -5,6 +5,7 @@
 #include <exception>
 
 #include "ln_common.h"
+#include "ln_conv_plan.h"
 #include "ln_f4.h"
 
 static thread_local std::string g_create_error;
@@ -290,6 +291,13 @@ int32_t ln_ctx_debug_cycles(ln_ctx* ctx, int64_t cycles[32]) {
 int32_t ln_debug_fail_alloc(ln_ctx* ctx, int64_t n) {
     if (!ctx || n < 0) return ln_fail(ctx, LN_ERR_ARG, "ln_debug_fail_alloc: n must not be negative");
     ctx->fail_alloc = n;
+    return LN_OK;
+}
+
+// Test aid: what a kernel that gave a wait up leaves for the host.
+int32_t ln_debug_set_status(ln_ctx* ctx, int32_t status) {
+    if (!ctx || status < 0 || status > 3) return ln_fail(ctx, LN_ERR_ARG, "ln_debug_set_status: a status of 0 to 3 is wanted");
+    *(volatile int*)ctx->h_status = status ? LN_STATUS_PRODUCER_TIMEOUT + status - 1 : LN_STATUS_OK;
     return LN_OK;
 }
 

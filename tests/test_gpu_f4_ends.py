@@ -269,3 +269,24 @@ def test_the_smallest_block_scales(be, source):
     codes = be.download_f4(q)[0]
     assert set(np.unique(codes[:, :48])) <= {0, 8}  # zeros of either sign
     assert not np.isnan(be.download_f32(be.widen_f4(q))).any()
+
+
+@pytest.mark.parametrize("status", [1, 2, 3])
+def test_a_wait_given_up_is_reported_once(be, status):
+    """The word that such a kernel leaves in host memory: the next product, a download or ln_sync says so, and the context goes on."""
+    x = np.random.default_rng(1).normal(0, 1, (1, 64, 9, 9)).astype(np.float32)
+
+    def product():
+        return product_of(be, "taps", ln.LN_F4, "leaky", np.ones(40), np.broadcast_to(x[:, :, :, :1], (1, 64, 9, 10)))
+
+    want = be.download_f32(product())
+    y, q = product(), be.narrow_f4(be.upload_f32(x.shape, x), 0.01)
+    be.sync()
+    for call in (product, be.sync, lambda: be.download_f32(y), lambda: be.download_f16(be.widen_f4(q, ln.LN_F16)), lambda: be.download_f4(q)):
+        assert be.lib.ln_debug_set_status(be.ctx, status) == 0
+        with pytest.raises(ln.BackendError) as e:
+            call()
+        assert e.value.kind == "timeout" and ("TMA producer", "MMA issuer", "epilogue")[status - 1] in str(e.value)
+        call()
+        assert np.array_equal(be.download_f32(product()), want)
+    assert be.lib.ln_debug_set_status(be.ctx, 4) == be.lib.ln_debug_set_status(None, 0) == 5
