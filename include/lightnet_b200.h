@@ -95,8 +95,9 @@ int32_t ln_tensor_dtype(const ln_tensor* t);
 int32_t ln_tensor_device_data(const ln_tensor* t, void** data, int64_t shape[4], int64_t strides[4]);
 /* Lets work on another stream of the ctx's device read a tensor (NULL: the legacy default stream): what `stream` is given from here on waits for
    what the ctx stream holds now, and once the last handle is gone the memory is used again only behind what `stream` holds then.  The stream
-   has to exist until that release.  A tensor may be shared with several streams.  Nothing waits on the host.  LN_ERR_UNSUPPORTED, and nothing is ordered, where one
-   of the two streams is being captured into a graph that the other is not part of. */
+   has to exist until that release.  (A network's own tensors: until its next forward, which waits for the stream and writes them again.)
+   A tensor may be shared with several streams.  Nothing waits on the host.  LN_ERR_UNSUPPORTED, and nothing is ordered, where one of the
+   two streams is being captured into a graph that the other is not part of. */
 int32_t ln_tensor_share(ln_ctx* ctx, ln_tensor* t, void* stream);
 /* A tensor from f32 or binary16 values (dtype LN_F32 or LN_F16) in memory of the ctx's device: a copy into this library's layout.  strides: the
    distance in values between neighbours along each axis, of any sign, 0 for an axis that is broadcast.  The copy waits for what `stream`

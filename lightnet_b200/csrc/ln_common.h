@@ -111,6 +111,7 @@ int ln_image_preprocess_into(ln_ctx* ctx, const uint8_t* pixels_host, const int6
                              int32_t count, int32_t mode, int32_t dst_w, int32_t dst_h, float* dst);
 void* ln_pool_alloc(ln_ctx* ctx, size_t bytes);
 void ln_pool_free(ln_ctx* ctx, void* p, size_t bytes);
+int ln_tensor_wait_readers(ln_ctx* ctx, ln_tensor* t, const char* who);  // in front of work that writes a tensor in place: behind the streams that it was shared with
 int ln_order_streams(ln_ctx* ctx, cudaStream_t first, cudaStream_t then, const char* who);  // what `then` is given next waits for what `first` holds now
 ln_tensor* ln_tensor_new(ln_ctx* ctx, int dtype, int64_t n, int64_t c, int64_t h, int64_t w);  // allocates storage
 ln_tensor* ln_tensor_view_q(ln_tensor* parent, int64_t channel_offset, int64_t channels);      // channel slice of an NHWC tensor

@@ -1150,8 +1150,12 @@ int forward_any(ln_net* net, const ln_tensor* input, cudaEvent_t* around = nullp
     if (!input || input->dtype != LN_F32 || input->n != net->batch || input->c != net->channels || input->h != net->height || input->w != net->width)
         return ln_fail(ctx, LN_ERR_SHAPE, "input tensor must be f32 [%d,%d,%d,%d]", net->batch, net->channels, net->height, net->width);
     cudaSetDevice(ctx->device);
+    int rc = LN_OK;
+    // tensors that this forward writes again, the heads and what a graph holds: behind streams that they were shared with
+    for (size_t k = 0; k < net->heads.size() && rc == LN_OK; ++k) rc = ln_tensor_wait_readers(ctx, net->heads[k], "ln_net_forward");
+    for (size_t k = 0; k < net->graph_f16.refs.size() && rc == LN_OK; ++k) rc = ln_tensor_wait_readers(ctx, net->graph_f16.refs[k].first, "ln_net_forward");
+    if (rc) return rc;
     if (around) LN_CUDA(ctx, cudaEventRecord(around[0], ctx->stream));
-    int rc;
     if (net->precision == LN_F32) rc = forward_f32(net, input, nullptr);
     else if (net->precision == LN_F16) rc = forward_f16(net, input);
     else {

@@ -68,6 +68,16 @@ int ln_order_streams(ln_ctx* ctx, cudaStream_t first, cudaStream_t then, const c
     return ln_fail(ctx, LN_ERR_CUDA, "%s: %s", who, cudaGetErrorString(e));
 }
 
+int ln_tensor_wait_readers(ln_ctx* ctx, ln_tensor* t, const char* who) {
+    while (t->parent) t = t->parent;
+    while (!t->readers.empty()) {  // (what they are to read of the new contents is shared again)
+        const int rc = ln_order_streams(ctx, t->readers.back(), ctx->stream, who);
+        if (rc) return rc;
+        t->readers.pop_back();
+    }
+    return LN_OK;
+}
+
 // Gives a block back that other streams may still read: what the ctx stream writes there next waits for what they hold now.  Where a capture
 // keeps that from being said now, the block waits for the next allocation outside of one.
 static void pool_free_behind(ln_ctx* ctx, void* p, size_t bytes, std::vector<cudaStream_t>&& readers) {

@@ -241,3 +241,33 @@ def test_from_device_refuses(be):
         refused("unsupported")
     del graph
     take()
+
+
+@pytest.mark.parametrize("precision", [ln.LN_F32, ln.LN_F16, ln.LN_Q8])
+def test_a_forward_waits_for_readers_of_the_last_one(be, precision):
+    """Heads and layers that a network writes in place, eager and replayed: what another stream still reads is the forward that it asked about."""
+    from lightnet_b200 import synth, zoo
+    net, other = [ln.GpuExecutableNetwork(be, zoo.yolov3_tiny_cfg(160, 96), 2, precision) for _ in range(2)]
+    blob = synth.he_weights(net.layers(), 3)
+    images = [synth.uniform_images(2, 3, 96, 160, s) for s in range(6)]
+    for n in (net, other):
+        n.load_weights(blob)
+        if precision == ln.LN_Q8:
+            n.calibrate(images[0])
+    want = []
+    for x in images:
+        other.forward(x)
+        want.append([be.download_f32(other.head(k)) for k in range(other.num_heads())])
+    read = []
+    for x in images:
+        net.forward(x)
+        views = [torch.as_tensor(net.head(k), device="cuda") for k in range(net.num_heads())]
+        torch.cuda._sleep(SPIN)
+        read.append([v.clone() for v in views])
+        del views
+    torch.cuda.synchronize()
+    if precision != ln.LN_F32:
+        assert net.debug_replays() >= 3
+    for got, ref in zip(read, want):
+        assert all(np.array_equal(a.cpu().numpy(), b) for a, b in zip(got, ref))
+    del net, other
