@@ -65,8 +65,10 @@ __global__ void __launch_bounds__(kThreads, 5) narrow_f16_kernel(const __half* _
     ln_f4_after_predecessor();
     constexpr int B = FMT == LN_F4 ? 16 : 32;
     const I total = (I)(pixels * groups), step = (I)(gridDim.x * blockDim.x);
-    for (I i = (I)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += step) {  // (total is even: the lanes of a pair leave together)
-        const I pix = i / (I)groups;
+    const int lane = threadIdx.x & 31;
+    for (I first = (I)blockIdx.x * blockDim.x + (threadIdx.x & ~31); first < total; first += step) {  // (whole warps, for the exchange)
+        const bool real = first + lane < total;
+        const I i = real ? first + lane : total - 1, pix = i / (I)groups;
         const int c0 = (int)(i - pix * (I)groups) * 32;
         uint4 q[4];
 #pragma unroll
@@ -90,8 +92,9 @@ __global__ void __launch_bounds__(kThreads, 5) narrow_f16_kernel(const __half* _
         uint32_t w[4], s = 0;
 #pragma unroll
         for (int b = 0; b < 32 / B; ++b) s |= ln_f4_quantise<FMT>(v + b * B, g, six_g, w + b * B / 8) << (8 * b);
+        const uint32_t other = __shfl_down_sync(0xFFFFFFFFu, s, 1);  // (blocks take different ways through the quantisation: all lanes are named)
+        if (!real) continue;
         *reinterpret_cast<uint4*>(codes + (int64_t)pix * cstride + c0 / 2) = make_uint4(w[0], w[1], w[2], w[3]);
-        const uint32_t other = __shfl_xor_sync(3u << (threadIdx.x & 30), s, 1);  // (the pair's own mask: blocks take different ways through the quantisation)
         if ((c0 & 32) == 0) {
             uint8_t* dst = sf + ln_f4_sf_at(pix, c0 / (4 * B), sf_words) + c0 / B % 4;
             if (FMT == LN_F4) *reinterpret_cast<uint32_t*>(dst) = s | other << 16;
