@@ -728,8 +728,8 @@ int ln_f4_umma_launch(ln_ctx* ctx, const ln_f4_conv& c) {
     p.log_tw = log2_of(p.TW); p.log_th = log2_of(p.TH);
     // filter tile
     // A launch takes about start + (k-blocks of a tile + (rounds - 1) x the longer of k-blocks and epilogue), rounds = tiles per SM, in ns
-    // as measured over 27 shapes of both types with binary16 output (leaky), 3 to 76 us, each with every tile; the choice was the best one or
-    // within 4 % of it on all of them.  Where most SMs have nothing to do, a k-block of 256 filters comes faster.
+    // as measured over 28 shapes of both types with binary16 output (leaky), 4 to 65 us, each with every tile; the choice was the best one or
+    // within 3 % of it on all of them.  Where most SMs have nothing to do, a k-block of 256 filters comes faster.
     // The tiles of the last, partly filled round may be cut into units of fewer filters, where those fit into one round.  Where all tiles
     // leave SMs idle, the k range may be split over a cluster, which costs 3.1 us more (launch, two barriers, exchange; 4.3 where most SMs take part): worth it from about
     // 20 k-blocks on (128 x 11008 -> 4096, LN_F4: 16.8 us, split over four 11.4; 3x3 C1024->K512 at 13x13: 14.9 and 10.2).
