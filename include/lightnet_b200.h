@@ -256,9 +256,10 @@ int32_t ln_conv_weights_f4(ln_ctx* ctx, const ln_tensor* weights_f32, int64_t fi
                            int32_t dtype, ln_conv_weights** out);
 /* acc = sum of the products of codes and block scales (binary32 sums), v = fma(acc, x.scale * w.scale[f], bias[f]), a = act(v).
    (The product of the two scales is a binary32 number: where they are so large or so small together that it leaves 2^-126 .. 2^128,
-   that filter's results are infinite or NaN, or lose bits.  Activations hold for every v: infinities give their limits, a NaN gives NaN.  The order of the sums depends on the number of pixels in the call: the same
-   call gives the same bits, an image alone and in a batch the same values to rounding; in a 4-bit output such a last bit is a whole step
-   where the value lies at a border between two codes or two scales.)
+   that filter's results are infinite or NaN, or lose bits.  Activations hold for every v: infinities give their limits, a NaN gives NaN.
+   The order of the sums depends on the number of pixels in the call: the same call gives the same bits, an image alone and in a batch the
+   same values to rounding; in a 4-bit output such a last bit is a whole step where the value lies at a border between two codes or two
+   scales.)
    LN_OUT_F32 stores a in NCHW, LN_OUT_F16 in binary16 NHWC, LN_OUT_Q narrows a to the input's 4-bit type again with y_scale.
    A 1x1 convolution of [tokens, channels, 1, 1] is the matrix product of tokens and weights.  groups and dilation must be 1.
    The call does not wait for the GPU: should the kernel give up a wait, ln_sync, a download or the next 4-bit

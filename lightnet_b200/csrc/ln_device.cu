@@ -3,8 +3,8 @@
 // A copy into the framework's layout, f32 NCHW or binary16 NHWC with channels padded to 32: what it moves is the bytes in and out once.  Source
 // and destination may run along different axes, so a block of threads takes 64 pixels x 64 channels through shared memory, reads along
 // the axis on which the source is denser and writes along the one on which the destination is.  A thread has its 16 reads in flight before it
-// stores the first (64 x 128 x 76 x 76 binary16 NCHW, 189 MB in and out: 47 us; with bounds
-// checked for every value, which issued in 77 % of the cycles, 62, with four reads in flight and scalar stores 120).
+// stores the first (64 x 128 x 76 x 76 binary16 NCHW, 189 MB in and out: 47 us; with bounds checked for every value, which issued in 77 % of the
+// cycles, 62, with four reads in flight and scalar stores 120).
 #include <exception>
 
 #include "ln_common.h"

@@ -1151,8 +1151,8 @@ int forward_any(ln_net* net, const ln_tensor* input, cudaEvent_t* around = nullp
         return ln_fail(ctx, LN_ERR_SHAPE, "input tensor must be f32 [%d,%d,%d,%d]", net->batch, net->channels, net->height, net->width);
     cudaSetDevice(ctx->device);
     int rc = LN_OK;
-    // tensors that this forward writes again, the heads and what a graph holds: behind streams that they were shared with
-    for (size_t k = 0; k < net->heads.size() && rc == LN_OK; ++k) rc = ln_tensor_wait_readers(ctx, net->heads[k], "ln_net_forward");
+    // tensors that this forward writes again, the heads and what a graph holds: behind streams that they were shared with (f32 ones are new every time)
+    for (size_t k = 0; net->precision != LN_F32 && k < net->heads.size() && rc == LN_OK; ++k) rc = ln_tensor_wait_readers(ctx, net->heads[k], "ln_net_forward");
     for (size_t k = 0; k < net->graph_f16.refs.size() && rc == LN_OK; ++k) rc = ln_tensor_wait_readers(ctx, net->graph_f16.refs[k].first, "ln_net_forward");
     if (rc) return rc;
     if (around) LN_CUDA(ctx, cudaEventRecord(around[0], ctx->stream));

@@ -68,31 +68,33 @@ int ln_order_streams(ln_ctx* ctx, cudaStream_t first, cudaStream_t then, const c
     return ln_fail(ctx, LN_ERR_CUDA, "%s: %s", who, cudaGetErrorString(e));
 }
 
-int ln_tensor_wait_readers(ln_ctx* ctx, ln_tensor* t, const char* who) {
-    while (t->parent) t = t->parent;
-    while (!t->readers.empty()) {  // (what they are to read of the new contents is shared again)
-        const int rc = ln_order_streams(ctx, t->readers.back(), ctx->stream, who);
-        if (rc) return rc;
-        t->readers.pop_back();
+// The ctx stream behind all readers, which are struck off.  One that no longer exists is waited for on the host, with all the device.
+// LN_ERR_UNSUPPORTED, and those that are left, where a capture keeps one from being ordered.
+static int wait_readers(ln_ctx* ctx, std::vector<cudaStream_t>& readers, const char* who) {
+    while (!readers.empty()) {
+        const int rc = ln_order_streams(ctx, readers.back(), ctx->stream, who);
+        if (rc == LN_ERR_UNSUPPORTED) return rc;
+        if (rc != LN_OK) {
+            device_guard guard(ctx);
+            cudaDeviceSynchronize();
+        }
+        readers.pop_back();
     }
     return LN_OK;
+}
+
+int ln_tensor_wait_readers(ln_ctx* ctx, ln_tensor* t, const char* who) {
+    while (t->parent) t = t->parent;
+    return wait_readers(ctx, t->readers, who);  // (what they are to read of the new contents is shared again)
 }
 
 // Gives a block back that other streams may still read: what the ctx stream writes there next waits for what they hold now.  Where a capture
 // keeps that from being said now, the block waits for the next allocation outside of one.
 static void pool_free_behind(ln_ctx* ctx, void* p, size_t bytes, std::vector<cudaStream_t>&& readers) {
     const std::string err = ctx->err;  // (a release has no status: the last error stays that of the last call that has one)
-    while (!readers.empty()) {
-        const int rc = ln_order_streams(ctx, readers.back(), ctx->stream, "release");
-        if (rc == LN_ERR_UNSUPPORTED) break;
-        if (rc != LN_OK) {  // (a stream that no longer exists)
-            device_guard guard(ctx);
-            cudaDeviceSynchronize();
-        }
-        readers.pop_back();
-    }
+    const int rc = wait_readers(ctx, readers, "release");
     ctx->err = err;
-    if (readers.empty()) ln_pool_free(ctx, p, bytes);
+    if (rc == LN_OK) ln_pool_free(ctx, p, bytes);
     else ctx->late_blocks.push_back({p, bytes, std::move(readers)});
 }
 

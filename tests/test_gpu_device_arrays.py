@@ -271,3 +271,29 @@ def test_a_forward_waits_for_readers_of_the_last_one(be, precision):
     for got, ref in zip(read, want):
         assert all(np.array_equal(a.cpu().numpy(), b) for a, b in zip(got, ref))
     del net, other
+
+
+def test_a_shared_f32_network_can_be_captured(be):
+    """The forward of an f32 network makes its outputs anew, so heads that another stream may still read do not stand in the way of a capture."""
+    from lightnet_b200 import synth, zoo
+    net = ln.GpuExecutableNetwork(be, zoo.yolov3_tiny_cfg(160, 96), 1)
+    net.load_weights(synth.he_weights(net.layers(), 3))
+    x = synth.uniform_images(1, 3, 96, 160, 1)
+    t = be.upload_f32(x.shape, x)
+    held = []
+    for _ in range(4):
+        be._check(be.lib.ln_net_forward_device(net.h, t.h))
+        held.append([torch.as_tensor(net.head(k), device="cuda") for k in range(net.num_heads())])
+    want = [be.download_f32(net.head(k)) for k in range(net.num_heads())]
+    views = held.pop()
+    del held  # (memory for the forward that is captured)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=torch.cuda.ExternalStream(be.stream)):
+        be._check(be.lib.ln_net_forward_device(net.h, t.h))
+    heads = [net.head(k) for k in range(net.num_heads())]
+    with torch.cuda.stream(torch.cuda.ExternalStream(be.stream)):
+        graph.replay()
+    be.sync()
+    for h, v, r in zip(heads, views, want):
+        assert np.array_equal(be.download_f32(h), r) and np.array_equal(v.cpu().numpy(), r)
+    del graph
